@@ -164,6 +164,14 @@ _SIGNATURES = {
     "ce_rowx_wait": [_vp, _vp],
     "ce_rowx_put": [_vp, _vp],
     "ce_rowx_close": [_vp],
+    "ce_paged_resize": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp],
+    "ce_paged_append": [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _i, _vp, _i, _vp],
+    "ce_paged_attention_workspace": [ctypes.POINTER(ctypes.c_size_t)],
+    "ce_paged_attention": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _f, _vp, ctypes.c_size_t, _vp],
+    "ce_beam_workspace": [_i, _i, _i, ctypes.POINTER(ctypes.c_size_t)],
+    "ce_beam_select": [_vp, _vp, _vp, _vp, _vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp, ctypes.c_size_t,
+                       _vp],
+    "ce_paged_reorder": [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp],
 }
 _RESTYPES = {"ce_version": ctypes.c_char_p}
 
@@ -991,3 +999,205 @@ def llama_shard_rows(cfg, rank, world, which):
     out = np.empty(n.value, np.int32)
     check(lib().ce_llama_shard_rows(ctypes.byref(c), rank, world, which, out.ctypes.data, ctypes.byref(n)))
     return out
+
+
+# --------------------------------------------------------------------------
+# Paged key-value cache and beam search (ce_paged_*, ce_beam_*)
+
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_E4M3 = 0, 1, 2, 3
+_TYPES = {}  # torch dtype -> CE_TYPE_*, filled on first use
+
+
+class _PagedKVStruct(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] +
+                [(n, ctypes.c_int32) for n in ("type", "layers", "pages", "kv_heads", "page_size", "head_dim")] +
+                [(n, _i64) for n in ("layer_stride", "page_stride", "head_stride", "token_stride")])
+
+
+class _PageTableStruct(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("table", "lens", "refs")] +
+                [(n, ctypes.c_int32) for n in ("seqs", "max_pages", "pages", "page_size")])
+
+
+def _type(t, what):
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16,
+                       torch.float8_e4m3fn: TYPE_E4M3})
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype}")
+    return code
+
+
+def _dense(t, name, dtype, count=None):
+    """Pointer of a contiguous device tensor of `dtype` with `count` elements (None: NULL)."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype or not t.is_cuda or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} device tensor (got {t.dtype}, {t.device})")
+    if count is not None and t.numel() != count:
+        raise ValueError(f"{name} must have {count} elements (got {t.numel()})")
+    return t.data_ptr()
+
+
+def _heads_of(t, name, tokens, heads, dim):
+    """(pointer, token stride) of a [tokens][heads][dim] tensor whose heads are contiguous."""
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or t.shape[2] != dim or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor [{tokens}][{heads}][{dim}] (got {tuple(t.shape)})")
+    ld, sh, sd = t.stride()
+    if (sd != 1 and dim > 1) or (sh != dim and heads > 1):
+        raise ValueError(f"{name}: the heads of a token must be contiguous (strides {t.stride()})")
+    return t.data_ptr(), ld if tokens > 1 else max(ld, heads * dim)
+
+
+class PagedKV:
+    """Pools of keys and values: k, v device tensors
+    [layers][pages][kv_heads][page_size][head_dim] of bfloat16, float16 or
+    float8_e4m3fn with the same strides (token-major pages are a permuted
+    view); k_scale, v_scale float32 [kv_heads] for an 8-bit cache. Holds the
+    attention workspace: calls of paged_attention on one PagedKV must be
+    ordered (one stream), or pass a workspace of their own
+    (paged_attention_workspace)."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise ValueError("k and v must be [layers][pages][kv_heads][page_size][head_dim] of one type and layout")
+        if not (k.is_cuda and v.is_cuda) or (k.stride(4) != 1 and k.shape[4] > 1):
+            raise ValueError("k and v must be device tensors with contiguous head rows")
+        L, P, H, S, D = k.shape
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = L, P, H, S, D
+        st = k.stride()
+        self._c = _PagedKVStruct(k.data_ptr(), v.data_ptr(), _dense(k_scale, "k_scale", "torch.float32", H),
+                                 _dense(v_scale, "v_scale", "torch.float32", H), _type(k, "cache"), L, P, H, S, D,
+                                 st[0], st[1], st[2], st[3])
+        self._p = ctypes.addressof(self._c)
+        self._ws = None
+
+    def workspace(self):
+        if self._ws is None:
+            self._ws = paged_attention_workspace(self.k.device)
+        return self._ws
+
+
+class PageTable:
+    """Block tables: table int32 [seqs][max_pages], lens int32 [seqs], refs
+    int32 [pages] (rows that hold each page; 0 = free)."""
+
+    def __init__(self, table, lens, refs, page_size):
+        if table.dim() != 2:
+            raise ValueError(f"table must be [seqs][max_pages] (got {tuple(table.shape)})")
+        n, P = table.shape
+        self.table, self.lens, self.refs, self.page_size = table, lens, refs, page_size
+        self.seqs, self.max_pages, self.pages = n, P, refs.numel()
+        self._c = _PageTableStruct(_dense(table, "table", "torch.int32"), _dense(lens, "lens", "torch.int32", n),
+                                   _dense(refs, "refs", "torch.int32"), n, P, refs.numel(), page_size)
+        self._p = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, seqs, max_pages, pages, page_size, device="cuda"):
+        """No request holds a page."""
+        import torch
+        z = [torch.zeros(s, dtype=torch.int32, device=device) for s in ((seqs, max_pages), (seqs,), (pages,))]
+        return cls(*z, page_size)
+
+
+def paged_resize(pt, new_lens, slots, pos, starts=None, status=None, out=None, stream=None):
+    """Gives every request of pt its new length (int32 [seqs]; negative: as it
+    is): pages, slots (int64 [capacity]) and pos (int32 [capacity]) of the new
+    tokens; in place, or into the PageTable `out` (ce_paged_resize)."""
+    out = pt if out is None else out
+    cap = slots.numel()
+    check(lib().ce_paged_resize(out._p, pt._p, _dense(new_lens, "new_lens", "torch.int32", pt.seqs),
+                                _dense(slots, "slots", "torch.int64"), _dense(pos, "pos", "torch.int32", cap), cap,
+                                _dense(starts, "starts", "torch.int32", pt.seqs + 1),
+                                _dense(status, "status", "torch.int32", 4), _stream(stream)))
+
+
+def paged_append(kv, q_out, q, k, v, slots, pos=None, rope=None, layer=0, stream=None):
+    """Rotary positions on q [tokens][heads][dim] and k, then k and v
+    [tokens][kv_heads][dim] into their slots of `layer`; rope float32
+    [positions][dim / 2][2] of (cos, sin), or None (ce_paged_append)."""
+    T, D = slots.numel(), kv.head_dim
+    kp, k_ld = _heads_of(k, "k", T, kv.kv_heads, D)
+    vp, v_ld = _heads_of(v, "v", T, kv.kv_heads, D)
+    qp, q_ld, qo, qt, heads = None, 0, None, TYPE_BF16, 0
+    if q is not None:
+        heads = q.shape[1]
+        qp, q_ld = _heads_of(q, "q", T, heads, D)
+        qo, qt = _dense(q_out, "q_out", str(q_out.dtype), T * heads * D), _type(q_out, "q_out")
+    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError("q, k and v must have one dtype")
+    if rope is not None and (rope.dim() != 3 or rope.shape[1] * 2 != D or rope.shape[2] != 2):
+        raise ValueError(f"rope must be [positions][{D // 2}][2] (got {tuple(rope.shape)})")
+    check(lib().ce_paged_append(kv._p, layer, qo, qt, qp, kp, vp, _type(k, "k"), q_ld, k_ld, v_ld,
+                                _dense(slots, "slots", "torch.int64"), _dense(pos, "pos", "torch.int32", T), T, heads,
+                                _dense(rope, "rope", "torch.float32"), 0 if rope is None else rope.shape[0],
+                                _stream(stream)))
+    return q_out
+
+
+def paged_attention_workspace(device="cuda"):
+    """A zeroed workspace (uint8 device tensor) of paged_attention."""
+    import torch
+    n = ctypes.c_size_t()
+    check(lib().ce_paged_attention_workspace(ctypes.byref(n)))
+    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+
+
+def paged_attention(kv, out, q, pt, lse=None, scale=None, layer=0, workspace=None, stream=None):
+    """Attention of one new token per request of pt over its pages: q, out
+    [seqs][heads][dim], lse float32 [seqs][heads]; scale 1 / sqrt(dim) unless
+    given (ce_paged_attention)."""
+    n, D = pt.seqs, kv.head_dim
+    heads = q.shape[1]
+    qp, q_ld = _heads_of(q, "q", n, heads, D)
+    op, o_ld = _heads_of(out, "out", n, heads, D)
+    if q.dtype != out.dtype:
+        raise TypeError("q and out must have one dtype")
+    ws = kv.workspace() if workspace is None else workspace
+    check(lib().ce_paged_attention(kv._p, layer, pt._p, op, _dense(lse, "lse", "torch.float32", n * heads), qp,
+                                   _type(q, "q"), heads, q_ld, o_ld, D ** -0.5 if scale is None else scale,
+                                   ws.data_ptr(), ws.numel(), _stream(stream)))
+    return out
+
+
+def beam_workspace(batch, beams, vocab, device="cuda"):
+    """A zeroed workspace (uint8 device tensor) of beam_select."""
+    import torch
+    n = ctypes.c_size_t()
+    check(lib().ce_beam_workspace(batch, beams, vocab, ctypes.byref(n)))
+    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+
+
+def beam_select(scores_out, parents, tokens, finished_out, logits, scores, finished, eos, pad, workspace, stream=None):
+    """One selection of a beam search: logits [batch * beams][vocab], scores
+    float32 and finished bool [batch][beams]; into scores_out, parents and
+    tokens (int32) and finished_out (bool), all [batch][beams]
+    (ce_beam_select). eos -1: no token ends a beam."""
+    B, K = scores.shape
+    n, V = B * K, logits.shape[1]
+    if logits.dim() != 2 or logits.shape[0] != n or not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits must be a device tensor [{n}][vocab] with contiguous rows (got {tuple(logits.shape)})")
+    check(lib().ce_beam_select(_dense(scores_out, "scores_out", "torch.float32", n),
+                               _dense(parents, "parents", "torch.int32", n), _dense(tokens, "tokens", "torch.int32", n),
+                               _dense(finished_out, "finished_out", "torch.bool", n), logits.data_ptr(),
+                               _type(logits, "logits"), logits.stride(0) if n > 1 else max(V, logits.stride(0)),
+                               _dense(scores, "scores", "torch.float32"),
+                               _dense(finished, "finished", "torch.bool", n), B, K, V, eos, pad, workspace.data_ptr(),
+                               workspace.numel(), _stream(stream)))
+
+
+def paged_reorder(pt, parents, beams, out, kv=None, copies=None, status=None, stream=None):
+    """Row i of `out` (a PageTable with a table of its own) becomes the row of
+    pt that parents[i] (int32 [seqs], in 0 .. beams - 1) names in its group of
+    `beams`; partly filled last pages that rows share are copied in kv
+    (ce_paged_reorder). Returns copies int32 [seqs][2]."""
+    if copies is None:
+        import torch
+        copies = torch.empty(pt.seqs, 2, dtype=torch.int32, device=pt.table.device)
+    check(lib().ce_paged_reorder(out._p, pt._p, _dense(parents, "parents", "torch.int32", pt.seqs), beams,
+                                 None if kv is None else kv._p, _dense(copies, "copies", "torch.int32", 2 * pt.seqs),
+                                 _dense(status, "status", "torch.int32", 4), _stream(stream)))
+    return copies

@@ -52,6 +52,8 @@ int gemm_status();
 int gemm_bs_status();
 int rowx_status();
 int rows_status();
+int paged_status();
+int paged_attention_status();
 int rows_set_wait_limit(unsigned long long ns);
 int rows_set_streaming(int on);
 int gemm_set_wait_limit(unsigned long long ns);
@@ -213,13 +215,17 @@ int ce_device_info(int *sms, int *sm100) {
 }
 
 // Synchronizes the device and returns CE_ERR_TIMEOUT if a bounded device
-// wait of a tensor-core kernel gave up since the last call (clearing it).
+// wait of a tensor-core kernel gave up since the last call, CE_ERR_USAGE if a
+// paged operator met a slot, position, page or length out of range (clearing
+// either).
 int ce_device_status(void) {
   const int a = gemm_status();
   const int b = gemm_bs_status();
   const int c = rowx_status();
   const int d = rows_status();
-  return a != CE_OK ? a : b != CE_OK ? b : c != CE_OK ? c : d;
+  const int e = paged_status();
+  const int f = paged_attention_status();
+  return a != CE_OK ? a : b != CE_OK ? b : c != CE_OK ? c : d != CE_OK ? d : e != CE_OK ? e : f;
 }
 
 int ce_set_wait_limit(double seconds) {

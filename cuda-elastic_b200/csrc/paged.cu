@@ -1,0 +1,724 @@
+// Block tables and cache writes of the paged key-value cache: resize
+// (request lengths -> pages, slots, positions), append (rotary positions and
+// the cache write) and reorder (rows follow their beam search parents).
+//
+// Page allocation needs no free list: a page is free when no row holds it
+// (refs 0), and the i-th page that a call takes is the i-th lowest free one.
+// So the answer depends on the inputs alone, never on the order in which
+// threads arrive: counts of references are sums of integers, and ranks among
+// free pages and among rows are prefix sums.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace ce {
+namespace paged {
+namespace {
+
+__device__ DeviceStatus g_paged_status;
+
+constexpr int kTableThreads = 1024;
+
+// ---------------------------------------------------------------------------
+// Pieces that resize and reorder share
+
+struct Tables {
+  const int32_t *table_in, *lens_in, *refs_in;
+  int32_t *table, *lens, *refs;
+  int32_t *status;
+  int n, max_pages, pages, shift;  // rows, columns, pool, log2(page_size)
+};
+
+__device__ __forceinline__ int pages_of(int len, int shift) {
+  return (int)(((long long)len + (1 << shift) - 1) >> shift);
+}
+
+// A length as the tables can hold it (a caller's mistake is cut, not followed).
+__device__ __forceinline__ int held_len(const Tables &t, int i) {
+  const long long top = (long long)t.max_pages << t.shift;
+  const int len = t.lens_in[i];
+  if (len < 0 || len > top) {
+    report_timeout(&g_paged_status, kSiteLen);
+    return len < 0 ? 0 : (int)(top < 0x7fffffff ? top : 0x7fffffff);
+  }
+  return len;
+}
+
+__device__ __forceinline__ bool page_ok(const Tables &t, int page) {
+  if ((unsigned)page < (unsigned)t.pages) return true;
+  report_timeout(&g_paged_status, kSitePage);
+  return false;
+}
+
+// This CTA's share [lo, hi) of the pages (a multiple of 32 pages each, so
+// that a word of the free map belongs to one CTA).
+struct Share {
+  int lo, hi;
+};
+__device__ __forceinline__ Share page_share(int pages, int rank, int ranks) {
+  const int per = ((pages + ranks - 1) / ranks + 31) / 32 * 32;
+  const int lo = min(pages, rank * per);
+  return {lo, min(pages, lo + per)};
+}
+
+// Free map of the CTA's share: bit p of word w is set when page lo + 32 w + p
+// has no holder. Returns the number of free pages (same value in all threads).
+__device__ __forceinline__ int map_free(const Tables &t, Share sh, uint32_t *map, int *scratch) {
+  const int lane = threadIdx.x & 31;
+  int mine = 0;
+  for (int p = sh.lo + (int)threadIdx.x; p - lane < sh.hi; p += blockDim.x) {
+    const bool free = p < sh.hi && __ldcg(t.refs + p) == 0;
+    const uint32_t word = __ballot_sync(0xffffffffu, free);
+    if (lane == 0) {
+      map[(p - sh.lo) >> 5] = word;
+      mine += __popc(word);
+    }
+  }
+  int total;
+  block_inclusive_sum(mine, scratch, total);
+  return total;
+}
+
+// Calls take(rank, page) for the free pages of the share whose rank (`base` +
+// the free pages of the share before it) is below `limit`.
+template <class F>
+__device__ __forceinline__ void each_free(Share sh, const uint32_t *map, int base, int limit, int *scratch, F &&take) {
+  const int words = (sh.hi - sh.lo + 31) >> 5;
+  for (int w0 = 0; w0 < words && base < limit; w0 += blockDim.x) {
+    const int w = w0 + threadIdx.x;
+    uint32_t bits = w < words ? map[w] : 0u;
+    int total;
+    int rank = base + block_inclusive_sum(__popc(bits), scratch, total) - __popc(bits);
+    for (; bits != 0u && rank < limit; bits &= bits - 1, ++rank) take(rank, sh.lo + 32 * w + __ffs(bits) - 1);
+    base += total;
+  }
+}
+
+// Free pages of the CTAs before this one, and of all.
+__device__ __forceinline__ void free_before(int *count, int rank, int ranks, int &before, int &total) {
+  before = total = 0;
+  const uint32_t here = smem_u32(count);
+  for (int r = 0; r < ranks; ++r) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_map(here, (uint32_t)r)) : "memory");
+    before += r < rank ? v : 0;
+    total += v;
+  }
+}
+
+__device__ __forceinline__ int cluster_ranks() {
+  int r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ int clamp_int(long long v) { return v > 0x7fffffffll ? 0x7fffffff : (int)v; }
+
+// ---------------------------------------------------------------------------
+// resize
+
+struct ResizeArgs {
+  Tables t;
+  const int32_t *new_lens;
+  int64_t *slots;
+  int32_t *pos, *starts;
+  int capacity;
+};
+
+// One cluster. Every CTA scans all rows (they are few) and a share of the
+// pages; the phases are parted by cluster barriers:
+//   1. shrinking rows give pages back (integer atomics on refs);
+//   2. each row's need of pages and tokens, their prefix sums; the free map;
+//   3. the free pages of rank below the need go to the row that the rank
+//      falls into (binary search in the prefix sums);
+//   4. slots and positions, token by token, the same way.
+__global__ void __launch_bounds__(kTableThreads) resize_kernel(ResizeArgs a) {
+  extern __shared__ int smem[];
+  __shared__ long long scratch8[32];
+  __shared__ int scratch4[32];
+  __shared__ int s_free, s_pages, s_tokens, s_refused;
+  const Tables &t = a.t;
+  const int n = t.n, tid = threadIdx.x, lane = tid & 31;
+  const int rank = (int)cluster_ctarank(), ranks = cluster_ranks();
+  int *need_end = smem, *tok_end = smem + n, *old_len = smem + 2 * n;
+  uint32_t *map = reinterpret_cast<uint32_t *>(smem + 3 * n);
+  const Share sh = page_share(t.pages, rank, ranks);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (t.refs != t.refs_in)
+    for (int p = sh.lo + tid; p < sh.hi; p += blockDim.x) t.refs[p] = t.refs_in[p];
+  if (tid == 0) s_pages = s_tokens = s_refused = 0;
+  cluster_sync();
+  // 1. pages given back (and, with another table, the rows that stay)
+  const int warps = ranks * (int)(blockDim.x >> 5);
+  for (int i = rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
+    const int have = pages_of(held_len(t, i), t.shift);
+    const int want = a.new_lens[i] < 0 ? have : pages_of(a.new_lens[i], t.shift);
+    const int32_t *row = t.table_in + (size_t)i * t.max_pages;
+    for (int j = want + lane; j < have; j += 32)
+      if (page_ok(t, row[j])) atomicAdd(t.refs + row[j], -1);
+    if (t.table != t.table_in)
+      for (int j = lane; j < min(want, have); j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
+  }
+  cluster_sync();
+  // 2. needs
+  const int free = map_free(t, sh, map, scratch4);
+  if (tid == 0) s_free = free;
+  cluster_sync();
+  int before, total_free;
+  free_before(&s_free, rank, ranks, before, total_free);
+  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
+  long long need_sum = 0, tok_sum = 0;
+  int growing = 0, granted = 0;
+  for (int i = r0; i < r1; ++i) {
+    const int old = held_len(t, i), len = a.new_lens[i];
+    const int have = pages_of(old, t.shift), want = pages_of(len, t.shift);
+    bool fits = len > old && want <= t.max_pages;
+    growing += len > old;
+    if (fits && (old & ((1 << t.shift) - 1)) != 0) {  // its last page is partly filled
+      const int tail = t.table_in[(size_t)i * t.max_pages + (old >> t.shift)];
+      fits = page_ok(t, tail) && __ldcg(t.refs + tail) == 1;
+    }
+    need_sum += fits ? want - have : 0;
+    tok_sum += fits ? len - old : 0;
+    old_len[i] = old;
+    need_end[i] = clamp_int(need_sum);  // made absolute below
+    tok_end[i] = fits ? clamp_int(tok_sum) : -1 - clamp_int(tok_sum);  // sign: does not fit
+  }
+  long long all;
+  const long long need0 = block_inclusive_sum(need_sum, scratch8, all) - need_sum;
+  const long long tok0 = block_inclusive_sum(tok_sum, scratch8, all) - tok_sum;
+  int pages_given = 0, tokens_given = 0;
+  for (int i = r0; i < r1; ++i) {
+    const bool fits = tok_end[i] >= 0;
+    const int need = clamp_int(need0 + need_end[i]), tok = clamp_int(tok0 + (fits ? tok_end[i] : -1 - tok_end[i]));
+    need_end[i] = need, tok_end[i] = tok;
+    if (fits && need <= total_free && tok <= a.capacity) pages_given = need, tokens_given = tok, ++granted;
+  }
+  if (granted) atomicMax(&s_pages, pages_given), atomicMax(&s_tokens, tokens_given);
+  if (growing != granted) atomicAdd(&s_refused, growing - granted);
+  cluster_sync();
+  const int R = s_pages, T = s_tokens;
+  // 3. pages
+  each_free(sh, map, before, R, scratch4, [&](int r, int page) {
+    const int i = first_above(need_end, n, r);
+    const int col = pages_of(old_len[i], t.shift) + r - (i ? need_end[i - 1] : 0);
+    t.table[(size_t)i * t.max_pages + col] = page;
+    t.refs[page] = 1;
+  });
+  cluster_sync();
+  // 4. slots; no CTA reads the old lengths any more
+  const int threads = ranks * (int)blockDim.x;
+  for (int j = rank * (int)blockDim.x + tid; j < a.capacity; j += threads) {
+    long long slot = -1;
+    int pos = -1;
+    if (j < T) {
+      const int i = first_above(tok_end, n, j);
+      pos = old_len[i] + j - (i ? tok_end[i - 1] : 0);
+      const int page = __ldcg(t.table + (size_t)i * t.max_pages + (pos >> t.shift));
+      slot = ((long long)page << t.shift) + (pos & ((1 << t.shift) - 1));
+    }
+    a.slots[j] = slot;
+    a.pos[j] = pos;
+  }
+  for (int i = rank * (int)blockDim.x + tid; i < n; i += threads) {
+    const int first = i ? tok_end[i - 1] : 0, old = old_len[i], len = a.new_lens[i];
+    const bool given = tok_end[i] > first && tok_end[i] <= T && need_end[i] <= R;
+    t.lens[i] = given || (len >= 0 && len < old) ? len : old;
+    if (a.starts != nullptr) a.starts[i] = min(first, T);
+  }
+  if (rank == 0 && tid == 0) {
+    if (a.starts != nullptr) a.starts[n] = T;
+    if (t.status != nullptr) {
+      t.status[0] = R;
+      t.status[1] = s_refused;
+      t.status[2] = total_free - R;
+      t.status[3] = T;
+    }
+  }
+  cluster_sync();  // no CTA leaves while another reads its free count
+}
+
+// ---------------------------------------------------------------------------
+// reorder
+
+struct ReorderArgs {
+  Tables t;
+  const int32_t *parents;
+  int beams;
+  int32_t *copies;
+};
+
+// One cluster, in the manner of resize_kernel:
+//   1. refs of every page of old row i change by (children of i) - 1, and
+//      each new row's pages are those of its parent;
+//   2. rows whose partly filled last page is held by another row too need a
+//      page of their own, all but the first of the group when the group
+//      alone holds it; prefix sum over rows, free map over pages;
+//   3. the free pages of the lowest ranks go to those rows.
+__global__ void __launch_bounds__(kTableThreads) reorder_kernel(ReorderArgs a) {
+  extern __shared__ int smem[];
+  __shared__ int scratch4[32];
+  __shared__ int s_free;
+  const Tables &t = a.t;
+  const int n = t.n, K = a.beams, tid = threadIdx.x, lane = tid & 31;
+  const int rank = (int)cluster_ctarank(), ranks = cluster_ranks();
+  int *new_len = smem, *tail = smem + n, *copy_end = smem + 2 * n;
+  uint32_t *map = reinterpret_cast<uint32_t *>(smem + 3 * n);
+  const Share sh = page_share(t.pages, rank, ranks);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  if (t.refs != t.refs_in)
+    for (int p = sh.lo + tid; p < sh.hi; p += blockDim.x) t.refs[p] = t.refs_in[p];
+  for (int i = tid; i < n; i += blockDim.x) {
+    const int p = a.parents[i], src = i - i % K + p;
+    const bool kept = p >= 0 && p < K;
+    const int len = kept ? held_len(t, src) : 0;
+    new_len[i] = len;
+    int page = -1;
+    if ((len & ((1 << t.shift) - 1)) != 0) {
+      page = t.table_in[(size_t)src * t.max_pages + (len >> t.shift)];
+      if (!page_ok(t, page)) page = -1;
+    }
+    tail[i] = page;
+  }
+  cluster_sync();
+  // 1. references and rows
+  const int warps = ranks * (int)(blockDim.x >> 5);
+  for (int i = rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
+    const int g = i - i % K;
+    int children = 0;
+    for (int k = lane; k < K; k += 32) children += a.parents[g + k] == i - g;
+    children = __reduce_add_sync(0xffffffffu, children);
+    if (children != 1) {
+      const int have = pages_of(held_len(t, i), t.shift);
+      for (int j = lane; j < have; j += 32) {
+        const int page = t.table_in[(size_t)i * t.max_pages + j];
+        if (page_ok(t, page)) atomicAdd(t.refs + page, children - 1);
+      }
+    }
+    const int held = pages_of(new_len[i], t.shift);
+    const int32_t *row = t.table_in + (size_t)(g + (held ? a.parents[i] : 0)) * t.max_pages;
+    for (int j = lane; j < held; j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
+  }
+  cluster_sync();
+  // 2. rows that need a page
+  const int free = map_free(t, sh, map, scratch4);
+  if (tid == 0) s_free = free;
+  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
+  int want = 0;
+  for (int i = r0; i < r1; ++i) {
+    const int page = tail[i], g = i - i % K;
+    if (page >= 0) {
+      int holders = 0, first = K;
+      for (int k = K - 1; k >= 0; --k)
+        if (tail[g + k] == page) ++holders, first = k;
+      want += !(first == i - g && __ldcg(t.refs + page) == holders);
+    }
+    copy_end[i] = want;  // made absolute below
+  }
+  int wanted;
+  const int want0 = block_inclusive_sum(want, scratch4, wanted) - want;
+  for (int i = r0; i < r1; ++i) copy_end[i] += want0;
+  cluster_sync();
+  int before, total_free;
+  free_before(&s_free, rank, ranks, before, total_free);
+  const int R = min(wanted, total_free);
+  // 3. pages
+  each_free(sh, map, before, R, scratch4, [&](int r, int page) {
+    const int i = first_above(copy_end, n, r);
+    t.table[(size_t)i * t.max_pages + (new_len[i] >> t.shift)] = page;
+    t.refs[page] = 1;
+    atomicAdd(t.refs + tail[i], -1);
+    a.copies[2 * i] = tail[i];
+    a.copies[2 * i + 1] = page;
+  });
+  const int threads = ranks * (int)blockDim.x;
+  for (int i = rank * (int)blockDim.x + tid; i < n; i += threads) {
+    const int r = i ? copy_end[i - 1] : 0;
+    if (copy_end[i] == r || r >= R) a.copies[2 * i] = a.copies[2 * i + 1] = -1;
+    t.lens[i] = new_len[i];
+  }
+  if (rank == 0 && tid == 0 && t.status != nullptr) {
+    t.status[0] = R;
+    t.status[1] = wanted - R;
+    t.status[2] = total_free - R;
+    t.status[3] = R;
+  }
+  cluster_sync();  // no CTA leaves while another reads its free count
+}
+
+// The page copies of a reorder: 16-byte pieces of the lens % page_size tokens
+// of every copied row, in all layers, K and V. Grid: (pieces, rows, layers).
+struct CopyArgs {
+  const int32_t *copies, *lens;
+  char *k, *v;
+  long long layer_stride, page_stride, head_stride, token_stride;  // bytes
+  int kv_heads, pieces, page_size;                                 // pieces: 16-byte pieces of a head's row
+};
+
+__global__ void __launch_bounds__(256) copy_pages_kernel(CopyArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = blockIdx.y;
+  const int src = a.copies[2 * row], dst = a.copies[2 * row + 1];
+  if (src < 0) return;
+  const int tokens = a.lens[row] & (a.page_size - 1);
+  const int total = tokens * a.kv_heads * a.pieces;
+  const long long layer = (long long)blockIdx.z * a.layer_stride;
+  for (int u = blockIdx.x * blockDim.x + threadIdx.x; u < total; u += gridDim.x * blockDim.x) {
+    const int piece = u % a.pieces, rest = u / a.pieces;
+    const long long at = layer + (rest / tokens) * a.head_stride + (rest % tokens) * a.token_stride + 16ll * piece;
+    const uint4 x = *reinterpret_cast<const uint4 *>(a.k + at + src * a.page_stride);
+    const uint4 y = *reinterpret_cast<const uint4 *>(a.v + at + src * a.page_stride);
+    *reinterpret_cast<uint4 *>(a.k + at + dst * a.page_stride) = x;
+    *reinterpret_cast<uint4 *>(a.v + at + dst * a.page_stride) = y;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// append
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  void *q_out;
+  char *kc, *vc;  // layer base
+  const float *k_scale, *v_scale;
+  const int64_t *slots;
+  const int32_t *pos;
+  const float *rope;
+  long long q_ld, k_ld, v_ld;
+  long long page_stride, head_stride, token_stride;  // elements
+  long long slot_end;                                // pages * page_size
+  int tokens, heads, kv_heads, dim, shift, rope_len;
+};
+
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+  const float4 a = __ldcs(reinterpret_cast<const float4 *>(p));
+  const float4 b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+  const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
+  const T *e = reinterpret_cast<const T *>(&a);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
+}
+
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
+  uint4 o;
+  __nv_bfloat162 *e = reinterpret_cast<__nv_bfloat162 *>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+  *reinterpret_cast<uint4 *>(p) = o;
+}
+__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
+  uint4 o;
+  __half2 *e = reinterpret_cast<__half2 *>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+  *reinterpret_cast<uint4 *>(p) = o;
+}
+__device__ __forceinline__ void store8(__nv_fp8_e4m3 *p, const float (&x)[8]) {
+  uint2 o;
+  __nv_fp8x2_storage_t *e = reinterpret_cast<__nv_fp8x2_storage_t *>(&o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  *reinterpret_cast<uint2 *>(p) = o;
+}
+
+// One thread per 8 elements (4 rotary pairs) of a q, k or v head: in fp32,
+// rounded once where it is stored. Bound by memory: every element is read
+// and written once, the rotary row of a token comes from L1 for all heads
+// but the first.
+template <typename In, typename Out, typename Cache>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int eighths = a.dim >> 3;
+  const int q_units = a.q != nullptr ? a.heads * eighths : 0, kv_units = a.kv_heads * eighths;
+  const int units = q_units + 2 * kv_units;
+  const long long total = (long long)a.tokens * units;
+  for (long long w = (long long)blockIdx.x * blockDim.x + threadIdx.x; w < total; w += (long long)gridDim.x * blockDim.x) {
+    const int tok = (int)(w / units);
+    int u = (int)(w % units);
+    const long long slot = a.slots[tok];
+    bool live = slot >= 0;
+    if (live && slot >= a.slot_end) {
+      report_timeout(&g_paged_status, kSiteSlot);
+      live = false;
+    }
+    int pos = 0;
+    if (live && a.rope != nullptr) {
+      pos = a.pos[tok];
+      if (pos < 0 || pos >= a.rope_len) {
+        report_timeout(&g_paged_status, kSitePos);
+        live = false;
+      }
+    }
+    const int part = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;
+    u -= part == 0 ? 0 : part == 1 ? q_units : q_units + kv_units;
+    const int head = u / eighths, d = 8 * (u % eighths);
+    if (!live) {
+      if (part == 0) {
+        const float zero[8] = {};
+        store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, zero);
+      }
+      continue;
+    }
+    const In *src = part == 0 ? static_cast<const In *>(a.q) + tok * a.q_ld
+                  : part == 1 ? static_cast<const In *>(a.k) + tok * a.k_ld
+                              : static_cast<const In *>(a.v) + tok * a.v_ld;
+    float x[8];
+    load8(src + head * a.dim + d, x);
+    if (part < 2 && a.rope != nullptr) {
+      const float4 *cs = reinterpret_cast<const float4 *>(a.rope + (long long)pos * a.dim + d);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // two pairs per 16 bytes of (cos, sin)
+        const float4 c = __ldg(cs + i);
+        const float x0 = x[4 * i], x1 = x[4 * i + 1], x2 = x[4 * i + 2], x3 = x[4 * i + 3];
+        x[4 * i] = x0 * c.x - x1 * c.y, x[4 * i + 1] = x0 * c.y + x1 * c.x;
+        x[4 * i + 2] = x2 * c.z - x3 * c.w, x[4 * i + 3] = x2 * c.w + x3 * c.z;
+      }
+    }
+    if (part == 0) {
+      store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, x);
+      continue;
+    }
+    const float *scale = part == 1 ? a.k_scale : a.v_scale;
+    if (scale != nullptr) {
+      const float s = __ldg(scale + head);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] / s;
+    }
+    Cache *base = reinterpret_cast<Cache *>(part == 1 ? a.kc : a.vc);
+    store8(base + (slot >> a.shift) * a.page_stride + head * a.head_stride +
+               (slot & ((1ll << a.shift) - 1)) * a.token_stride + d, x);
+  }
+}
+
+// Launches one cluster of `ranks` CTAs (a table kernel).
+template <typename Args>
+int launch_tables(void (*kernel)(Args), const Args &a, int ranks, size_t smem, cudaStream_t s, const char *what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ranks);
+  cfg.blockDim = dim3(kTableThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  return e == cudaSuccess ? CE_OK : cuda_error(e, what);
+}
+
+// Dynamic shared memory of a table kernel: three words per row, and the free
+// map of a CTA's share of the pages.
+size_t table_smem(const ce_page_table *t, int ranks) {
+  const int words = ((t->pages + ranks - 1) / ranks + 31) / 32;
+  return 12ull * t->seqs + 4ull * words;
+}
+constexpr size_t kTableSmemMax = 12ull * kMaxRows + kMaxPages / 8 / 8 + 128;  // a cluster of 8
+static_assert(kTableSmemMax <= 224 * 1024, "a table kernel's shared memory");
+
+// CTAs of a table kernel.
+int table_ranks(const ce_page_table *t) { return t->pages <= 32768 && t->seqs <= 4096 ? 1 : 8; }
+
+// Opts the table kernels into their shared memory, once per device.
+int configure_tables() {
+  static bool done[64] = {};
+  int dev = 0;
+  CE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && done[dev]) return CE_OK;
+  CE_CUDA_TRY(cudaFuncSetAttribute(resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTableSmemMax));
+  CE_CUDA_TRY(cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)kTableSmemMax));
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return CE_OK;
+}
+
+int check_pair(const ce_page_table *to, const ce_page_table *from) {
+  int rc = check_table(from, "from");
+  if (rc == CE_OK) rc = check_table(to, "to");
+  if (rc != CE_OK) return rc;
+  CE_REQUIRE(to->seqs == from->seqs && to->max_pages == from->max_pages && to->pages == from->pages &&
+                 to->page_size == from->page_size,
+             "`to` and `from` must have the same rows, columns, pages and page size");
+  return CE_OK;
+}
+
+Tables tables_of(const ce_page_table *to, const ce_page_table *from, int32_t *status) {
+  return {from->table_dev, from->lens_dev, from->refs_dev, to->table_dev, to->lens_dev, to->refs_dev, status,
+          from->seqs, from->max_pages, from->pages, log2_of(from->page_size)};
+}
+
+template <typename In, typename Out>
+int launch_append(int cache_type, const AppendArgs &a, dim3 grid, cudaStream_t s) {
+  if (cache_type == CE_TYPE_BF16)
+    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, dim3(256), 0, s, true, "append_kernel", a);
+  if (cache_type == CE_TYPE_F16)
+    return launch_kernel(append_kernel<In, Out, __half>, grid, dim3(256), 0, s, true, "append_kernel", a);
+  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, dim3(256), 0, s, true, "append_kernel", a);
+}
+
+template <typename In>
+int launch_append(int out_type, int cache_type, const AppendArgs &a, dim3 grid, cudaStream_t s) {
+  return out_type == CE_TYPE_F16 ? launch_append<In, __half>(cache_type, a, grid, s)
+                                 : launch_append<In, __nv_bfloat16>(cache_type, a, grid, s);
+}
+
+}  // namespace
+
+int check_kv(const ce_paged_kv *kv, int layer) {
+  CE_REQUIRE(kv != nullptr, "null cache");
+  CE_REQUIRE(type16(kv->type) || kv->type == CE_TYPE_E4M3, "cache type must be BF16, F16 or E4M3 (got %d)", kv->type);
+  CE_REQUIRE(kv->k_dev != nullptr && kv->v_dev != nullptr, "null k or v pool");
+  CE_REQUIRE(kv->type == CE_TYPE_E4M3 || (kv->k_scale_dev == nullptr && kv->v_scale_dev == nullptr),
+             "a 16-bit cache takes no scales");
+  CE_REQUIRE(kv->layers >= 1 && kv->kv_heads >= 1 && kv->pages >= 1 && kv->pages <= kMaxPages,
+             "layers and kv_heads must be >= 1 and pages in [1, %d] (got %d, %d, %d)", kMaxPages, kv->layers,
+             kv->kv_heads, kv->pages);
+  CE_REQUIRE(kv->page_size >= 1 && kv->page_size <= kMaxPage && (kv->page_size & (kv->page_size - 1)) == 0,
+             "page_size must be a power of two in [1, %d] (got %d)", kMaxPage, kv->page_size);
+  CE_REQUIRE(kv->head_dim >= 16 && kv->head_dim <= 128 && kv->head_dim % 16 == 0,
+             "head_dim must be a multiple of 16 in [16, 128] (got %d)", kv->head_dim);
+  CE_REQUIRE(layer >= 0 && layer < kv->layers, "layer %d of %d", layer, kv->layers);
+  const int64_t unit = 16 / type_bytes(kv->type);
+  CE_REQUIRE(aligned16(kv->k_dev) && aligned16(kv->v_dev) && kv->layer_stride % unit == 0 &&
+                 kv->page_stride % unit == 0 && kv->head_stride % unit == 0 && kv->token_stride % unit == 0,
+             "the cache's bases and strides must be multiples of 16 bytes");
+  return CE_OK;
+}
+
+int check_table(const ce_page_table *t, const char *what) {
+  CE_REQUIRE(t != nullptr, "null page table (%s)", what);
+  CE_REQUIRE(t->table_dev != nullptr && t->lens_dev != nullptr && t->refs_dev != nullptr,
+             "null buffer in the page table (%s)", what);
+  CE_REQUIRE(t->seqs >= 1 && t->seqs <= kMaxRows && t->max_pages >= 1,
+             "seqs must be in [1, %d] and max_pages >= 1 (got %d, %d)", kMaxRows, t->seqs, t->max_pages);
+  CE_REQUIRE(t->pages >= 1 && t->pages <= kMaxPages, "pages must be in [1, %d] (got %d)", kMaxPages, t->pages);
+  CE_REQUIRE(t->page_size >= 1 && t->page_size <= kMaxPage && (t->page_size & (t->page_size - 1)) == 0,
+             "page_size must be a power of two in [1, %d] (got %d)", kMaxPage, t->page_size);
+  CE_REQUIRE((int64_t)t->max_pages * t->page_size <= 0x7fffffff, "max_pages * page_size must be below 2^31");
+  return CE_OK;
+}
+
+}  // namespace paged
+
+using namespace paged;
+
+// Reads and clears the status word of the table and append kernels.
+int paged_status() {
+  CE_CUDA_TRY(cudaDeviceSynchronize());
+  DeviceStatus h{};
+  CE_CUDA_TRY(cudaMemcpyFromSymbol(&h, g_paged_status, sizeof(h)));
+  if (h.code == 0) return CE_OK;
+  const DeviceStatus zero{};
+  CE_CUDA_TRY(cudaMemcpyToSymbol(g_paged_status, &zero, sizeof(zero)));
+  return set_error(CE_ERR_USAGE, h.where == kSiteSlot  ? "paged append: a slot lies past the pool"
+                                 : h.where == kSitePos ? "paged append: a position lies past the rotary table"
+                                 : h.where == kSitePage ? "block table: a page id lies outside the pool"
+                                                        : "block table: a length does not fit its row");
+}
+
+}  // namespace ce
+
+using namespace ce;
+
+extern "C" {
+
+int ce_paged_resize(const ce_page_table *to, const ce_page_table *from, const int32_t *new_lens, int64_t *slots,
+                    int32_t *pos, int capacity, int32_t *starts, int32_t *status, ce_stream_t stream) {
+  int rc = check_pair(to, from);
+  if (rc != CE_OK) return rc;
+  CE_REQUIRE(new_lens != nullptr, "null new lengths");
+  CE_REQUIRE(capacity >= 0 && (capacity == 0 || (slots != nullptr && pos != nullptr)),
+             "slots and pos are required for a capacity of %d", capacity);
+  rc = configure_tables();
+  if (rc != CE_OK) return rc;
+  const int ranks = table_ranks(from);
+  const ResizeArgs a = {tables_of(to, from, status), new_lens, slots, pos, starts, capacity};
+  return launch_tables(resize_kernel, a, ranks, table_smem(from, ranks), (cudaStream_t)stream, "resize_kernel");
+}
+
+int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const int32_t *parents, int beams,
+                     const ce_paged_kv *kv, int32_t *copies, int32_t *status, ce_stream_t stream) {
+  int rc = check_pair(to, from);
+  if (rc != CE_OK) return rc;
+  CE_REQUIRE(to->table_dev != from->table_dev, "the tables of `to` and `from` must differ");
+  CE_REQUIRE(parents != nullptr && copies != nullptr, "null parents or copies");
+  CE_REQUIRE(beams >= 1 && from->seqs % beams == 0, "%d rows are no whole number of groups of %d", from->seqs, beams);
+  if (kv != nullptr) {
+    rc = check_kv(kv, 0);
+    if (rc != CE_OK) return rc;
+    CE_REQUIRE(kv->pages == from->pages && kv->page_size == from->page_size,
+               "the cache has %d pages of %d, the block table %d of %d", kv->pages, kv->page_size, from->pages,
+               from->page_size);
+  }
+  rc = configure_tables();
+  if (rc != CE_OK) return rc;
+  const cudaStream_t s = (cudaStream_t)stream;
+  const int ranks = table_ranks(from);
+  const ReorderArgs a = {tables_of(to, from, status), parents, beams, copies};
+  rc = launch_tables(reorder_kernel, a, ranks, table_smem(from, ranks), s, "reorder_kernel");
+  if (rc != CE_OK || kv == nullptr || kv->page_size == 1) return rc;
+  const int b = type_bytes(kv->type);
+  const CopyArgs c = {copies, to->lens_dev, static_cast<char *>(kv->k_dev), static_cast<char *>(kv->v_dev),
+                      kv->layer_stride * b, kv->page_stride * b, kv->head_stride * b, kv->token_stride * b,
+                      kv->kv_heads, kv->head_dim * b / 16, kv->page_size};
+  const int most = (kv->page_size - 1) * c.kv_heads * c.pieces;  // pieces of a row in one layer
+  const dim3 grid((unsigned)((most + 1023) / 1024), (unsigned)from->seqs, (unsigned)kv->layers);
+  CE_REQUIRE(kv->layers <= 65535, "layers must be below 65536 (got %d)", kv->layers);
+  return launch_kernel(copy_pages_kernel, grid, dim3(256), 0, s, true, "copy_pages_kernel", c);
+}
+
+int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out, int q_out_type, const void *q, const void *k,
+                    const void *v, int in_type, int64_t q_ld, int64_t k_ld, int64_t v_ld, const int64_t *slots,
+                    const int32_t *pos, int tokens, int heads, const float *rope, int rope_len, ce_stream_t stream) {
+  const int rc = check_kv(kv, layer);
+  if (rc != CE_OK) return rc;
+  CE_REQUIRE(tokens >= 0, "tokens must be >= 0 (got %d)", tokens);
+  if (tokens == 0) return CE_OK;
+  CE_REQUIRE(k != nullptr && v != nullptr && slots != nullptr, "null k, v or slots");
+  CE_REQUIRE((q == nullptr) == (q_out == nullptr), "q and q_out come together");
+  CE_REQUIRE(in_type == CE_TYPE_F32 || type16(in_type), "q, k, v must be F32, BF16 or F16 (got %d)", in_type);
+  CE_REQUIRE(q == nullptr || type16(q_out_type), "q_out must be BF16 or F16 (got %d)", q_out_type);
+  CE_REQUIRE(q == nullptr || heads >= 1, "heads must be >= 1 (got %d)", heads);
+  CE_REQUIRE(rope == nullptr || (pos != nullptr && rope_len >= 1), "a rotary table needs positions and rope_len >= 1");
+  const int64_t unit = 16 / type_bytes(in_type), dim = kv->head_dim;
+  CE_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(rope) && q_ld % unit == 0 &&
+                 k_ld % unit == 0 && v_ld % unit == 0,
+             "q, k, v, q_out and rope must be 16-byte aligned, their row strides multiples of 16 bytes");
+  CE_REQUIRE((q == nullptr || q_ld >= heads * dim) && k_ld >= kv->kv_heads * dim && v_ld >= kv->kv_heads * dim,
+             "a row stride is shorter than its heads");
+  const int b = type_bytes(kv->type);
+  AppendArgs a = {};
+  a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+  a.kc = static_cast<char *>(kv->k_dev) + (long long)layer * kv->layer_stride * b;
+  a.vc = static_cast<char *>(kv->v_dev) + (long long)layer * kv->layer_stride * b;
+  a.k_scale = kv->k_scale_dev, a.v_scale = kv->v_scale_dev;
+  a.slots = slots, a.pos = pos, a.rope = rope;
+  a.q_ld = q_ld, a.k_ld = k_ld, a.v_ld = v_ld;
+  a.page_stride = kv->page_stride, a.head_stride = kv->head_stride, a.token_stride = kv->token_stride;
+  a.slot_end = (long long)kv->pages * kv->page_size;
+  a.tokens = tokens, a.heads = q != nullptr ? heads : 0, a.kv_heads = kv->kv_heads, a.dim = kv->head_dim;
+  a.shift = log2_of(kv->page_size), a.rope_len = rope_len;
+  const long long units = (long long)tokens * (a.heads + 2 * a.kv_heads) * (a.dim / 8);
+  const dim3 grid((unsigned)std::min<long long>((units + 255) / 256, 8ll * sm_count()));
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (in_type == CE_TYPE_F32) return launch_append<float>(q_out_type, kv->type, a, grid, s);
+  if (in_type == CE_TYPE_F16) return launch_append<__half>(q_out_type, kv->type, a, grid, s);
+  return launch_append<__nv_bfloat16>(q_out_type, kv->type, a, grid, s);
+}
+
+}  // extern "C"

@@ -72,7 +72,9 @@ int ce_device_info(int *sm_count, int *is_sm100);
  * wait of a tensor-core kernel gave up since the last call (CE_ERR_TIMEOUT,
  * then cleared). The reference's stream-K consumer waits without a limit
  * (applications/loom_private/decoder/decoder_optimized.cu:391-394); every
- * wait of this library is bounded and reported here instead. */
+ * wait of this library is bounded and reported here instead. Slots, positions,
+ * pages and lengths that a paged operator found out of range on the device
+ * are reported here too (CE_ERR_USAGE, then cleared). */
 int ce_device_status(void);
 
 /* ------------------------------------------------------------------ */
@@ -819,6 +821,155 @@ int ce_llama_read_nvfp4(ce_llama *model, int which, int layer, uint8_t *packed_h
  * a step ran past the end of the KV cache, CE_ERR_TIMEOUT when a staging wait
  * gave up. Synchronizes the device. */
 int ce_llama_status(void);
+
+/* ------------------------------------------------------------------ */
+/* Paged key-value cache and beam search.                              */
+/*
+ * A server's requests have lengths of their own, start and end at any step
+ * and, under beam search, share prefixes. Their keys and values live in a
+ * pool of pages of page_size tokens; a block table names each request's
+ * pages in order. One decode step of a beam search is
+ *
+ *   ce_paged_resize     every request one token longer: pages, slots, positions
+ *   ce_paged_append     rotary positions, k and v into their slots  (per layer)
+ *   ce_paged_attention  the new token's attention over its pages    (per layer)
+ *   ce_beam_select      the next tokens and the beams they extend
+ *   ce_paged_reorder    every row becomes its parent; shared last pages are copied
+ *
+ * all on the device, capturable, without a host copy of any length. The
+ * reference has no counterpart (its decoder has no attention and no cache).
+ */
+
+/* Element types of the paged operators. */
+#define CE_TYPE_F32 0
+#define CE_TYPE_BF16 1
+#define CE_TYPE_F16 2
+#define CE_TYPE_E4M3 3
+
+/* Pools of keys and values, in one layout: element d of token t (of
+ * page_size) of head h of page p of layer l is at
+ *   l * layer_stride + p * page_stride + h * head_stride + t * token_stride + d
+ * (strides in elements, 64-bit), so head-major pages and token-major pages
+ * are both served. type is CE_TYPE_BF16, _F16 or _E4M3; an E4M3 code stands
+ * for code * scale[h] with one fp32 scale per head (NULL: 1; NULL for the
+ * 16-bit types). page_size is a power of two from 1 to 1024, head_dim a
+ * multiple of 16 from 16 to 128; base pointers and strides are multiples of
+ * 16 bytes. */
+typedef struct ce_paged_kv {
+  void *k_dev, *v_dev;
+  const float *k_scale_dev, *v_scale_dev; /* [kv_heads] */
+  int32_t type, layers, pages, kv_heads, page_size, head_dim;
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+} ce_paged_kv;
+
+/* Block tables: row i holds the pages of request i in order, of which the
+ * first ceil(lens[i] / page_size) count; what stands behind them means
+ * nothing. refs[p] counts the rows that hold page p: 0 is a free page, and a
+ * caller that adds 1 of its own keeps a page out of reuse. At most 16384
+ * rows and 2^20 pages. */
+typedef struct ce_page_table {
+  int32_t *table_dev; /* [seqs][max_pages] */
+  int32_t *lens_dev;  /* [seqs], tokens in the cache */
+  int32_t *refs_dev;  /* [pages] */
+  int32_t seqs, max_pages, pages, page_size;
+} ce_page_table;
+
+/* Gives every request its new length. First the requests that get shorter
+ * (0 ends one) give back the pages past their new end; then, in row order,
+ * those that get longer take the free pages of the lowest numbers. A
+ * negative new length leaves a request as it is.
+ *
+ * New tokens are numbered request by request: starts[i] is the first number
+ * of request i (starts[seqs] their count), slots[j] = page * page_size +
+ * offset is where token j's key and value belong and pos[j] its position in
+ * its request; from the count up to `capacity` slots and pos are -1. starts
+ * and status may be NULL.
+ *
+ * A growing request is refused (it keeps its old length, takes nothing) when
+ * it would need more than max_pages pages, when its last page is partly
+ * filled and held by more than one row (ce_paged_reorder copies such pages),
+ * or when the free pages or the capacity do not suffice for it and those
+ * before it; from the first that does not suffice on, all are refused.
+ * status[0..3] = pages taken, requests refused, pages still free, new tokens.
+ *
+ * `to` and `from` describe the same rows and pages; each of their buffers may
+ * be the same one (in place) or another. */
+int ce_paged_resize(const ce_page_table *to, const ce_page_table *from, const int32_t *new_lens_dev,
+                    int64_t *slots_dev, int32_t *pos_dev, int capacity, int32_t *starts_dev,
+                    int32_t *status_dev, ce_stream_t stream);
+
+/* Rotary positions and the cache write of `tokens` new tokens. Token t has
+ * heads q rows and kv_heads k and v rows of head_dim elements, heads
+ * contiguous, tokens q_ld / k_ld / v_ld elements apart (the slices of one
+ * QKV row), all of in_type (CE_TYPE_F32, _BF16 or _F16). Pair (2i, 2i+1) of
+ * q and k turns by the angle whose (cos, sin) is rope[pos[t]][i] (fp32,
+ * [rope_len][head_dim / 2][2]; NULL: no turn, pos may then be NULL), in fp32.
+ * q goes to q_out [tokens][heads][head_dim] of q_out_type (16 bits), k and v
+ * to slot slots[t] of `layer`, rounded to the nearest value of the pool's
+ * type (E4M3: of x / scale, saturating at 448). A token whose slot is
+ * negative writes no cache, and zeros to q_out. Slots past the pool and
+ * positions past rope_len are left out the same way and reported by
+ * ce_device_status (CE_ERR_USAGE). q_dev and q_out_dev may both be NULL. */
+int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out_dev, int q_out_type, const void *q_dev,
+                    const void *k_dev, const void *v_dev, int in_type, int64_t q_ld, int64_t k_ld,
+                    int64_t v_ld, const int64_t *slots_dev, const int32_t *pos_dev, int tokens, int heads,
+                    const float *rope_dev, int rope_len, ce_stream_t stream);
+
+/* Bytes of ce_paged_attention's workspace on the current device. Zero it once
+ * before the first call; every call leaves it ready for the next. Calls that
+ * may run at the same time need a workspace each. */
+int ce_paged_attention_workspace(size_t *bytes);
+
+/* Attention of one new token per request over its pages: for each of `heads`
+ * query heads h (kv head h / (heads / kv_heads)), over positions j < lens[i],
+ *   s_j = scale * q . k_j,   out = sum_j e^s_j v_j / sum_j e^s_j,
+ *   lse = log sum_j e^s_j    (natural; lse_dev may be NULL).
+ * A request of length 0 gets out = 0, lse = -inf. q and out are
+ * [seqs][heads][head_dim] of io_type (the pool's type; for an E4M3 pool
+ * CE_TYPE_BF16 or _F16), rows of one request contiguous, requests q_ld /
+ * out_ld elements apart (16-byte aligned). Scores, softmax and sums are fp32.
+ * Lengths past max_pages * page_size are cut there, pages outside the pool
+ * read as zeros; both are reported by ce_device_status (CE_ERR_USAGE). */
+int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pages, void *out_dev,
+                       float *lse_dev, const void *q_dev, int io_type, int heads, int64_t q_ld,
+                       int64_t out_ld, float scale, void *workspace_dev, size_t workspace_bytes,
+                       ce_stream_t stream);
+
+/* Bytes of ce_beam_select's workspace; zeroed once, as above. */
+int ce_beam_workspace(int batch, int beams, int vocab, size_t *bytes);
+
+/* One selection of a beam search. logits [batch * beams][vocab] (row stride
+ * ld elements; CE_TYPE_F32, _BF16 or _F16), scores [batch][beams] the beams'
+ * log probabilities so far. Beam k of a batch element offers its best
+ * min(beams, vocab) tokens by logit (ties to the lowest token), each with
+ *   score = scores[k] + (logit - lse),  lse = max + log sum e^(logit - max),
+ * in fp32; a finished beam offers `pad` with its score as it is. The `beams`
+ * best of a batch element's offers by score (ties to the lowest beam, then
+ * the better rank in it) become its next beams, best first: scores_out,
+ * parents (the beam of the same element that each extends), tokens, and
+ * finished_out (the parent was finished, or the token is eos). NaN and -inf
+ * logits are tokens of probability 0 (score -inf); +inf counts as the
+ * largest finite fp32; a NaN score counts as -inf. beams <= 32. Outputs may
+ * not overlap the inputs. */
+int ce_beam_select(float *scores_out_dev, int32_t *parents_dev, int32_t *tokens_dev,
+                   uint8_t *finished_out_dev, const void *logits_dev, int type, int64_t ld,
+                   const float *scores_dev, const uint8_t *finished_dev, int batch, int beams, int vocab,
+                   int eos, int pad, void *workspace_dev, size_t workspace_bytes, ce_stream_t stream);
+
+/* Row i of `to` becomes the row that parents[i] (0 .. beams-1) names within
+ * i's group of `beams` consecutive rows of `from`; a parent outside that
+ * range drops the row (length 0). refs follows: each page counts the new
+ * rows. Then every new row must own its partly filled last page: where a
+ * page is held by rows of one group alone the first of them keeps it, and
+ * each other row takes the lowest-numbered free page, in row order, into
+ * which the lens % page_size tokens are copied, in all layers of kv (NULL:
+ * the tables alone). copies[i] = (from page, to page), or (-1, -1);
+ * status[0..3] = pages taken, rows that found no free page (they keep
+ * sharing; ce_paged_resize refuses to grow them), pages still free, rows
+ * copied. copies is required, status may be NULL. The table buffers of `to`
+ * and `from` must differ; lens and refs may be the same or others. */
+int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const int32_t *parents_dev, int beams,
+                     const ce_paged_kv *kv, int32_t *copies_dev, int32_t *status_dev, ce_stream_t stream);
 
 #ifdef __cplusplus
 }
