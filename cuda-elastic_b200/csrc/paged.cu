@@ -597,6 +597,8 @@ int check_kv(const ce_paged_kv *kv, int layer) {
   CE_REQUIRE(aligned16(kv->k_dev) && aligned16(kv->v_dev) && kv->layer_stride % unit == 0 &&
                  kv->page_stride % unit == 0 && kv->head_stride % unit == 0 && kv->token_stride % unit == 0,
              "the cache's bases and strides must be multiples of 16 bytes");
+  CE_REQUIRE(kv->layer_stride >= 0 && kv->page_stride >= 0 && kv->head_stride >= 0 && kv->token_stride >= 0,
+             "the cache's strides must not be negative");
   return CE_OK;
 }
 

@@ -1,4 +1,39 @@
 // Attention of one new token per request over a paged key-value cache.
+//
+// For a request and a kv head the G query heads that share it attend to the
+// same keys: S^T = K Q^T, O^T = V^T P^T, a matrix product with the keys (or
+// the head's dimensions) as the 16-row side and the query heads as the 8-wide
+// side. Every key and value is used once, G x 4 flops per element pair, so
+// the bound is the memory that K and V come from. The design serves that:
+//
+//   * The unit of work is 16 keys of one (request, kv head). All units of the
+//     batch form one line, in which every warp of the grid (one CTA per SM)
+//     takes an equal contiguous share, whatever the lengths: a long request
+//     is split over many SMs, many short ones share a warp, and no SM ends
+//     early. Lengths are read on the device; the grid never depends on them.
+//   * A warp runs alone: no block barrier until its share is done. It copies
+//     its units with cp.async into a ring of its own, several units ahead and
+//     across request boundaries, and each lane copies exactly the bytes that
+//     it will itself feed to the tensor core, so a wait for its own copies is
+//     all the synchronisation there is, and shared memory is read back in
+//     16-byte pieces without bank conflicts or transposition: a lane's 16
+//     bytes of a key serve as that lane's part of the contracted dimension
+//     (any order will do, when q is laid out alike), and its 16 bytes of four
+//     values are paired by byte permutes into the rows of V^T.
+//   * mma.sync (m16n8k16), not tcgen05: with 8 query heads on the narrow side
+//     nothing is wasted on padding rows up to 8 heads, accumulators stay in
+//     registers beside the softmax, and the tensor work is far from binding.
+//     A tcgen05 tile would have 128 rows of queries to fill from at most 16.
+//   * The softmax keeps a running maximum and sum per query head in fp32. The
+//     weights e^(s - max) enter the second product as two 16-bit parts (the
+//     rounded value and what the rounding lost): rounded once to 16 bits they
+//     would err as much as the output's own rounding.
+//   * A request split over warps or CTAs is joined from (max, sum, O) parts:
+//     within a CTA from shared memory, across CTAs by the last to arrive, in
+//     the order of the keys, so the result does not depend on who is last.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace ce {
@@ -6,6 +41,11 @@ namespace paged {
 namespace {
 
 __device__ DeviceStatus g_attention_status;
+
+constexpr int kUnit = 16;              // keys of a unit
+constexpr int kMaxSplitHeads = 16;     // query heads of one pass over the keys
+constexpr int kMaxGrid = 1024;         // CTAs the workspace's counters are laid out for
+constexpr int kPartFloats = kMaxSplitHeads * (128 + 2);
 
 struct AttnArgs {
   const void *q;
@@ -15,83 +55,650 @@ struct AttnArgs {
   const float *k_scale, *v_scale;
   const int32_t *table, *lens;
   long long q_ld, out_ld;
-  long long page_stride, head_stride, token_stride;  // elements
+  long long page_stride, head_stride, token_stride;  // bytes
   int seqs, max_pages, pages, heads, kv_heads, dim, shift;
+  int group, tiles;  // query heads per kv head; passes over them
   float scale;
+  int *arrivals;  // [kMaxGrid], zero between calls
+  float *parts;   // [grid][2][kPartFloats]
 };
 
-template <typename T>
-__device__ __forceinline__ float as_float(T x) {
-  if constexpr (sizeof(T) == 1) return float(x);
-  else return paged::to_float(x);
-}
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+// How many warps a CTA has and how many units each keeps in its ring: about
+// 200 KB of shared memory, two thirds of it in flight.
+template <int D, int NT, bool F8>
+struct Shape {
+  static constexpr int kItem = F8 ? 1 : 2;                    // bytes of a cached element
+  static constexpr int kKeyChunks = D * kItem / 64;           // 16-byte pieces of a key row per lane
+  static constexpr int kValBytes = D * kItem / 8 >= 16 ? 16 : 8;
+  static constexpr int kValChunks = D * kItem / 8 / kValBytes;  // pieces of a value row per lane
+  static constexpr int kKeyBytes = 2 * kKeyChunks * 512;
+  static constexpr int kStageBytes = kKeyBytes + 4 * kValChunks * 32 * kValBytes;
+  static constexpr int kWarps = NT == 1 ? (kStageBytes == 8192 ? 8 : F8 && D == 128 ? 12 : 16)
+                                        : (kStageBytes == 8192 ? 6 : F8 && D == 128 ? 8 : 12);
+  static constexpr int kStages = kStageBytes == 2048 ? 5 : F8 && D == 128 && NT == 2 ? 4 : 3;
+  static constexpr int kHeads = 8 * NT;
+  static constexpr int kPart = kHeads * (D + 2);  // floats of one (O, max, sum) part
+  static constexpr int kVals = D / 8;             // dimensions of a value row per lane
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr size_t kSmem = (size_t)kWarps * (kRing + 4 * kPart);
+  static_assert(4 * kPart <= kRing, "a warp's second part lies in its ring");
+  static_assert(4 * kThreads <= kWarps * 4 * kPart, "the prefix sums lie in the parts' place");
+  static_assert(kSmem <= 230 * 1024, "shared memory of an SM, with 2 KB besides");
+};
 
-// One warp per (request, head): an online softmax over its positions, lane l
-// holding dimensions l, l + 32, ...
-template <typename Io, typename Cache>
-__global__ void __launch_bounds__(32) attention_kernel(AttnArgs a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  const int kh = h / (a.heads / a.kv_heads);
+// One part of a split request as a warp or CTA holds it.
+struct Span {
+  long long unit0;         // its first unit on the line
+  int row, hq;             // request; kv head and pass
+  int k0, k1, units;       // its units of the request's `units`
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  if constexpr (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// (lo, hi) as two 16-bit values of the product's type, and what that lost.
+template <bool BF>
+__device__ __forceinline__ void split16(float lo, float hi, uint32_t &big, uint32_t &rest) {
+  if constexpr (BF) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(lo - __low2float(b), hi - __high2float(b));
+    big = *reinterpret_cast<const uint32_t *>(&b), rest = *reinterpret_cast<const uint32_t *>(&r);
+  } else {
+    const __half2 b = __floats2half2_rn(lo, hi);
+    const __half2 r = __floats2half2_rn(lo - __low2float(b), hi - __high2float(b));
+    big = *reinterpret_cast<const uint32_t *>(&b), rest = *reinterpret_cast<const uint32_t *>(&r);
+  }
+}
+
+template <typename Io>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&b);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 b = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&b);
+}
+
+__device__ __forceinline__ int row_len(const AttnArgs &a, int b) {
   const long long top = (long long)a.max_pages << a.shift;
-  int len = a.lens[b];
+  const int len = __ldg(a.lens + b);
   if (len < 0 || len > top) {
     report_timeout(&g_attention_status, kSiteLen);
-    len = len < 0 ? 0 : (int)top;
+    return len < 0 ? 0 : (int)top;
   }
-  const float ks = a.k_scale ? a.k_scale[kh] : 1.f, vs = a.v_scale ? a.v_scale[kh] : 1.f;
-  float q[4], o[4] = {};
+  return len;
+}
+
+// A place on the line of units. Requests of length 0 have none.
+struct Cursor {
+  int row, hq, k, len, units;
+  __device__ __forceinline__ void next_row(const AttnArgs &a) {
+    k = hq = 0;
+    do {
+      if (++row >= a.seqs) {  // only if the lengths changed under the call: stay inside the buffers
+        row = a.seqs - 1, len = 0, units = 1;
+        return;
+      }
+      len = row_len(a, row);
+    } while (len == 0);
+    units = (len + kUnit - 1) / kUnit;
+  }
+  __device__ __forceinline__ void step(const AttnArgs &a) {
+    if (++k == units) {
+      k = 0;
+      if (++hq == a.kv_heads * a.tiles) next_row(a);
+    }
+  }
+};
+
+// Writes the normalised output of query head `head` (within its request),
+// dimensions d .. d + 7, and its lse.
+template <typename Io>
+__device__ __forceinline__ void store_out8(const AttnArgs &a, int row, int head, int d, const float (&x)[8]) {
+  uint4 w;
+  w.x = pack2<Io>(x[0], x[1]), w.y = pack2<Io>(x[2], x[3]), w.z = pack2<Io>(x[4], x[5]), w.w = pack2<Io>(x[6], x[7]);
+  *reinterpret_cast<uint4 *>(static_cast<Io *>(a.out) + row * a.out_ld + (long long)head * a.dim + d) = w;
+}
+
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Joins `count` parts, part(i) giving the i-th part's floats (O [heads][D],
+// then (max, sum) per head): every thread takes 8 dimensions of a head.
+// emit(head, d, x, max, sum) gets the sums, not normalised.
+template <int D, int HEADS, class Part, class Emit>
+__device__ __forceinline__ void join_parts(int heads, int count, Part &&part, Emit &&emit) {
+  for (int u = threadIdx.x; u < heads * (D / 8); u += blockDim.x) {
+    const int h = u / (D / 8), d = 8 * (u % (D / 8));
+    float m = -INFINITY;
+    for (int i = 0; i < count; ++i) m = fmaxf(m, part(i)[HEADS * D + 2 * h]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x[8] = {};
+    for (int i = 0; i < count; ++i) {
+      const float *p = part(i);
+      const float f = exp2_approx(p[HEADS * D + 2 * h] - base);
+      l += f * p[HEADS * D + 2 * h + 1];
+      const float4 y = *reinterpret_cast<const float4 *>(p + h * D + d);
+      const float4 z = *reinterpret_cast<const float4 *>(p + h * D + d + 4);
+      x[0] += f * y.x, x[1] += f * y.y, x[2] += f * y.z, x[3] += f * y.w;
+      x[4] += f * z.x, x[5] += f * z.y, x[6] += f * z.z, x[7] += f * z.w;
+    }
+    emit(h, d, x, m, l);
+  }
+}
+
+template <int D, int NT, bool F8, typename Io>
+__global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kernel(AttnArgs a) {
+  using S = Shape<D, NT, F8>;
+  constexpr bool BF = !F8 && std::is_same<Io, __nv_bfloat16>::value;  // type of the products
+  constexpr int W = S::kWarps, ST = S::kStages;
+  extern __shared__ __align__(128) uint8_t smem[];
+  // units of the requests up to each thread's last, per kv head and pass; in
+  // the place of the warps' first parts until every warp has found its share
+  int *const ends = reinterpret_cast<int *>(smem + (size_t)W * S::kRing);
+  __shared__ Span spans[2 * W];
+  __shared__ int span_used[2 * W], members[2 * W], scratch[32], any_empty, is_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int passes = a.kv_heads * a.tiles;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- the line of units: prefix sums over the requests
+  if (tid == 0) any_empty = 0;
+  if (tid < 2 * W) span_used[tid] = 0;
+  __syncthreads();
+  const int per = (a.seqs + S::kThreads - 1) / S::kThreads;
+  int mine = 0;
+  for (int b = tid * per; b < min(a.seqs, (tid + 1) * per); ++b) {
+    const int len = row_len(a, b);
+    mine += (len + kUnit - 1) / kUnit;
+    if (len == 0) any_empty = 1;
+  }
+  int sum;
+  ends[tid] = block_inclusive_sum(mine, scratch, sum);
+  __syncthreads();
+  if (any_empty) {
+    const float zero[8] = {};
+    for (int b = blockIdx.x; b < a.seqs; b += gridDim.x) {
+      if (row_len(a, b) != 0) continue;
+      for (int u = tid; u < a.heads * (a.dim >> 3); u += S::kThreads)
+        store_out8<Io>(a, b, u / (a.dim >> 3), 8 * (u % (a.dim >> 3)), zero);
+      for (int h = tid; a.lse != nullptr && h < a.heads; h += S::kThreads) a.lse[(size_t)b * a.heads + h] = -INFINITY;
+    }
+  }
+  // Shares of the line, per warp. Where there are fewer units than CTAs the
+  // last CTAs have none: each of the others has one at least, which the count
+  // of arrivals at a join relies on.
+  const long long line = (long long)sum * passes;
+  const long long ctas = min((long long)gridDim.x, line);
+  if ((long long)blockIdx.x >= ctas) return;
+  const long long all_warps = ctas * W;
+  const long long gw = (long long)blockIdx.x * W + warp;
+  const long long u0 = gw * line / all_warps, u1 = (gw + 1) * line / all_warps;
+  const int count = (int)(u1 - u0);
+
+  const uint32_t ring = smem_u32(smem) + (uint32_t)warp * S::kRing;
+  float *const part0 = reinterpret_cast<float *>(smem + (size_t)W * S::kRing) + warp * S::kPart;
+  float *const part1 = reinterpret_cast<float *>(smem + (size_t)warp * S::kRing);
+
+  // ---- where the share begins
+  Cursor at = {0, 0, 0, 0, 1};
+  if (count > 0) {
+    int lo = 0, hi = S::kThreads - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((long long)ends[mid] * passes > u0) hi = mid; else lo = mid + 1;
+    }
+    long long before = lo > 0 ? ends[lo - 1] : 0;
+    const int last = min(a.seqs, (lo + 1) * per) - 1;
+    for (at.row = lo * per;; ++at.row) {
+      at.len = row_len(a, at.row);
+      at.units = (at.len + kUnit - 1) / kUnit;
+      if (at.row >= last || (before + at.units) * passes > u0) break;
+      before += at.units;
+    }
+    at.units = max(1, at.units);
+    const long long in = u0 - before * passes;
+    at.hq = (int)min((long long)passes - 1, in / at.units);
+    at.k = (int)(in - (long long)at.hq * at.units);
+  }
+  __syncthreads();
+
+  if (count > 0) {
+    Cursor look = at;  // the unit whose page is looked up next
+    int look_page = 0, look_key = 0, look_hq = 0;
+    bool look_live = false;
+    int looked = 0, issued = 0;
+    auto look_up = [&] {  // lane l < 16: the page of the unit's key l
+      look_key = look.k * kUnit + (lane & 15);
+      look_hq = look.hq;
+      look_live = looked < count && look_key < look.len;
+      look_page = 0;
+      if (look_live) look_page = __ldg(a.table + (size_t)look.row * a.max_pages + (look_key >> a.shift));
+      if (++looked < count) look.step(a);
+    };
+    const int dim_bytes = a.dim * S::kItem;
+    auto issue = [&] {  // copies the looked-up unit into its stage, then looks up the next
+      if (issued < count) {
+        long long off = -1;
+        if (look_live) {
+          if ((unsigned)look_page < (unsigned)a.pages)
+            off = look_page * a.page_stride + (look_key & ((1 << a.shift) - 1)) * a.token_stride +
+                  (look_hq / a.tiles) * a.head_stride;
+          else
+            report_timeout(&g_attention_status, kSitePage);
+        }
+        const uint32_t st = ring + (uint32_t)(issued % ST) * S::kStageBytes;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 32 * i;
-    q[i] = d < a.dim ? as_float(static_cast<const Io *>(a.q)[b * a.q_ld + h * a.dim + d]) * ks * a.scale : 0.f;
+        for (int r = 0; r < 2; ++r) {  // keys g and g + 8, pieces t, t + 4, ...
+          const long long o = __shfl_sync(0xffffffffu, off, g + 8 * r);
+          const char *src = a.k + (o < 0 ? 0 : o) + 16 * t;
+#pragma unroll
+          for (int c = 0; c < S::kKeyChunks; ++c) {
+            const bool live = o >= 0 && 16 * (t + 4 * c) < dim_bytes;
+            cp16(st + (r * S::kKeyChunks + c) * 512 + 16 * lane, live ? src + 64 * c : a.k, live ? 16 : 0);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // values 2t, 2t + 1, 2t + 8, 2t + 9, pieces g, g + 8, ...
+          const long long o = __shfl_sync(0xffffffffu, off, 2 * t + (r & 1) + 8 * (r >> 1));
+          const char *src = a.v + (o < 0 ? 0 : o) + S::kValBytes * g;
+#pragma unroll
+          for (int c = 0; c < S::kValChunks; ++c) {
+            const bool live = o >= 0 && S::kValBytes * (g + 8 * c) < dim_bytes;
+            const uint32_t dst = st + S::kKeyBytes + (r * S::kValChunks + c) * (32 * S::kValBytes) + S::kValBytes * lane;
+            const void *from = live ? src + 8 * S::kValBytes * c : a.v;
+            if constexpr (S::kValBytes == 16) cp16(dst, from, live ? 16 : 0); else cp8(dst, from, live ? 8 : 0);
+          }
+        }
+        ++issued;
+        look_up();
+      }
+      cp_commit();
+    };
+    look_up();
+    for (int s = 0; s < ST - 1; ++s) issue();
+
+    // ---- the share
+    uint32_t q[NT][D / 8];       // this lane's part of the contracted dimension, heads 8 nt + g
+    float cs[NT][2];             // score factor (base 2) of heads 8 nt + 2t, + 1
+    float m[NT][2], l[NT][2];    // running maximum (base 2) and this lane's sum
+    float o[NT][S::kVals / 2][4];
+    int k0 = at.k;               // first unit of the current request part
+    long long start = u0;
+    bool fresh = true;
+    for (int it = 0; it < count; ++it) {
+      if (fresh) {
+        fresh = false;
+        const int kh = at.hq / a.tiles, h0 = (at.hq % a.tiles) * S::kHeads;
+        const float ks = a.k_scale != nullptr ? __ldg(a.k_scale + kh) : 1.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int h = h0 + 8 * nt + g;
+          const Io *src = static_cast<const Io *>(a.q) + at.row * a.q_ld + (long long)(kh * a.group + h) * a.dim;
+          uint4 raw[D / 32];
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            // element run of 8: for 16-bit caches chunk t + 4c, for 8-bit ones half of a 16-element chunk
+            const int d = F8 ? 16 * (t + 4 * (c >> 1)) + 8 * (c & 1) : 8 * (t + 4 * c);
+            raw[c] = h < a.group && d < a.dim ? __ldg(reinterpret_cast<const uint4 *>(src + d)) : make_uint4(0, 0, 0, 0);
+          }
+          float f = a.scale * kLog2e * ks;
+          if constexpr (F8) {
+            // The 8-bit cache's products are f16. q is brought into f16's
+            // range by a power of two per head (exact but for elements 2^-14
+            // below the largest), which the score factor takes back.
+            float x[D / 4], top = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              const Io *e = reinterpret_cast<const Io *>(&raw[c]);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[8 * c + i] = to_float(e[i]), top = fmaxf(top, fabsf(x[8 * c + i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^e above top, kept where both powers are normal
+            const int e = min(126, max(-126, (int)(__float_as_uint(top) >> 23) - 126));
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) q[nt][i] = pack2<__half>(x[2 * i] * down, x[2 * i + 1] * down);
+            f *= up;
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c)
+              q[nt][4 * c] = raw[c].x, q[nt][4 * c + 1] = raw[c].y, q[nt][4 * c + 2] = raw[c].z, q[nt][4 * c + 3] = raw[c].w;
+          }
+          // the factor of head 8 nt + g lives in lanes 4g ..; this lane's columns are 2t, 2t + 1
+          cs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
+          cs[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+          m[nt][0] = m[nt][1] = -INFINITY;
+          l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        }
+      }
+      cp_wait<ST - 2>();
+      issue();  // into the stage that the previous unit left
+      const uint32_t st = ring + (uint32_t)(it % ST) * S::kStageBytes;
+      // ---- scores: 16 keys x 8 NT heads
+      float s[NT][4], s2[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < S::kKeyChunks; ++c) {
+        const uint4 x = lds16(st + c * 512 + 16 * lane), y = lds16(st + (S::kKeyChunks + c) * 512 + 16 * lane);
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (F8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma<BF>((j & 1) ? s2[nt] : s[nt], e4m3x2_to_f16x2(xw[j]), e4m3x2_to_f16x2(yw[j]),
+                      e4m3x2_to_f16x2(xw[j] >> 16), e4m3x2_to_f16x2(yw[j] >> 16), q[nt][8 * c + 2 * j],
+                      q[nt][8 * c + 2 * j + 1]);
+          } else {
+            mma<BF>(s[nt], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
+            mma<BF>(s2[nt], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
+          }
+        }
+      }
+      // ---- softmax: keys g (elements 0, 1) and g + 8 (2, 3) of heads 2t, 2t + 1
+      const int key = at.k * kUnit + g;
+      uint32_t big[NT][2], rest[NT][2];
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[nt][i] = key + 8 * (i >> 1) < at.len ? (s[nt][i] + s2[nt][i]) * cs[nt][i & 1] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(s[nt][j], s[nt][j + 2]);
+      }
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) grew = grew || top[nt][0] > m[nt][0] || top[nt][1] > m[nt][1];
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float mn = fmaxf(m[nt][j], top[nt][j]);
+            const float f = mn == -INFINITY ? 1.f : exp2_approx(m[nt][j] - mn);
+            m[nt][j] = mn;
+            l[nt][j] *= f;
+#pragma unroll
+            for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][j] *= f, o[nt][i][j + 2] *= f;
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float base = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
+          p[i] = exp2_approx(s[nt][i] - base);
+        }
+        l[nt][0] += p[0] + p[2];
+        l[nt][1] += p[1] + p[3];
+        split16<BF>(p[0], p[1], big[nt][0], rest[nt][0]);
+        split16<BF>(p[2], p[3], big[nt][1], rest[nt][1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) big[nt][r] = transpose8x8(big[nt][r]), rest[nt][r] = transpose8x8(rest[nt][r]);
+      }
+      // ---- values: rows of V^T are this lane's kVals dimensions, in pairs (i, i + kVals / 2)
+      constexpr int kWords = S::kValBytes * S::kValChunks / 4;
+      uint32_t x[4][kWords];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < S::kValChunks; ++c) {
+          const uint32_t from = st + S::kKeyBytes + (r * S::kValChunks + c) * (32 * S::kValBytes) + S::kValBytes * lane;
+          if constexpr (S::kValBytes == 16) {
+            const uint4 y = lds16(from);
+            x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
+          } else {
+            const uint2 y = lds8(from);
+            x[r][0] = y.x, x[r][1] = y.y;
+          }
+        }
+      constexpr int kPer = 4 / S::kItem;  // elements of a word
+#pragma unroll
+      for (int i = 0; i < S::kVals / 2; ++i) {
+        uint32_t v[4];  // (row g | g + 8) x (keys 2t, 2t + 1 | 2t + 8, 2t + 9)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int e = i + (r & 1) * (S::kVals / 2), w = e / kPer, b = e % kPer, pr = 2 * (r >> 1);
+          if constexpr (F8)
+            v[r] = e4m3x2_to_f16x2(__byte_perm(x[pr][w], x[pr + 1][w], b | (4 + b) << 4));
+          else
+            v[r] = __byte_perm(x[pr][w], x[pr + 1][w], b ? 0x7632 : 0x5410);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], big[nt][0], big[nt][1]);
+          mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], rest[nt][0], rest[nt][1]);
+        }
+      }
+
+      // ---- end of the request's keys, or of the share
+      const bool ends_here = at.k + 1 == at.units;
+      if (ends_here || it + 1 == count) {
+        const int kh = at.hq / a.tiles, h0 = (at.hq % a.tiles) * S::kHeads;
+        const bool whole = ends_here && k0 == 0;
+        const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
+        const int slot = start == u0 ? 0 : 1;
+        float *part = slot ? part1 : part0;
+        if (slot && !whole) {  // the ring is the second part's place: only after the last unit
+          cp_wait<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float sum = l[nt][j];
+#pragma unroll
+            for (int y = 4; y < 32; y <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+            const int h = 8 * nt + 2 * t + j;
+            const bool live = h0 + h < a.group;
+            const float f = whole ? vs / sum : 1.f;
+            constexpr int kRun = S::kValBytes / S::kItem;  // consecutive dimensions of a piece
+#pragma unroll
+            for (int e0 = 0; e0 < S::kVals; e0 += 8) {
+              const int d = (g + 8 * (e0 / kRun)) * kRun + e0 % kRun;
+              float y[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                y[i] = o[nt][e % (S::kVals / 2)][j + 2 * (e / (S::kVals / 2))] * f;
+              }
+              if (!whole) {
+                *reinterpret_cast<float4 *>(part + h * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4 *>(part + h * D + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
+              } else if (live && d < a.dim) {
+                store_out8<Io>(a, at.row, kh * a.group + h0 + h, d, y);
+              }
+            }
+            if (g == 0) {
+              if (!whole) {
+                part[S::kHeads * D + 2 * h] = m[nt][j];
+                part[S::kHeads * D + 2 * h + 1] = sum;
+              } else if (live && a.lse != nullptr) {
+                a.lse[(size_t)at.row * a.heads + kh * a.group + h0 + h] = m[nt][j] * kLn2 + logf(sum);
+              }
+            }
+          }
+        if (!whole && lane == 0) {
+          spans[2 * warp + slot] = {start, at.row, at.hq, k0, at.k + 1, at.units};
+          span_used[2 * warp + slot] = 1;
+        }
+        fresh = true;
+        start = u0 + it + 1;
+        k0 = 0;
+      }
+      if (it + 1 < count) at.step(a);
+    }
+    cp_wait<0>();
   }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < len; ++j) {
-    const int page = a.table[(size_t)b * a.max_pages + (j >> a.shift)];
-    if ((unsigned)page >= (unsigned)a.pages) {
-      report_timeout(&g_attention_status, kSitePage);
+  __syncthreads();
+
+  // ---- parts of the CTA's warps, joined in the order of the keys
+  auto warp_part = [&](int e) {
+    const int w = e >> 1;
+    return (e & 1) ? reinterpret_cast<const float *>(smem + (size_t)w * S::kRing)
+                   : reinterpret_cast<const float *>(smem + (size_t)W * S::kRing) + w * S::kPart;
+  };
+  for (int e = 0; e < 2 * W;) {
+    if (!span_used[e]) {
+      ++e;
       continue;
     }
-    const long long at = page * a.page_stride + kh * a.head_stride + (j & ((1 << a.shift) - 1)) * a.token_stride;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      if (d < a.dim) s += q[i] * as_float(reinterpret_cast<const Cache *>(a.k)[at + d]);
+    const Span first = spans[e];
+    int n = 0, last = e, f = e;
+    for (; f < 2 * W; ++f) {
+      if (!span_used[f]) continue;
+      if (spans[f].row != first.row || spans[f].hq != first.hq) break;
+      if (tid == 0) members[n] = f;
+      ++n, last = f;
     }
+    e = f;
+    __syncthreads();
+    const int kh = first.hq / a.tiles, h0 = (first.hq % a.tiles) * S::kHeads;
+    const int heads = min(S::kHeads, a.group - h0);
+    const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
+    auto finish = [&](int h, int d, const float (&x)[8], float m, float l) {
+      const float f = vs / l;
+      float y[8];
 #pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - base), p = expf(s - base);
-    m = mn, l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      if (d < a.dim) o[i] = o[i] * f + p * as_float(reinterpret_cast<const Cache *>(a.v)[at + d]);
+      for (int i = 0; i < 8; ++i) y[i] = x[i] * f;
+      if (d < a.dim) store_out8<Io>(a, first.row, kh * a.group + h0 + h, d, y);
+      if (d == 0 && a.lse != nullptr)
+        a.lse[(size_t)first.row * a.heads + kh * a.group + h0 + h] = m * kLn2 + logf(l);
+    };
+    const bool here = first.k0 == 0 && spans[last].k1 == first.units;
+    auto member = [&](int i) { return warp_part(members[i]); };
+    if (here) {
+      join_parts<D, S::kHeads>(heads, n, member, finish);
+    } else {
+      // across CTAs: place 1 holds the part of a request that begins in this
+      // CTA, place 0 of one that began before
+      float *place = a.parts + ((size_t)blockIdx.x * 2 + (first.k0 == 0)) * kPartFloats;
+      join_parts<D, S::kHeads>(heads, n, member, [&](int h, int d, const float (&x)[8], float m, float l) {
+        __stcg(reinterpret_cast<float4 *>(place + h * D + d), make_float4(x[0], x[1], x[2], x[3]));
+        __stcg(reinterpret_cast<float4 *>(place + h * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
+        if (d == 0) __stcg(place + S::kHeads * D + 2 * h, m), __stcg(place + S::kHeads * D + 2 * h + 1, l);
+      });
+      // CTAs of the request's first and last unit
+      const long long b0 = first.unit0 - first.k0, b1 = b0 + first.units - 1;
+      const int c0 = (int)(((b0 + 1) * all_warps - 1) / line / W), c1 = (int)(((b1 + 1) * all_warps - 1) / line / W);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        is_last = atomicAdd(a.arrivals + c0, 1) == c1 - c0;
+        if (is_last) a.arrivals[c0] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (is_last)
+        join_parts<D, S::kHeads>(heads, c1 - c0 + 1, [&](int i) {
+          return const_cast<const float *>(a.parts) + ((size_t)(c0 + i) * 2 + (i == 0)) * kPartFloats;
+        }, finish);
     }
+    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 32 * i;
-    if (d < a.dim)
-      static_cast<Io *>(a.out)[b * a.out_ld + h * a.dim + d] = from_float<Io>(len ? o[i] * vs / l : 0.f);
-  }
-  if (lane == 0 && a.lse) a.lse[(size_t)b * a.heads + h] = len ? m + logf(l) : -INFINITY;
 }
+
+template <int D, int NT, bool F8, typename Io>
+int launch_attention(const AttnArgs &a, int grid, cudaStream_t s) {
+  using S = Shape<D, NT, F8>;
+  static bool done[64] = {};
+  int dev = 0;
+  CE_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    CE_CUDA_TRY(cudaFuncSetAttribute(attention_kernel<D, NT, F8, Io>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)S::kSmem));
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  return launch_kernel(attention_kernel<D, NT, F8, Io>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, s, true,
+                       "attention_kernel", a);
+}
+
+template <bool F8, typename Io>
+int dispatch_attention(const AttnArgs &a, int grid, cudaStream_t s) {
+  if (a.dim <= 64)
+    return a.group <= 8 ? launch_attention<64, 1, F8, Io>(a, grid, s) : launch_attention<64, 2, F8, Io>(a, grid, s);
+  return a.group <= 8 ? launch_attention<128, 1, F8, Io>(a, grid, s) : launch_attention<128, 2, F8, Io>(a, grid, s);
+}
+
+size_t workspace_bytes_of(int grid) { return 4ull * kMaxGrid + (size_t)grid * 2 * kPartFloats * 4; }
 
 }  // namespace
 }  // namespace paged
 
 using namespace paged;
 
+// Reads and clears the status word of the attention kernels.
 int paged_attention_status() {
   CE_CUDA_TRY(cudaDeviceSynchronize());
   DeviceStatus h{};
@@ -111,7 +718,7 @@ extern "C" {
 
 int ce_paged_attention_workspace(size_t *bytes) {
   CE_REQUIRE(bytes != nullptr, "null argument");
-  *bytes = 16;
+  *bytes = workspace_bytes_of(std::min(sm_count(), kMaxGrid));
   return CE_OK;
 }
 
@@ -130,12 +737,13 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
              kv->type);
   CE_REQUIRE(heads >= 1 && heads % kv->kv_heads == 0, "heads must be a multiple of kv_heads (got %d, %d)", heads,
              kv->kv_heads);
+  CE_REQUIRE((int64_t)pt->seqs * ((int64_t)pt->max_pages * pt->page_size / kUnit + 1) < (1ll << 31),
+             "seqs x max_pages x page_size must be below 2^35");
   const int64_t row = (int64_t)heads * kv->head_dim;
   CE_REQUIRE(aligned16(q) && aligned16(out) && q_ld % 8 == 0 && out_ld % 8 == 0 && q_ld >= row && out_ld >= row,
              "q and out must be 16-byte aligned, their row strides multiples of 8 and at least heads * head_dim");
-  size_t need = 0;
-  rc = ce_paged_attention_workspace(&need);
-  if (rc != CE_OK) return rc;
+  const int grid = std::min(sm_count(), kMaxGrid);
+  const size_t need = workspace_bytes_of(grid);
   CE_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
              "the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
   AttnArgs a = {};
@@ -146,17 +754,19 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   a.k_scale = kv->k_scale_dev, a.v_scale = kv->v_scale_dev;
   a.table = pt->table_dev, a.lens = pt->lens_dev;
   a.q_ld = q_ld, a.out_ld = out_ld;
-  a.page_stride = kv->page_stride, a.head_stride = kv->head_stride, a.token_stride = kv->token_stride;
+  a.page_stride = kv->page_stride * b, a.head_stride = kv->head_stride * b, a.token_stride = kv->token_stride * b;
   a.seqs = pt->seqs, a.max_pages = pt->max_pages, a.pages = kv->pages;
   a.heads = heads, a.kv_heads = kv->kv_heads, a.dim = kv->head_dim, a.shift = log2_of(kv->page_size);
+  a.group = heads / kv->kv_heads;
+  a.tiles = a.group <= 8 ? 1 : (a.group + kMaxSplitHeads - 1) / kMaxSplitHeads;
   a.scale = scale;
-  const dim3 grid((unsigned)heads, (unsigned)pt->seqs);
+  a.arrivals = static_cast<int *>(workspace);
+  a.parts = reinterpret_cast<float *>(a.arrivals + kMaxGrid);
   const cudaStream_t s = (cudaStream_t)stream;
-  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, dim3(32), 0, s, true, "attention_kernel", a); };
-  if (kv->type == CE_TYPE_BF16) return go(attention_kernel<__nv_bfloat16, __nv_bfloat16>);
-  if (kv->type == CE_TYPE_F16) return go(attention_kernel<__half, __half>);
-  return io_type == CE_TYPE_F16 ? go(attention_kernel<__half, __nv_fp8_e4m3>)
-                                : go(attention_kernel<__nv_bfloat16, __nv_fp8_e4m3>);
+  if (kv->type == CE_TYPE_BF16) return dispatch_attention<false, __nv_bfloat16>(a, grid, s);
+  if (kv->type == CE_TYPE_F16) return dispatch_attention<false, __half>(a, grid, s);
+  return io_type == CE_TYPE_F16 ? dispatch_attention<true, __half>(a, grid, s)
+                                : dispatch_attention<true, __nv_bfloat16>(a, grid, s);
 }
 
 }  // extern "C"
