@@ -1004,8 +1004,27 @@ def llama_shard_rows(cfg, rank, world, which):
 # --------------------------------------------------------------------------
 # Paged key-value cache and beam search (ce_paged_*, ce_beam_*)
 
+# A decode step makes these calls once per layer, so their Python side is kept
+# short: structures and pointers of the long-lived objects are made once, and
+# each argument is checked by a few identity comparisons (about 6 us a call).
 TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_E4M3 = 0, 1, 2, 3
-_TYPES = {}  # torch dtype -> CE_TYPE_*, filled on first use
+_TYPES = {}  # torch dtype -> CE_TYPE_*
+_I32 = _I64 = _F32 = _BOOL = _raw_stream = _device = _L = None  # torch dtypes and functions, set by _paged_setup
+
+
+def _paged_setup():
+    """torch is imported on first use of a paged operator."""
+    global _I32, _I64, _F32, _BOOL, _raw_stream, _device, _L
+    import torch
+    _I32, _I64, _F32, _BOOL = torch.int32, torch.int64, torch.float32, torch.bool
+    _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16,
+                   torch.float8_e4m3fn: TYPE_E4M3})
+    _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+    _L = lib()
+
+
+def _stream_of(stream):
+    return _raw_stream(_device()) if stream is None else _stream(stream)
 
 
 class _PagedKVStruct(ctypes.Structure):
@@ -1020,10 +1039,6 @@ class _PageTableStruct(ctypes.Structure):
 
 
 def _type(t, what):
-    if not _TYPES:
-        import torch
-        _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16,
-                       torch.float8_e4m3fn: TYPE_E4M3})
     code = _TYPES.get(t.dtype)
     if code is None:
         raise TypeError(f"{what}: unsupported dtype {t.dtype}")
@@ -1034,7 +1049,7 @@ def _dense(t, name, dtype, count=None):
     """Pointer of a contiguous device tensor of `dtype` with `count` elements (None: NULL)."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or not t.is_cuda or not t.is_contiguous():
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} device tensor (got {t.dtype}, {t.device})")
     if count is not None and t.numel() != count:
         raise ValueError(f"{name} must have {count} elements (got {t.numel()})")
@@ -1043,10 +1058,10 @@ def _dense(t, name, dtype, count=None):
 
 def _heads_of(t, name, tokens, heads, dim):
     """(pointer, token stride) of a [tokens][heads][dim] tensor whose heads are contiguous."""
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or t.shape[2] != dim or not t.is_cuda:
+    if t.shape != (tokens, heads, dim) or not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor [{tokens}][{heads}][{dim}] (got {tuple(t.shape)})")
     ld, sh, sd = t.stride()
-    if (sd != 1 and dim > 1) or (sh != dim and heads > 1):
+    if sd != 1 or (sh != dim and heads > 1):
         raise ValueError(f"{name}: the heads of a token must be contiguous (strides {t.stride()})")
     return t.data_ptr(), ld if tokens > 1 else max(ld, heads * dim)
 
@@ -1061,6 +1076,8 @@ class PagedKV:
     (paged_attention_workspace)."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
+        if _L is None:
+            _paged_setup()
         if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
             raise ValueError("k and v must be [layers][pages][kv_heads][page_size][head_dim] of one type and layout")
         if not (k.is_cuda and v.is_cuda) or (k.stride(4) != 1 and k.shape[4] > 1):
@@ -1069,8 +1086,8 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = L, P, H, S, D
         st = k.stride()
-        self._c = _PagedKVStruct(k.data_ptr(), v.data_ptr(), _dense(k_scale, "k_scale", "torch.float32", H),
-                                 _dense(v_scale, "v_scale", "torch.float32", H), _type(k, "cache"), L, P, H, S, D,
+        self._c = _PagedKVStruct(k.data_ptr(), v.data_ptr(), _dense(k_scale, "k_scale", _F32, H),
+                                 _dense(v_scale, "v_scale", _F32, H), _type(k, "cache"), L, P, H, S, D,
                                  st[0], st[1], st[2], st[3])
         self._p = ctypes.addressof(self._c)
         self._ws = None
@@ -1086,13 +1103,15 @@ class PageTable:
     int32 [pages] (rows that hold each page; 0 = free)."""
 
     def __init__(self, table, lens, refs, page_size):
+        if _L is None:
+            _paged_setup()
         if table.dim() != 2:
             raise ValueError(f"table must be [seqs][max_pages] (got {tuple(table.shape)})")
         n, P = table.shape
         self.table, self.lens, self.refs, self.page_size = table, lens, refs, page_size
         self.seqs, self.max_pages, self.pages = n, P, refs.numel()
-        self._c = _PageTableStruct(_dense(table, "table", "torch.int32"), _dense(lens, "lens", "torch.int32", n),
-                                   _dense(refs, "refs", "torch.int32"), n, P, refs.numel(), page_size)
+        self._c = _PageTableStruct(_dense(table, "table", _I32), _dense(lens, "lens", _I32, n),
+                                   _dense(refs, "refs", _I32), n, P, refs.numel(), page_size)
         self._p = ctypes.addressof(self._c)
 
     @classmethod
@@ -1109,10 +1128,10 @@ def paged_resize(pt, new_lens, slots, pos, starts=None, status=None, out=None, s
     tokens; in place, or into the PageTable `out` (ce_paged_resize)."""
     out = pt if out is None else out
     cap = slots.numel()
-    check(lib().ce_paged_resize(out._p, pt._p, _dense(new_lens, "new_lens", "torch.int32", pt.seqs),
-                                _dense(slots, "slots", "torch.int64"), _dense(pos, "pos", "torch.int32", cap), cap,
-                                _dense(starts, "starts", "torch.int32", pt.seqs + 1),
-                                _dense(status, "status", "torch.int32", 4), _stream(stream)))
+    check(_L.ce_paged_resize(out._p, pt._p, _dense(new_lens, "new_lens", _I32, pt.seqs),
+                                _dense(slots, "slots", _I64), _dense(pos, "pos", _I32, cap), cap,
+                                _dense(starts, "starts", _I32, pt.seqs + 1),
+                                _dense(status, "status", _I32, 4), _stream_of(stream)))
 
 
 def paged_append(kv, q_out, q, k, v, slots, pos=None, rope=None, layer=0, stream=None):
@@ -1126,15 +1145,15 @@ def paged_append(kv, q_out, q, k, v, slots, pos=None, rope=None, layer=0, stream
     if q is not None:
         heads = q.shape[1]
         qp, q_ld = _heads_of(q, "q", T, heads, D)
-        qo, qt = _dense(q_out, "q_out", str(q_out.dtype), T * heads * D), _type(q_out, "q_out")
+        qo, qt = _dense(q_out, "q_out", q_out.dtype, T * heads * D), _type(q_out, "q_out")
     if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
         raise TypeError("q, k and v must have one dtype")
     if rope is not None and (rope.dim() != 3 or rope.shape[1] * 2 != D or rope.shape[2] != 2):
         raise ValueError(f"rope must be [positions][{D // 2}][2] (got {tuple(rope.shape)})")
-    check(lib().ce_paged_append(kv._p, layer, qo, qt, qp, kp, vp, _type(k, "k"), q_ld, k_ld, v_ld,
-                                _dense(slots, "slots", "torch.int64"), _dense(pos, "pos", "torch.int32", T), T, heads,
-                                _dense(rope, "rope", "torch.float32"), 0 if rope is None else rope.shape[0],
-                                _stream(stream)))
+    check(_L.ce_paged_append(kv._p, layer, qo, qt, qp, kp, vp, _type(k, "k"), q_ld, k_ld, v_ld,
+                                _dense(slots, "slots", _I64), _dense(pos, "pos", _I32, T), T, heads,
+                                _dense(rope, "rope", _F32), 0 if rope is None else rope.shape[0],
+                                _stream_of(stream)))
     return q_out
 
 
@@ -1157,9 +1176,9 @@ def paged_attention(kv, out, q, pt, lse=None, scale=None, layer=0, workspace=Non
     if q.dtype != out.dtype:
         raise TypeError("q and out must have one dtype")
     ws = kv.workspace() if workspace is None else workspace
-    check(lib().ce_paged_attention(kv._p, layer, pt._p, op, _dense(lse, "lse", "torch.float32", n * heads), qp,
+    check(_L.ce_paged_attention(kv._p, layer, pt._p, op, _dense(lse, "lse", _F32, n * heads), qp,
                                    _type(q, "q"), heads, q_ld, o_ld, D ** -0.5 if scale is None else scale,
-                                   ws.data_ptr(), ws.numel(), _stream(stream)))
+                                   ws.data_ptr(), ws.numel(), _stream_of(stream)))
     return out
 
 
@@ -1176,17 +1195,19 @@ def beam_select(scores_out, parents, tokens, finished_out, logits, scores, finis
     float32 and finished bool [batch][beams]; into scores_out, parents and
     tokens (int32) and finished_out (bool), all [batch][beams]
     (ce_beam_select). eos -1: no token ends a beam."""
+    if _L is None:
+        _paged_setup()
     B, K = scores.shape
     n, V = B * K, logits.shape[1]
     if logits.dim() != 2 or logits.shape[0] != n or not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits must be a device tensor [{n}][vocab] with contiguous rows (got {tuple(logits.shape)})")
-    check(lib().ce_beam_select(_dense(scores_out, "scores_out", "torch.float32", n),
-                               _dense(parents, "parents", "torch.int32", n), _dense(tokens, "tokens", "torch.int32", n),
-                               _dense(finished_out, "finished_out", "torch.bool", n), logits.data_ptr(),
+    check(_L.ce_beam_select(_dense(scores_out, "scores_out", _F32, n),
+                               _dense(parents, "parents", _I32, n), _dense(tokens, "tokens", _I32, n),
+                               _dense(finished_out, "finished_out", _BOOL, n), logits.data_ptr(),
                                _type(logits, "logits"), logits.stride(0) if n > 1 else max(V, logits.stride(0)),
-                               _dense(scores, "scores", "torch.float32"),
-                               _dense(finished, "finished", "torch.bool", n), B, K, V, eos, pad, workspace.data_ptr(),
-                               workspace.numel(), _stream(stream)))
+                               _dense(scores, "scores", _F32),
+                               _dense(finished, "finished", _BOOL, n), B, K, V, eos, pad, workspace.data_ptr(),
+                               workspace.numel(), _stream_of(stream)))
 
 
 def paged_reorder(pt, parents, beams, out, kv=None, copies=None, status=None, stream=None):
@@ -1197,7 +1218,7 @@ def paged_reorder(pt, parents, beams, out, kv=None, copies=None, status=None, st
     if copies is None:
         import torch
         copies = torch.empty(pt.seqs, 2, dtype=torch.int32, device=pt.table.device)
-    check(lib().ce_paged_reorder(out._p, pt._p, _dense(parents, "parents", "torch.int32", pt.seqs), beams,
-                                 None if kv is None else kv._p, _dense(copies, "copies", "torch.int32", 2 * pt.seqs),
-                                 _dense(status, "status", "torch.int32", 4), _stream(stream)))
+    check(_L.ce_paged_reorder(out._p, pt._p, _dense(parents, "parents", _I32, pt.seqs), beams,
+                                 None if kv is None else kv._p, _dense(copies, "copies", _I32, 2 * pt.seqs),
+                                 _dense(status, "status", _I32, 4), _stream_of(stream)))
     return copies

@@ -1,6 +1,24 @@
 // Beam search selection: the best tokens of each beam, then the best beams x
-// tokens of each batch element.
+// tokens of each batch element, in one launch.
+//
+// The bound is one read of the logits. A row is cut into slices, one CTA
+// each, so that a few rows still occupy many SMs; a CTA reads its slice once,
+// in tiles held in registers, and keeps a running (max, sum) per thread and
+// the slice's `beams` best keys. A tile's candidates are found by a threshold
+// that is a lower bound of its beams-th best value: for the first tile the
+// beams-th largest of a warp's 32 lane maxima (the largest such over the
+// warps), later the worst key kept. On real logits a handful of values pass
+// it, and their ranks among themselves and the keys kept (counted, each
+// against all) put them in order. Keys are (logit, token) pairs as 64-bit
+// integers, all different, so the order is total and independent of the
+// order in which threads append.
+//
+// The last CTA of a batch element to arrive joins the slices: a warp per
+// beam plays the sorted lists of its slices off against one another (a lane
+// per slice), then one warp does the same with the beams' sorted offers.
 #include <float.h>
+
+#include <algorithm>
 
 #include "paged.cuh"
 
@@ -9,6 +27,12 @@ namespace paged {
 namespace {
 
 constexpr int kMaxBeams = 32;
+constexpr int kMaxGroups = 16384;  // batch elements: arrival counters at the front of the workspace
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kElems = 16;         // logits per thread and tile
+constexpr int kBuffer = 1024;      // candidates of a tile
+constexpr int kListKeys = 256;     // keys of one beam's lists at the join: slices x beams
 
 struct BeamArgs {
   float *scores_out;
@@ -18,17 +42,20 @@ struct BeamArgs {
   long long ld;
   const float *scores;
   const uint8_t *finished;
-  int batch, beams, vocab, eos, pad;
-  unsigned long long *best;  // [rows][beams]
-  float *lse;                // [rows]
+  int batch, beams, vocab, eos, pad, slices;
+  int *arrivals;             // [batch], zero between calls
+  unsigned long long *best;  // [rows][slices][beams], 0: none
+  float2 *sums;              // [rows][slices]: max, sum of e^(x - max)
 };
+
+constexpr float kLog2e = 1.44269504088896341f;
 
 // A logit as the selection takes it: NaN is -inf, +inf the largest finite
 // value, -0 is +0.
 template <typename T>
 __device__ __forceinline__ float logit_of(T v) {
   const float x = to_float(v);
-  return x != x ? -INFINITY : fminf(x, FLT_MAX) + 0.f;
+  return fminf(fmaxf(x, -INFINITY), FLT_MAX) + 0.f;  // fmaxf gives the number where the other is NaN
 }
 
 // Keys order tokens by (logit descending, token ascending) as integers.
@@ -43,97 +70,271 @@ __device__ __forceinline__ float key_logit(unsigned long long k) {
 }
 __device__ __forceinline__ int key_token(unsigned long long k) { return (int)~(uint32_t)k; }
 
-template <typename T>
-__device__ __forceinline__ T block_reduce_max(T v, T *scratch) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const T y = __shfl_xor_sync(0xffffffffu, v, o);
-    v = y > v ? y : v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v = scratch[w] > v ? scratch[w] : v;
-  return v;
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// One CTA per beam: its log sum, then its best tokens one after the other.
-template <typename T>
-__global__ void __launch_bounds__(256) rows_kernel(BeamArgs a) {
-  __shared__ unsigned long long best8[8];
-  __shared__ float red[8];
-  const int row = blockIdx.x;
-  const T *x = static_cast<const T *>(a.logits) + row * a.ld;
-  pdl_launch_dependents();
-  pdl_wait();
-  if (a.finished[row]) return;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) m = fmaxf(m, logit_of(x[i]));
-  m = block_reduce_max(m, red);
-  float sum = 0.f;
-  if (m > -INFINITY)
-    for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) sum += expf(logit_of(x[i]) - m);
+// The k-th largest of the warp's 32 values (k from 1).
+__device__ __forceinline__ float warp_kth(float v, int k) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) sum += red[w];
-    a.lse[row] = m + logf(sum);
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int step = size >> 1; step; step >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, v, step);
+      const bool up = ((lane & step) != 0) == ((lane & size) != 0);  // this lane keeps the larger one
+      v = up ? fmaxf(v, y) : fminf(v, y);
+    }
+  return __shfl_sync(0xffffffffu, v, k - 1);
+}
+
+// Joins (max, sum of e^(x - max)) pairs.
+__device__ __forceinline__ void add_sum(float &m, float &l, float m1, float l1) {
+  if (m1 > m) {
+    const float x = m;
+    m = m1, m1 = x;
+    const float y = l;
+    l = l1, l1 = y;
   }
+  if (m1 != -INFINITY) l += l1 * exp2_approx((m1 - m) * kLog2e);
+}
+
+struct Shared {
+  unsigned long long buffer[kWarps * kListKeys];  // candidates; at the join the lists, per warp
+  unsigned long long top[kMaxBeams], next[kMaxBeams];
+  float kth[kWarps];
+  float2 sums[kWarps];
+  unsigned long long round[kWarps];
+  float score[kMaxBeams][kMaxBeams];  // [beam][rank]
+  int token[kMaxBeams][kMaxBeams];
+  int count[2], last;  // candidates of even and odd tiles
+};
+static_assert(kBuffer + kMaxBeams <= kWarps * kListKeys, "candidates and keys kept");
+
+// A tile's `beams` best by taking the best that is below the last taken, once
+// per rank: for tiles where the threshold leaves too much (rows of equal
+// logits) or none (rows banned but for a few tokens).
+template <class Key>
+__device__ __forceinline__ int take_in_rounds(Shared &sh, int beams, Key &&key) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long last = ~0ull;
-  for (int r = 0; r < min(a.beams, a.vocab); ++r) {
+  int n = 0;
+  for (; n < beams; ++n) {
     unsigned long long k = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += blockDim.x) {
-      const unsigned long long c = key_of(logit_of(x[i]), i);
-      if (c < last && c > k) k = c;
+#pragma unroll
+    for (int i = 0; i <= kElems; ++i) {
+      const unsigned long long c = key(i);
+      k = c < last && c > k ? c : k;
     }
-    last = block_reduce_max(k, best8);
-    if (threadIdx.x == 0) a.best[(size_t)row * a.beams + r] = last;
-  }
-}
-
-// One warp per batch element: lane k walks down beam k's sorted offers.
-__global__ void __launch_bounds__(32) groups_kernel(BeamArgs a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int g = blockIdx.x, lane = threadIdx.x, row = g * a.beams + lane;
-  const bool beam = lane < a.beams;
-  const bool done = beam && a.finished[row] != 0;
-  float base = beam ? a.scores[row] : 0.f;
-  const float lse = beam && !done ? a.lse[row] : 0.f;
-  const int offers = !beam ? 0 : done ? 1 : min(a.beams, a.vocab);
-  int at = 0, token = a.pad;
-  float score = base;
-  auto load = [&] {
-    if (!done && at < offers) {
-      const unsigned long long k = a.best[(size_t)row * a.beams + at];
-      const float x = key_logit(k);
-      token = key_token(k);
-      score = x == -INFINITY ? -INFINITY : base + (x - lse);
-    }
-    if (score != score) score = -INFINITY;
-  };
-  load();
-  for (int r = 0; r < a.beams; ++r) {
-    // the best head; ties go to the lowest beam
-    unsigned long long k = at < offers ? key_of(score + 0.f, lane) : 0ull;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       const unsigned long long y = __shfl_xor_sync(0xffffffffu, k, o);
       k = y > k ? y : k;
     }
-    if (lane == key_token(k)) {
-      const size_t to = (size_t)g * a.beams + r;
-      a.scores_out[to] = score;
-      a.parents[to] = lane;
-      a.tokens[to] = token;
-      a.finished_out[to] = done || token == a.eos;
+    if (lane == 0) sh.round[warp] = k;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) k = sh.round[w] > k ? sh.round[w] : k;
+    __syncthreads();
+    if (k == 0) break;
+    if (threadIdx.x == 0) sh.buffer[n] = k;
+    last = k;
+  }
+  return n;
+}
+
+template <typename T>
+__device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int row, int slice) {
+  constexpr int kPerVec = 16 / sizeof(T), kVecs = kElems / kPerVec;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
+  const T *x = static_cast<const T *>(a.logits) + row * a.ld;
+  // 16-byte vectors of the row from its first aligned element on; the few
+  // elements before and after them go to the first and last slice, one per thread
+  const int head = min(a.vocab, (int)((16u - (unsigned)(reinterpret_cast<uintptr_t>(x) & 15u)) % 16u / sizeof(T)));
+  const int vecs = (a.vocab - head) / kPerVec, tail = a.vocab - head - vecs * kPerVec;
+  const int per = (vecs + a.slices - 1) / a.slices;
+  const int v0 = min(vecs, slice * per), v1 = min(vecs, v0 + per);
+  const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
+  int extra = -1;  // token of this thread's single element
+  if (slice == 0 && tid < head) extra = tid;
+  if (slice == a.slices - 1 && tid >= 128 && tid < 128 + tail) extra = a.vocab - tail + tid - 128;
+
+  float m = -INFINITY, l = 0.f;
+  if (tid < K) sh.top[tid] = 0;
+  if (tid == 0) sh.count[0] = sh.count[1] = 0;
+  const int tiles = max(1, (v1 - v0 + kThreads * kVecs - 1) / (kThreads * kVecs));
+  for (int tile = 0; tile < tiles; ++tile) {
+    float e[kElems + 1];
+    const int at = v0 + tile * kThreads * kVecs + tid;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      const bool live = at + v * kThreads < v1;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (live) raw = __ldcs(xv + at + v * kThreads);
+      const T *p = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int i = 0; i < kPerVec; ++i) e[v * kPerVec + i] = live ? logit_of(p[i]) : -INFINITY;
+    }
+    const bool single = tile == 0 && extra >= 0;
+    e[kElems] = single ? logit_of(x[extra]) : -INFINITY;
+    auto token = [&](int i) { return i == kElems ? extra : head + (at + i / kPerVec * kThreads) * kPerVec + i % kPerVec; };
+    auto live = [&](int i) { return i == kElems ? single : at + i / kPerVec * kThreads < v1; };
+    float top = e[0];
+#pragma unroll
+    for (int i = 1; i <= kElems; ++i) top = fmaxf(top, e[i]);
+    if (top > -INFINITY) {
+      float s = 0.f;
+      const float base = fmaxf(top, m);
+#pragma unroll
+      for (int i = 0; i <= kElems; ++i) s += exp2_approx((e[i] - base) * kLog2e);  // a difference cannot overflow upwards
+      l = l * exp2_approx((m - base) * kLog2e) + s;
+      m = base;
+    }
+    // candidates
+    bool rounds = false, full = false;
+    float bar;
+    if (tile == 0) {
+      const float kth = warp_kth(top, K);
+      if (lane == 0) sh.kth[warp] = kth;
+      __syncthreads();
+      bar = sh.kth[0];
+      for (int w = 1; w < kWarps; ++w) bar = fmaxf(bar, sh.kth[w]);
+      rounds = bar == -INFINITY;
+    } else {
+      full = sh.top[K - 1] != 0;  // then an equal value of a later token is no better
+      bar = full ? key_logit(sh.top[K - 1]) : -INFINITY;
+      rounds = !full;
+    }
+    if (!rounds && (full ? top > bar : top >= bar)) {
+#pragma unroll
+      for (int i = 0; i <= kElems; ++i)
+        if (full ? e[i] > bar : e[i] >= bar) {
+          const int n = atomicAdd(&sh.count[tile & 1], 1);
+          if (n < kBuffer) sh.buffer[n] = key_of(e[i], token(i));
+        }
+    }
+    __syncthreads();
+    int n = sh.count[tile & 1];
+    if (n == 0 && !rounds) continue;  // no barrier: the next tile counts in the other word
+    if (rounds || n > kBuffer)
+      n = take_in_rounds(sh, K, [&](int i) { return live(i) ? key_of(e[i], token(i)) : 0ull; });
+    // ranks among the candidates and the keys kept
+    if (tid < K) sh.buffer[n + tid] = sh.top[tid], sh.next[tid] = 0;
+    __syncthreads();
+    n += K;
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long k = sh.buffer[i];
+      int rank = 0;
+      for (int q = 0; q < n; ++q) rank += sh.buffer[q] > k;
+      if (k != 0 && rank < K) sh.next[rank] = k;
+    }
+    __syncthreads();
+    if (tid < K) sh.top[tid] = sh.next[tid];
+    if (tid == 0) sh.count[tile & 1] = 0;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
+  if (lane == 0) sh.sums[warp] = make_float2(m, l);
+  __syncthreads();
+  const size_t list = (size_t)row * a.slices + slice;
+  if (tid < K) __stcg(a.best + list * K + tid, sh.top[tid]);
+  if (tid == 0) {
+    for (int w = 1; w < kWarps; ++w) add_sum(m, l, sh.sums[w].x, sh.sums[w].y);
+    __stcg(a.sums + list, make_float2(m, l));
+  }
+}
+
+// The best key of the warp's lanes, and which lane holds it (keys differ).
+__device__ __forceinline__ bool warp_best(unsigned long long k) {
+  const uint32_t hi = (uint32_t)(k >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+  const uint32_t lo = hi == top ? (uint32_t)k : 0u;
+  const uint32_t low = __reduce_max_sync(0xffffffffu, lo);
+  return hi == top && lo == low && k != 0;
+}
+
+// The offers of one beam, best first, from the sorted lists of its slices.
+__device__ __forceinline__ int offers_of_row(const BeamArgs &a, Shared &sh, int group, int beam) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.beams;
+  const size_t row = (size_t)group * K + beam;
+  const float base = a.scores[row];
+  if (a.finished[row]) {
+    if (lane == 0) sh.score[beam][0] = base != base ? -INFINITY : base, sh.token[beam][0] = a.pad;
+    return 1;
+  }
+  unsigned long long *lists = sh.buffer + warp * kListKeys;
+  for (int i = lane; i < a.slices * K; i += 32) lists[i] = __ldcg(a.best + row * a.slices * K + i);
+  float m = -INFINITY, l = 0.f;
+  if (lane < a.slices) {
+    const float2 p = __ldcg(a.sums + row * a.slices + lane);
+    m = p.x, l = p.y;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
+  const float lse = m + logf(l);
+  __syncwarp();
+  int at = 0, r = 0;
+  const int n = min(K, a.vocab);
+  for (; r < n; ++r) {
+    const unsigned long long k = lane < a.slices && at < K ? lists[lane * K + at] : 0ull;
+    if (warp_best(k)) {
+      const float x = key_logit(k);
+      const float s = x == -INFINITY ? -INFINITY : base + (x - lse);
+      sh.score[beam][r] = s != s ? -INFINITY : s;
+      sh.token[beam][r] = key_token(k);
       ++at;
-      load();
     }
   }
+  return n;
+}
+
+// Grid (slices, beams, batch).
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) select_kernel(BeamArgs a) {
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, group = blockIdx.z;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = group * K + blockIdx.y;
+  if (!a.finished[row]) slice_of_row<T>(a, sh, row, blockIdx.x);
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    sh.last = atomicAdd(a.arrivals + group, 1) == K * a.slices - 1;
+    if (sh.last) a.arrivals[group] = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!sh.last) return;
+  for (int beam = warp; beam < K; beam += kWarps) {
+    offers_of_row(a, sh, group, beam);
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  const int offers = lane >= K ? 0 : a.finished[group * K + lane] ? 1 : min(K, a.vocab);
+  int at = 0;
+  for (int r = 0; r < K; ++r) {
+    const float s = at < offers ? sh.score[lane][at] : 0.f;
+    // ties go to the lowest beam
+    if (warp_best(at < offers ? key_of(s + 0.f, lane) : 0ull)) {
+      const size_t to = (size_t)group * K + r;
+      const int token = sh.token[lane][at];
+      a.scores_out[to] = s;
+      a.parents[to] = lane;
+      a.tokens[to] = token;
+      a.finished_out[to] = a.finished[group * K + lane] != 0 || token == a.eos;
+      ++at;
+    }
+  }
+}
+
+// Slices of a row: enough CTAs for about six on every SM, no slice below one
+// tile of a CTA, and lists that fit the join.
+int slices_of(int rows, int beams, int vocab, int sms) {
+  const int most = std::min({32, kListKeys / beams, (vocab + kThreads * kElems - 1) / (kThreads * kElems)});
+  return std::max(1, std::min(most, (6 * sms + rows - 1) / rows));
 }
 
 }  // namespace
@@ -146,10 +347,12 @@ using namespace ce::paged;
 extern "C" {
 
 int ce_beam_workspace(int batch, int beams, int vocab, size_t *bytes) {
-  CE_REQUIRE(batch >= 1 && beams >= 1 && beams <= kMaxBeams && vocab >= 1,
-             "batch and vocab must be >= 1 and beams in [1, %d] (got %d, %d, %d)", kMaxBeams, batch, vocab, beams);
+  CE_REQUIRE(batch >= 1 && batch <= kMaxGroups && beams >= 1 && beams <= kMaxBeams && vocab >= 1,
+             "batch must be in [1, %d], beams in [1, %d], vocab >= 1 (got %d, %d, %d)", kMaxGroups, kMaxBeams, batch,
+             beams, vocab);
   CE_REQUIRE(bytes != nullptr, "null argument");
-  *bytes = (size_t)batch * beams * (8 * beams + 8);
+  const size_t lists = (size_t)batch * beams * slices_of(1, beams, vocab, 1 << 20);
+  *bytes = 4ull * kMaxGroups + lists * 8 * (beams + 1);
   return CE_OK;
 }
 
@@ -162,22 +365,22 @@ int ce_beam_select(float *scores_out, int32_t *parents, int32_t *tokens, uint8_t
   CE_REQUIRE(scores_out != nullptr && parents != nullptr && tokens != nullptr && finished_out != nullptr &&
                  logits != nullptr && scores != nullptr && finished != nullptr, "null argument");
   CE_REQUIRE(type == CE_TYPE_F32 || type16(type), "logits must be F32, BF16 or F16 (got %d)", type);
+  CE_REQUIRE(reinterpret_cast<uintptr_t>(logits) % type_bytes(type) == 0, "the logits must be aligned to their type");
   CE_REQUIRE(ld >= vocab, "the row stride %lld is shorter than the vocabulary %d", (long long)ld, vocab);
-  CE_REQUIRE((int64_t)batch * beams <= 0x7fffffff / 32, "batch x beams is too large (%d x %d)", batch, beams);
   CE_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
              "the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
-  const size_t rows = (size_t)batch * beams;
+  const int slices = slices_of(batch * beams, beams, vocab, sm_count());
+  const size_t lists = (size_t)batch * beams * slices;
   BeamArgs a = {scores_out, parents, tokens, finished_out, logits, ld, scores, finished, batch, beams, vocab, eos, pad,
-                static_cast<unsigned long long *>(workspace), nullptr};
-  a.lse = reinterpret_cast<float *>(a.best + rows * beams);
-  const cudaStream_t s = (cudaStream_t)stream;
+                slices, static_cast<int *>(workspace), nullptr, nullptr};
+  a.best = reinterpret_cast<unsigned long long *>(a.arrivals + kMaxGroups);
+  a.sums = reinterpret_cast<float2 *>(a.best + lists * beams);
+  const dim3 grid((unsigned)slices, (unsigned)beams, (unsigned)batch);
   auto go = [&](auto kernel) {
-    return launch_kernel(kernel, dim3((unsigned)rows), dim3(256), 0, s, true, "rows_kernel", a);
+    return launch_kernel(kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, true, "select_kernel", a);
   };
-  const int r = type == CE_TYPE_F32 ? go(rows_kernel<float>) : type == CE_TYPE_F16 ? go(rows_kernel<__half>)
-                                                                                   : go(rows_kernel<__nv_bfloat16>);
-  if (r != CE_OK) return r;
-  return launch_kernel(groups_kernel, dim3((unsigned)batch), dim3(32), 0, s, true, "groups_kernel", a);
+  return type == CE_TYPE_F32 ? go(select_kernel<float>) : type == CE_TYPE_F16 ? go(select_kernel<__half>)
+                                                                             : go(select_kernel<__nv_bfloat16>);
 }
 
 }  // extern "C"

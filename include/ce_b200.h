@@ -949,7 +949,7 @@ int ce_beam_workspace(int batch, int beams, int vocab, size_t *bytes);
  * parents (the beam of the same element that each extends), tokens, and
  * finished_out (the parent was finished, or the token is eos). NaN and -inf
  * logits are tokens of probability 0 (score -inf); +inf counts as the
- * largest finite fp32; a NaN score counts as -inf. beams <= 32. Outputs may
+ * largest finite fp32; a NaN score counts as -inf. beams <= 32, batch <= 16384. Outputs may
  * not overlap the inputs. */
 int ce_beam_select(float *scores_out_dev, int32_t *parents_dev, int32_t *tokens_dev,
                    uint8_t *finished_out_dev, const void *logits_dev, int type, int64_t ld,

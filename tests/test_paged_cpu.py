@@ -122,7 +122,7 @@ def test_beam_refusals(ce):
     L = ce.lib()
     n = ctypes.c_size_t()
     for shape in ((0, 4, 100), (1, 0, 100), (1, 33, 100), (1, 4, 0)):
-        refused(ce, L.ce_beam_workspace(*shape, ctypes.byref(n)), "beams in")
+        refused(ce, L.ce_beam_workspace(*shape, ctypes.byref(n)), "beams in [1, 32]")
     refused(ce, L.ce_beam_workspace(1, 4, 100, None), "null")
 
     def call(so=PTR, pa=PTR, to=PTR, fo=PTR, lg=PTR, ty=ce.TYPE_F32, ld=100, sc=PTR, fi=PTR, B=1, K=4, V=100, ws=PTR,
@@ -131,7 +131,7 @@ def test_beam_refusals(ce):
 
     for change, word in ((dict(so=None), "null"), (dict(pa=None), "null"), (dict(to=None), "null"), (dict(fo=None), "null"),
                          (dict(lg=None), "null"), (dict(sc=None), "null"), (dict(fi=None), "null"), (dict(ty=3), "logits"),
-                         (dict(ld=99), "row stride"), (dict(K=33), "beams"), (dict(B=1 << 28, K=32), "too large"),
+                         (dict(ld=99), "row stride"), (dict(K=33), "beams"), (dict(B=16385), "batch"),
                          (dict(ws=None), "workspace"), (dict(wb=8), "workspace"), (dict(ws=PTR + 4), "workspace")):
         refused(ce, call(**change), word)
 
