@@ -60,6 +60,7 @@ int gemm_set_wait_limit(unsigned long long ns);
 int gemm_bs_set_wait_limit(unsigned long long ns);
 int llama_set_wait_limit(unsigned long long ns);
 int rowx_set_wait_limit(unsigned long long ns);
+int paged_attention_set_wait_limit(unsigned long long ns);
 int rowx_sync(const ce_rowx *x, RowxSync *rx, float **out, int *lo, int *hi, int *batch, int *rows);
 int x_device_of(const ce_rowx *x);
 int gemm_rowx(int kind, float *d, const void *a, const void *b, int M, int N, int K, int lda, int ldb,
@@ -233,7 +234,7 @@ int ce_set_wait_limit(double seconds) {
   const unsigned long long ns = (unsigned long long)(seconds * 1e9);
   for (int (*set)(unsigned long long) :
        {gemm_set_wait_limit, gemm_bs_set_wait_limit, llama_set_wait_limit, rowx_set_wait_limit,
-        rows_set_wait_limit}) {
+        rows_set_wait_limit, paged_attention_set_wait_limit}) {
     const int rc = set(ns);
     if (rc != CE_OK) return set_error(rc, "cudaMemcpyToSymbol(wait limit) failed");
   }

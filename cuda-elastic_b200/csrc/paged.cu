@@ -597,8 +597,10 @@ int check_kv(const ce_paged_kv *kv, int layer) {
   CE_REQUIRE(aligned16(kv->k_dev) && aligned16(kv->v_dev) && kv->layer_stride % unit == 0 &&
                  kv->page_stride % unit == 0 && kv->head_stride % unit == 0 && kv->token_stride % unit == 0,
              "the cache's bases and strides must be multiples of 16 bytes");
-  CE_REQUIRE(kv->layer_stride >= 0 && kv->page_stride >= 0 && kv->head_stride >= 0 && kv->token_stride >= 0,
-             "the cache's strides must not be negative");
+  auto bad = [](int64_t stride, int size) { return stride < 0 || stride >= (1ll << 36) || (size > 1 && stride == 0); };
+  CE_REQUIRE(!bad(kv->layer_stride, kv->layers) && !bad(kv->page_stride, kv->pages) &&
+                 !bad(kv->head_stride, kv->kv_heads) && !bad(kv->token_stride, kv->page_size),
+             "the cache's strides must be positive and below 2^36 elements");
   return CE_OK;
 }
 

@@ -21,6 +21,7 @@ constexpr unsigned kSiteSlot = 950;  // slot past the pool
 constexpr unsigned kSitePos = 951;   // position past the rotary table
 constexpr unsigned kSitePage = 952;  // page id outside the pool
 constexpr unsigned kSiteLen = 953;   // length outside the table's row
+constexpr unsigned kSiteWait = 954;  // a bounded wait for a copy gave up
 
 inline bool type16(int t) { return t == CE_TYPE_BF16 || t == CE_TYPE_F16; }
 inline int type_bytes(int t) { return t == CE_TYPE_F32 ? 4 : t == CE_TYPE_E4M3 ? 1 : 2; }

@@ -11,15 +11,18 @@
 //     takes an equal contiguous share, whatever the lengths: a long request
 //     is split over many SMs, many short ones share a warp, and no SM ends
 //     early. Lengths are read on the device; the grid never depends on them.
-//   * A warp runs alone: no block barrier until its share is done. It copies
-//     its units with cp.async into a ring of its own, several units ahead and
-//     across request boundaries, and each lane copies exactly the bytes that
-//     it will itself feed to the tensor core, so a wait for its own copies is
-//     all the synchronisation there is, and shared memory is read back in
-//     16-byte pieces without bank conflicts or transposition: a lane's 16
-//     bytes of a key serve as that lane's part of the contracted dimension
-//     (any order will do, when q is laid out alike), and its 16 bytes of four
-//     values are paired by byte permutes into the rows of V^T.
+//   * A warp runs alone: no block barrier until its share is done. TMA brings
+//     its units into a ring of its own, several ahead and across request
+//     boundaries (one 4-D box per 128 bytes of head row: head-major and
+//     token-major pages are the same to it, and what lies past head_dim or
+//     the pool reads as zeros), with an mbarrier per stage.
+//   * Lanes read shared memory in 16-byte pieces without bank conflicts and
+//     without transposing: 16 bytes of a key serve as the lane's part of the
+//     contracted dimension (any order will do, when q is laid out alike), and
+//     16 bytes of four values are paired by byte permutes into the rows of
+//     V^T. Which key takes which row of the product is free too; row g takes
+//     key g if even, (g + 4) mod 8 if odd, so that with the 128-byte swizzle
+//     the eight lanes of a phase meet eight different bank groups in both.
 //   * mma.sync (m16n8k16), not tcgen05: with 8 query heads on the narrow side
 //     nothing is wasted on padding rows up to 8 heads, accumulators stay in
 //     registers beside the softmax, and the tensor work is far from binding.
@@ -34,13 +37,17 @@
 #include <algorithm>
 #include <type_traits>
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "paged.cuh"
 
 namespace ce {
 namespace paged {
 namespace {
 
-__device__ DeviceStatus g_attention_status;
+__device__ DeviceStatus g_attention_status;  // bad pages and lengths
+__device__ DeviceStatus g_attention_wait;    // a wait that gave up (it ends the waits of others, too)
 
 constexpr int kUnit = 16;              // keys of a unit
 constexpr int kMaxSplitHeads = 16;     // query heads of one pass over the keys
@@ -51,11 +58,9 @@ struct AttnArgs {
   const void *q;
   void *out;
   float *lse;
-  const char *k, *v;  // layer base
   const float *k_scale, *v_scale;
   const int32_t *table, *lens;
   long long q_ld, out_ld;
-  long long page_stride, head_stride, token_stride;  // bytes
   int seqs, max_pages, pages, heads, kv_heads, dim, shift;
   int group, tiles;  // query heads per kv head; passes over them
   float scale;
@@ -71,11 +76,12 @@ struct Shape {
   static constexpr int kKeyChunks = D * kItem / 64;           // 16-byte pieces of a key row per lane
   static constexpr int kValBytes = D * kItem / 8 >= 16 ? 16 : 8;
   static constexpr int kValChunks = D * kItem / 8 / kValBytes;  // pieces of a value row per lane
-  static constexpr int kKeyBytes = 2 * kKeyChunks * 512;
-  static constexpr int kStageBytes = kKeyBytes + 4 * kValChunks * 32 * kValBytes;
-  static constexpr int kWarps = NT == 1 ? (kStageBytes == 8192 ? 8 : F8 && D == 128 ? 12 : 16)
-                                        : (kStageBytes == 8192 ? 6 : F8 && D == 128 ? 8 : 12);
-  static constexpr int kStages = kStageBytes == 2048 ? 5 : F8 && D == 128 && NT == 2 ? 4 : 3;
+  static constexpr int kTiles = D * kItem > 128 ? 2 : 1;        // 128-byte wide tiles of 16 rows
+  static constexpr int kTileBytes = 128 * kUnit;
+  static constexpr int kStageBytes = 2 * kTiles * kTileBytes;   // keys, then values
+  static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : D == 128 ? 12 : 16)
+                                        : (kTiles == 2 ? 6 : D == 128 ? 8 : 12);
+  static constexpr int kStages = kTiles == 1 && D == 128 && NT == 2 ? 4 : 3;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPart = kHeads * (D + 2);  // floats of one (O, max, sum) part
   static constexpr int kVals = D / 8;             // dimensions of a value row per lane
@@ -90,20 +96,18 @@ struct Shape {
 // One part of a split request as a warp or CTA holds it.
 struct Span {
   long long unit0;         // its first unit on the line
-  int row, hq;             // request; kv head and pass
+  int row, kh, tile;       // request, kv head, pass over its query heads
   int k0, k1, units;       // its units of the request's `units`
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void *src, int bytes) {
-  asm volatile("cp.async.ca.shared.global.L2::128B [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A box of one page's rows of one head into shared memory (128-byte swizzle).
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int token,
+                                              int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(token), "r"(head), "r"(page)
+      : "memory");
 }
 
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
@@ -139,10 +143,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t x) {
-  uint32_t y;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(y) : "r"(x));
-  return y;
+// Four E4M3 values as two f16 pairs (every E4M3 value is an f16 value).
+__device__ __forceinline__ void e4m3_to_f16(uint32_t x, uint32_t &lo, uint32_t &hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(x));
 }
 
 // (lo, hi) as two 16-bit values of the product's type, and what that lost.
@@ -184,9 +188,8 @@ __device__ __forceinline__ int row_len(const AttnArgs &a, int b) {
 
 // A place on the line of units. Requests of length 0 have none.
 struct Cursor {
-  int row, hq, k, len, units;
+  int row, kh, tile, k, len, units;  // request, kv head, pass over its query heads, unit; the request's length and units
   __device__ __forceinline__ void next_row(const AttnArgs &a) {
-    k = hq = 0;
     do {
       if (++row >= a.seqs) {  // only if the lengths changed under the call: stay inside the buffers
         row = a.seqs - 1, len = 0, units = 1;
@@ -197,10 +200,13 @@ struct Cursor {
     units = (len + kUnit - 1) / kUnit;
   }
   __device__ __forceinline__ void step(const AttnArgs &a) {
-    if (++k == units) {
-      k = 0;
-      if (++hq == a.kv_heads * a.tiles) next_row(a);
-    }
+    if (++k < units) return;
+    k = 0;
+    if (++tile < a.tiles) return;
+    tile = 0;
+    if (++kh < a.kv_heads) return;
+    kh = 0;
+    next_row(a);
   }
 };
 
@@ -241,11 +247,14 @@ __device__ __forceinline__ void join_parts(int heads, int count, Part &&part, Em
 }
 
 template <int D, int NT, bool F8, typename Io>
-__global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1)
+attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                 const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, NT, F8>;
   constexpr bool BF = !F8 && std::is_same<Io, __nv_bfloat16>::value;  // type of the products
   constexpr int W = S::kWarps, ST = S::kStages;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[W][ST];
   // units of the requests up to each thread's last, per kv head and pass; in
   // the place of the warps' first parts until every warp has found its share
   int *const ends = reinterpret_cast<int *>(smem + (size_t)W * S::kRing);
@@ -258,6 +267,10 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
 
   // ---- the line of units: prefix sums over the requests
   if (tid == 0) any_empty = 0;
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+  }
   if (tid < 2 * W) span_used[tid] = 0;
   __syncthreads();
   const int per = (a.seqs + S::kThreads - 1) / S::kThreads;
@@ -295,7 +308,7 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
   float *const part1 = reinterpret_cast<float *>(smem + (size_t)warp * S::kRing);
 
   // ---- where the share begins
-  Cursor at = {0, 0, 0, 0, 1};
+  Cursor at = {0, 0, 0, 0, 0, 1};
   if (count > 0) {
     int lo = 0, hi = S::kThreads - 1;
     while (lo < hi) {
@@ -312,62 +325,56 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
     }
     at.units = max(1, at.units);
     const long long in = u0 - before * passes;
-    at.hq = (int)min((long long)passes - 1, in / at.units);
-    at.k = (int)(in - (long long)at.hq * at.units);
+    const int pass = (int)min((long long)passes - 1, in / at.units);
+    at.kh = pass / a.tiles, at.tile = pass % a.tiles;
+    at.k = (int)(in - (long long)pass * at.units);
   }
   __syncthreads();
 
   if (count > 0) {
-    Cursor look = at;  // the unit whose page is looked up next
-    int look_page = 0, look_key = 0, look_hq = 0;
-    bool look_live = false;
-    int looked = 0, issued = 0;
-    auto look_up = [&] {  // lane l < 16: the page of the unit's key l
-      look_key = look.k * kUnit + (lane & 15);
-      look_hq = look.hq;
-      look_live = looked < count && look_key < look.len;
-      look_page = 0;
-      if (look_live) look_page = __ldg(a.table + (size_t)look.row * a.max_pages + (look_key >> a.shift));
-      if (++looked < count) look.step(a);
+    // Copies run ahead of the products by ST - 1 units, page lookups by one
+    // more, so that no copy waits for its page id. A unit is one box of a
+    // page, or 16 / page_size boxes of as many pages, one per lane.
+    Cursor look = at;  // the unit whose pages are looked up next
+    const int32_t *pages = a.table + (size_t)look.row * a.max_pages;
+    const int rows = min(kUnit, 1 << a.shift), mask = (1 << a.shift) - 1, sub = lane * rows;  // of this lane's box
+    int page = 0, token = 0, head = 0, left = 0;  // of the looked-up unit; left: live keys (less than 1: no unit)
+    int to_look = count;
+    auto look_up = [&] {
+      left = 0;
+      if (to_look == 0) return;
+      const int key = look.k * kUnit + sub;
+      left = look.len - look.k * kUnit;
+      head = look.kh;
+      token = key & mask;
+      page = sub < min(left, kUnit) ? __ldg(pages + (key >> a.shift)) : 0;
+      if (--to_look == 0) return;
+      const int row = look.row;
+      look.step(a);
+      if (look.row != row) pages = a.table + (size_t)look.row * a.max_pages;
     };
-    const int dim_bytes = a.dim * S::kItem;
+    int to = 0, issued = 0;
     auto issue = [&] {  // copies the looked-up unit into its stage, then looks up the next
-      if (issued < count) {
-        long long off = -1;
-        if (look_live) {
-          if ((unsigned)look_page < (unsigned)a.pages)
-            off = look_page * a.page_stride + (look_key & ((1 << a.shift) - 1)) * a.token_stride +
-                  (look_hq / a.tiles) * a.head_stride;
-          else
-            report_timeout(&g_attention_status, kSitePage);
+      if (left <= 0) return;
+      uint64_t *bar = &full[warp][to];
+      const int boxes = (min(left, kUnit) + rows - 1) / rows;
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * rows * 128 * 2 * S::kTiles));
+      __syncwarp();
+      if (lane < boxes) {
+        if ((unsigned)page >= (unsigned)a.pages) {
+          report_timeout(&g_attention_status, kSitePage);
+          page = a.pages;  // past the map: zeros
         }
-        const uint32_t st = ring + (uint32_t)(issued % ST) * S::kStageBytes;
+        const uint32_t dst = ring + (uint32_t)to * S::kStageBytes + (uint32_t)sub * 128;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {  // keys g and g + 8, pieces t, t + 4, ...
-          const long long o = __shfl_sync(0xffffffffu, off, g + 8 * r);
-          const char *src = a.k + (o < 0 ? 0 : o) + 16 * t;
-#pragma unroll
-          for (int c = 0; c < S::kKeyChunks; ++c) {
-            const bool live = o >= 0 && 16 * (t + 4 * c) < dim_bytes;
-            cp16(st + (r * S::kKeyChunks + c) * 512 + 16 * lane, live ? src + 64 * c : a.k, live ? 16 : 0);
-          }
+        for (int i = 0; i < S::kTiles; ++i) {
+          tma_load_page(dst + i * S::kTileBytes, &k_map, bar, i * (128 / S::kItem), token, head, page);
+          tma_load_page(dst + (S::kTiles + i) * S::kTileBytes, &v_map, bar, i * (128 / S::kItem), token, head, page);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {  // values 2t, 2t + 1, 2t + 8, 2t + 9, pieces g, g + 8, ...
-          const long long o = __shfl_sync(0xffffffffu, off, 2 * t + (r & 1) + 8 * (r >> 1));
-          const char *src = a.v + (o < 0 ? 0 : o) + S::kValBytes * g;
-#pragma unroll
-          for (int c = 0; c < S::kValChunks; ++c) {
-            const bool live = o >= 0 && S::kValBytes * (g + 8 * c) < dim_bytes;
-            const uint32_t dst = st + S::kKeyBytes + (r * S::kValChunks + c) * (32 * S::kValBytes) + S::kValBytes * lane;
-            const void *from = live ? src + 8 * S::kValBytes * c : a.v;
-            if constexpr (S::kValBytes == 16) cp16(dst, from, live ? 16 : 0); else cp8(dst, from, live ? 8 : 0);
-          }
-        }
-        ++issued;
-        look_up();
       }
-      cp_commit();
+      to = to + 1 == ST ? 0 : to + 1;
+      ++issued;
+      look_up();
     };
     look_up();
     for (int s = 0; s < ST - 1; ++s) issue();
@@ -380,10 +387,22 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
     int k0 = at.k;               // first unit of the current request part
     long long start = u0;
     bool fresh = true;
+    // Row g of the products stands for key pi, row g + 8 for pi + 8.
+    const int pi = g & 1 ? (g + 4) & 7 : g, pe = 2 * t, po = (2 * t + 5) & 7;  // pi of g, 2t, 2t + 1
+    uint32_t key_at[2], val_at[2];  // this lane's pieces in a stage
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      key_at[p] = pi * 128 + (((t + 4 * p) ^ pi) << 4);
+      const int key = p ? po : pe;
+      val_at[p] = S::kTiles * S::kTileBytes + key * 128 +
+                  (S::kValBytes == 16 ? (g ^ key) << 4 : (((g >> 1) ^ key) << 4) + 8 * (g & 1));
+    }
+    int stage = 0, landed = 0;
+    uint32_t parity = 0;
     for (int it = 0; it < count; ++it) {
       if (fresh) {
         fresh = false;
-        const int kh = at.hq / a.tiles, h0 = (at.hq % a.tiles) * S::kHeads;
+        const int kh = at.kh, h0 = at.tile * S::kHeads;
         const float ks = a.k_scale != nullptr ? __ldg(a.k_scale + kh) : 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -430,9 +449,10 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
           for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
         }
       }
-      cp_wait<ST - 2>();
+      if (!warp_wait(&full[warp][stage], parity, &g_attention_wait, kSiteWait)) break;
+      ++landed;
       issue();  // into the stage that the previous unit left
-      const uint32_t st = ring + (uint32_t)(it % ST) * S::kStageBytes;
+      const uint32_t st = ring + (uint32_t)stage * S::kStageBytes;
       // ---- scores: 16 keys x 8 NT heads
       float s[NT][4], s2[NT][4];
 #pragma unroll
@@ -441,16 +461,19 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
         for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
 #pragma unroll
       for (int c = 0; c < S::kKeyChunks; ++c) {
-        const uint4 x = lds16(st + c * 512 + 16 * lane), y = lds16(st + (S::kKeyChunks + c) * 512 + 16 * lane);
+        const uint32_t from = st + key_at[c & 1] + (c >> 1) * S::kTileBytes;
+        const uint4 x = lds16(from), y = lds16(from + 8 * 128);
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if constexpr (F8) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              mma<BF>((j & 1) ? s2[nt] : s[nt], e4m3x2_to_f16x2(xw[j]), e4m3x2_to_f16x2(yw[j]),
-                      e4m3x2_to_f16x2(xw[j] >> 16), e4m3x2_to_f16x2(yw[j] >> 16), q[nt][8 * c + 2 * j],
-                      q[nt][8 * c + 2 * j + 1]);
+            for (int j = 0; j < 4; ++j) {
+              uint32_t x0, x1, y0, y1;
+              e4m3_to_f16(xw[j], x0, x1);
+              e4m3_to_f16(yw[j], y0, y1);
+              mma<BF>((j & 1) ? s2[nt] : s[nt], x0, y0, x1, y1, q[nt][8 * c + 2 * j], q[nt][8 * c + 2 * j + 1]);
+            }
           } else {
             mma<BF>(s[nt], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
             mma<BF>(s2[nt], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
@@ -458,14 +481,17 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
         }
       }
       // ---- softmax: keys g (elements 0, 1) and g + 8 (2, 3) of heads 2t, 2t + 1
-      const int key = at.k * kUnit + g;
       uint32_t big[NT][2], rest[NT][2];
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[nt][i] = key + 8 * (i >> 1) < at.len ? (s[nt][i] + s2[nt][i]) * cs[nt][i & 1] : -INFINITY;
+        for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * cs[nt][i & 1];
+        if (at.k + 1 == at.units) {  // the last unit may have keys past the length
+          const int n = at.len - at.k * kUnit;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][i] = pi + 8 * (i >> 1) < n ? s[nt][i] : -INFINITY;
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(s[nt][j], s[nt][j + 2]);
       }
@@ -493,12 +519,11 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+        float p[4], base[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float base = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
-          p[i] = exp2_approx(s[nt][i] - base);
-        }
+        for (int j = 0; j < 2; ++j) base[j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[nt][i] - base[i & 1]);
         l[nt][0] += p[0] + p[2];
         l[nt][1] += p[1] + p[3];
         split16<BF>(p[0], p[1], big[nt][0], rest[nt][0]);
@@ -513,7 +538,7 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < S::kValChunks; ++c) {
-          const uint32_t from = st + S::kKeyBytes + (r * S::kValChunks + c) * (32 * S::kValBytes) + S::kValBytes * lane;
+          const uint32_t from = st + val_at[r & 1] + c * S::kTileBytes + (r >> 1) * (8 * 128);
           if constexpr (S::kValBytes == 16) {
             const uint4 y = lds16(from);
             x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
@@ -522,37 +547,49 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
             x[r][0] = y.x, x[r][1] = y.y;
           }
         }
-      constexpr int kPer = 4 / S::kItem;  // elements of a word
+      if (at.k + 1 == at.units) {  // weights of 0 must meet values of 0, whatever the cache holds there
+        const int n = at.len - at.k * kUnit;
 #pragma unroll
-      for (int i = 0; i < S::kVals / 2; ++i) {
-        uint32_t v[4];  // (row g | g + 8) x (keys 2t, 2t + 1 | 2t + 8, 2t + 9)
+        for (int r = 0; r < 4; ++r)
+          if ((r & 1 ? po : pe) + 8 * (r >> 1) >= n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int e = i + (r & 1) * (S::kVals / 2), w = e / kPer, b = e % kPer, pr = 2 * (r >> 1);
-          if constexpr (F8)
-            v[r] = e4m3x2_to_f16x2(__byte_perm(x[pr][w], x[pr + 1][w], b | (4 + b) << 4));
-          else
-            v[r] = __byte_perm(x[pr][w], x[pr + 1][w], b ? 0x7632 : 0x5410);
-        }
+            for (int w = 0; w < kWords; ++w) x[r][w] = 0;
+      }
+      auto product = [&](int i, const uint32_t (&v)[4]) {  // v: (row g | g + 8) x (keys 2t, 2t + 1 | 2t + 8, 2t + 9)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], big[nt][0], big[nt][1]);
           mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], rest[nt][0], rest[nt][1]);
         }
+      };
+      constexpr int kPer = 4 / S::kItem;  // elements of a word
+#pragma unroll
+      for (int i = 0; i < S::kVals / 2; i += 2) {
+        uint32_t v[2][4];  // elements i and i + 1
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int e = i + (r & 1) * (S::kVals / 2), w = e / kPer, pr = 2 * (r >> 1);
+          if constexpr (F8) {
+            e4m3_to_f16(__byte_perm(x[pr][w], x[pr + 1][w], e % kPer ? 0x7362 : 0x5140), v[0][r], v[1][r]);
+          } else {
+            v[0][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x5410);
+            v[1][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x7632);
+          }
+        }
+        product(i, v[0]);
+        product(i + 1, v[1]);
       }
+      if (++stage == ST) stage = 0, parity ^= 1u;
 
       // ---- end of the request's keys, or of the share
       const bool ends_here = at.k + 1 == at.units;
       if (ends_here || it + 1 == count) {
-        const int kh = at.hq / a.tiles, h0 = (at.hq % a.tiles) * S::kHeads;
+        const int kh = at.kh, h0 = at.tile * S::kHeads;
         const bool whole = ends_here && k0 == 0;
         const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
         const int slot = start == u0 ? 0 : 1;
         float *part = slot ? part1 : part0;
-        if (slot && !whole) {  // the ring is the second part's place: only after the last unit
-          cp_wait<0>();
-          __syncwarp();
-        }
+        if (slot && !whole) __syncwarp();  // the ring is the second part's place: every lane is done with the last unit
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -590,7 +627,7 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
             }
           }
         if (!whole && lane == 0) {
-          spans[2 * warp + slot] = {start, at.row, at.hq, k0, at.k + 1, at.units};
+          spans[2 * warp + slot] = {start, at.row, at.kh, at.tile, k0, at.k + 1, at.units};
           span_used[2 * warp + slot] = 1;
         }
         fresh = true;
@@ -599,7 +636,11 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
       }
       if (it + 1 < count) at.step(a);
     }
-    cp_wait<0>();
+    // After a wait that gave up: no copy may land in the memory of a CTA that has left.
+    for (; landed < issued; ++landed) {
+      warp_wait(&full[warp][stage], parity, nullptr, kSiteWait);
+      if (++stage == ST) stage = 0, parity ^= 1u;
+    }
   }
   __syncthreads();
 
@@ -618,13 +659,13 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
     int n = 0, last = e, f = e;
     for (; f < 2 * W; ++f) {
       if (!span_used[f]) continue;
-      if (spans[f].row != first.row || spans[f].hq != first.hq) break;
+      if (spans[f].row != first.row || spans[f].kh != first.kh || spans[f].tile != first.tile) break;
       if (tid == 0) members[n] = f;
       ++n, last = f;
     }
     e = f;
     __syncthreads();
-    const int kh = first.hq / a.tiles, h0 = (first.hq % a.tiles) * S::kHeads;
+    const int kh = first.kh, h0 = first.tile * S::kHeads;
     const int heads = min(S::kHeads, a.group - h0);
     const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
     auto finish = [&](int h, int d, const float (&x)[8], float m, float l) {
@@ -670,7 +711,7 @@ __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1) attention_kerne
 }
 
 template <int D, int NT, bool F8, typename Io>
-int launch_attention(const AttnArgs &a, int grid, cudaStream_t s) {
+int launch_attention(const AttnArgs &a, const CUtensorMap (&maps)[2], int grid, cudaStream_t s) {
   using S = Shape<D, NT, F8>;
   static bool done[64] = {};
   int dev = 0;
@@ -681,14 +722,46 @@ int launch_attention(const AttnArgs &a, int grid, cudaStream_t s) {
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
   return launch_kernel(attention_kernel<D, NT, F8, Io>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, s, true,
-                       "attention_kernel", a);
+                       "attention_kernel", a, maps[0], maps[1]);
 }
 
 template <bool F8, typename Io>
-int dispatch_attention(const AttnArgs &a, int grid, cudaStream_t s) {
+int dispatch_attention(const AttnArgs &a, const CUtensorMap (&maps)[2], int grid, cudaStream_t s) {
   if (a.dim <= 64)
-    return a.group <= 8 ? launch_attention<64, 1, F8, Io>(a, grid, s) : launch_attention<64, 2, F8, Io>(a, grid, s);
-  return a.group <= 8 ? launch_attention<128, 1, F8, Io>(a, grid, s) : launch_attention<128, 2, F8, Io>(a, grid, s);
+    return a.group <= 8 ? launch_attention<64, 1, F8, Io>(a, maps, grid, s) : launch_attention<64, 2, F8, Io>(a, maps, grid, s);
+  return a.group <= 8 ? launch_attention<128, 1, F8, Io>(a, maps, grid, s) : launch_attention<128, 2, F8, Io>(a, maps, grid, s);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p) : nullptr;
+  }();
+  return fn;
+}
+
+// The map of one layer of a pool: [pages][heads][tokens][head_dim] with the
+// pool's strides; boxes of 128 bytes x min(16, page_size) tokens.
+int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer) {
+  const auto fn = encode_fn();
+  if (fn == nullptr) return set_error(CE_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const int b = type_bytes(kv->type);
+  const cuuint64_t dims[4] = {(cuuint64_t)kv->head_dim, (cuuint64_t)kv->page_size, (cuuint64_t)kv->kv_heads,
+                              (cuuint64_t)kv->pages};
+  // the stride of a dimension of size 1 is never used; any that the map takes will do
+  auto stride = [&](int64_t elements, int size) { return size > 1 ? (cuuint64_t)elements * b : (cuuint64_t)16; };
+  const cuuint64_t strides[3] = {stride(kv->token_stride, kv->page_size), stride(kv->head_stride, kv->kv_heads),
+                                 stride(kv->page_stride, kv->pages)};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / b), (cuuint32_t)std::min(kUnit, kv->page_size), 1, 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  char *base = static_cast<char *>(pool) + (long long)layer * kv->layer_stride * b;
+  const CUresult r = fn(map, b == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims,
+                        strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? CE_OK : set_error(CE_ERR_CUDA, format("cuTensorMapEncodeTiled failed (%d)", (int)r));
 }
 
 size_t workspace_bytes_of(int grid) { return 4ull * kMaxGrid + (size_t)grid * 2 * kPartFloats * 4; }
@@ -698,17 +771,23 @@ size_t workspace_bytes_of(int grid) { return 4ull * kMaxGrid + (size_t)grid * 2 
 
 using namespace paged;
 
-// Reads and clears the status word of the attention kernels.
+// Reads and clears the status words of the attention kernels.
 int paged_attention_status() {
   CE_CUDA_TRY(cudaDeviceSynchronize());
-  DeviceStatus h{};
-  CE_CUDA_TRY(cudaMemcpyFromSymbol(&h, g_attention_status, sizeof(h)));
-  if (h.code == 0) return CE_OK;
+  DeviceStatus bad{}, wait{};
+  CE_CUDA_TRY(cudaMemcpyFromSymbol(&bad, g_attention_status, sizeof(bad)));
+  CE_CUDA_TRY(cudaMemcpyFromSymbol(&wait, g_attention_wait, sizeof(wait)));
+  if (bad.code == 0 && wait.code == 0) return CE_OK;
   const DeviceStatus zero{};
   CE_CUDA_TRY(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero)));
-  return set_error(CE_ERR_USAGE, h.where == kSitePage ? "paged attention: a page id lies outside the pool"
-                                                      : "paged attention: a length does not fit its table row");
+  CE_CUDA_TRY(cudaMemcpyToSymbol(g_attention_wait, &zero, sizeof(zero)));
+  if (wait.code != 0)
+    return set_error(CE_ERR_TIMEOUT, format("paged attention: a copy did not land in time (block %u)", wait.block));
+  return set_error(CE_ERR_USAGE, bad.where == kSitePage ? "paged attention: a page id lies outside the pool"
+                                                        : "paged attention: a length does not fit its table row");
 }
+
+int paged_attention_set_wait_limit(unsigned long long ns) { return set_wait_limit_here(ns); }
 
 }  // namespace ce
 
@@ -747,14 +826,14 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   CE_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
              "the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
   AttnArgs a = {};
-  const int b = type_bytes(kv->type);
+  CUtensorMap maps[2];
+  rc = make_page_map(&maps[0], kv, kv->k_dev, layer);
+  if (rc == CE_OK) rc = make_page_map(&maps[1], kv, kv->v_dev, layer);
+  if (rc != CE_OK) return rc;
   a.q = q, a.out = out, a.lse = lse;
-  a.k = static_cast<const char *>(kv->k_dev) + (long long)layer * kv->layer_stride * b;
-  a.v = static_cast<const char *>(kv->v_dev) + (long long)layer * kv->layer_stride * b;
   a.k_scale = kv->k_scale_dev, a.v_scale = kv->v_scale_dev;
   a.table = pt->table_dev, a.lens = pt->lens_dev;
   a.q_ld = q_ld, a.out_ld = out_ld;
-  a.page_stride = kv->page_stride * b, a.head_stride = kv->head_stride * b, a.token_stride = kv->token_stride * b;
   a.seqs = pt->seqs, a.max_pages = pt->max_pages, a.pages = kv->pages;
   a.heads = heads, a.kv_heads = kv->kv_heads, a.dim = kv->head_dim, a.shift = log2_of(kv->page_size);
   a.group = heads / kv->kv_heads;
@@ -763,10 +842,10 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   a.arrivals = static_cast<int *>(workspace);
   a.parts = reinterpret_cast<float *>(a.arrivals + kMaxGrid);
   const cudaStream_t s = (cudaStream_t)stream;
-  if (kv->type == CE_TYPE_BF16) return dispatch_attention<false, __nv_bfloat16>(a, grid, s);
-  if (kv->type == CE_TYPE_F16) return dispatch_attention<false, __half>(a, grid, s);
-  return io_type == CE_TYPE_F16 ? dispatch_attention<true, __half>(a, grid, s)
-                                : dispatch_attention<true, __nv_bfloat16>(a, grid, s);
+  if (kv->type == CE_TYPE_BF16) return dispatch_attention<false, __nv_bfloat16>(a, maps, grid, s);
+  if (kv->type == CE_TYPE_F16) return dispatch_attention<false, __half>(a, maps, grid, s);
+  return io_type == CE_TYPE_F16 ? dispatch_attention<true, __half>(a, maps, grid, s)
+                                : dispatch_attention<true, __nv_bfloat16>(a, maps, grid, s);
 }
 
 }  // extern "C"
