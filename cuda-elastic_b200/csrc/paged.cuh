@@ -39,28 +39,30 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-// Inclusive sum over the block of one value per thread; `total` is the
-// block's sum. scratch: one word per warp, free for reuse after the call.
 template <typename T>
-__device__ __forceinline__ T block_inclusive_sum(T v, T *scratch, T &total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  T x = v;
+__device__ __forceinline__ T warp_inclusive_sum(T x) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
+  return x;
+}
+
+// Inclusive sum over the block of one value per thread; `total` is the
+// block's sum. scratch: one word per warp, free for reuse after the call.
+template <typename T>
+__device__ __forceinline__ T block_inclusive_sum(T v, T *scratch, T &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const T x = warp_inclusive_sum(v);
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
-  T before = 0;
-  total = 0;
-  for (int w = 0; w < warps; ++w) {
-    const T t = scratch[w];
-    before += w < warp ? t : T(0);
-    total += t;
-  }
+  const T ends = warp_inclusive_sum(lane < warps ? scratch[lane] : T(0));
+  total = __shfl_sync(0xffffffffu, ends, 31);
+  const T before = __shfl_sync(0xffffffffu, ends, warp > 0 ? warp - 1 : 0);
   __syncthreads();
-  return before + x;
+  return (warp > 0 ? before : T(0)) + x;
 }
 
 // First index of [0, n) whose value is above x (n if none); a ascending.

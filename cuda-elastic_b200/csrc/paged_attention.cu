@@ -210,8 +210,7 @@ struct Cursor {
   }
 };
 
-// Writes the normalised output of query head `head` (within its request),
-// dimensions d .. d + 7, and its lse.
+// Writes dimensions d .. of query head `head` of a request.
 template <typename Io>
 __device__ __forceinline__ void store_out8(const AttnArgs &a, int row, int head, int d, const float (&x)[8]) {
   uint4 w;
@@ -222,29 +221,21 @@ __device__ __forceinline__ void store_out8(const AttnArgs &a, int row, int head,
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 
-// Joins `count` parts, part(i) giving the i-th part's floats (O [heads][D],
-// then (max, sum) per head): every thread takes 8 dimensions of a head.
-// emit(head, d, x, max, sum) gets the sums, not normalised.
-template <int D, int HEADS, class Part, class Emit>
-__device__ __forceinline__ void join_parts(int heads, int count, Part &&part, Emit &&emit) {
-  for (int u = threadIdx.x; u < heads * (D / 8); u += blockDim.x) {
-    const int h = u / (D / 8), d = 8 * (u % (D / 8));
-    float m = -INFINITY;
-    for (int i = 0; i < count; ++i) m = fmaxf(m, part(i)[HEADS * D + 2 * h]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, x[8] = {};
-    for (int i = 0; i < count; ++i) {
-      const float *p = part(i);
-      const float f = exp2_approx(p[HEADS * D + 2 * h] - base);
-      l += f * p[HEADS * D + 2 * h + 1];
-      const float4 y = *reinterpret_cast<const float4 *>(p + h * D + d);
-      const float4 z = *reinterpret_cast<const float4 *>(p + h * D + d + 4);
-      x[0] += f * y.x, x[1] += f * y.y, x[2] += f * y.z, x[3] += f * y.w;
-      x[4] += f * z.x, x[5] += f * z.y, x[6] += f * z.z, x[7] += f * z.w;
-    }
-    emit(h, d, x, m, l);
-  }
+template <typename Io>
+__device__ __forceinline__ void store_out4(const AttnArgs &a, int row, int head, int d, float4 x, float f) {
+  uint2 w;
+  w.x = pack2<Io>(x.x * f, x.y * f), w.y = pack2<Io>(x.z * f, x.w * f);
+  *reinterpret_cast<uint2 *>(static_cast<Io *>(a.out) + row * a.out_ld + (long long)head * a.dim + d) = w;
 }
+
+__device__ __forceinline__ void add_scaled(float4 &x, float f, float4 y) {
+  x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+}
+
+// The request part that a CTA shares with others, for the join across CTAs.
+struct Crossing {
+  int row, kh, tile, c0, c1;  // and the first and last of its CTAs
+};
 
 template <int D, int NT, bool F8, typename Io>
 __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1)
@@ -259,20 +250,25 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   // the place of the warps' first parts until every warp has found its share
   int *const ends = reinterpret_cast<int *>(smem + (size_t)W * S::kRing);
   __shared__ Span spans[2 * W];
-  __shared__ int span_used[2 * W], members[2 * W], scratch[32], any_empty, is_last;
+  __shared__ Crossing crossing[2];
+  __shared__ int span_used[2 * W], scratch[32], any_empty, n_crossing, is_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int passes = a.kv_heads * a.tiles;
   pdl_launch_dependents();
-  pdl_wait();
-
-  // ---- the line of units: prefix sums over the requests
-  if (tid == 0) any_empty = 0;
+  if (tid == 0) {
+    any_empty = n_crossing = 0;
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  if (tid < 2 * W) span_used[tid] = 0;
   if (lane == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
     fence_barrier_init();
   }
-  if (tid < 2 * W) span_used[tid] = 0;
   __syncthreads();
+  pdl_wait();
+
+  // ---- the line of units: prefix sums over the requests
   const int per = (a.seqs + S::kThreads - 1) / S::kThreads;
   int mine = 0;
   for (int b = tid * per; b < min(a.seqs, (tid + 1) * per); ++b) {
@@ -610,18 +606,19 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
                 const int e = e0 + i;
                 y[i] = o[nt][e % (S::kVals / 2)][j + 2 * (e / (S::kVals / 2))] * f;
               }
+              if (!live) continue;
               if (!whole) {
                 *reinterpret_cast<float4 *>(part + h * D + d) = make_float4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<float4 *>(part + h * D + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
-              } else if (live && d < a.dim) {
+              } else if (d < a.dim) {
                 store_out8<Io>(a, at.row, kh * a.group + h0 + h, d, y);
               }
             }
-            if (g == 0) {
+            if (g == 0 && live) {
               if (!whole) {
                 part[S::kHeads * D + 2 * h] = m[nt][j];
                 part[S::kHeads * D + 2 * h + 1] = sum;
-              } else if (live && a.lse != nullptr) {
+              } else if (a.lse != nullptr) {
                 a.lse[(size_t)at.row * a.heads + kh * a.group + h0 + h] = m[nt][j] * kLn2 + logf(sum);
               }
             }
@@ -644,67 +641,141 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   }
   __syncthreads();
 
-  // ---- parts of the CTA's warps, joined in the order of the keys
+  // ---- parts of the CTA's warps, joined in the order of the keys. Lane e
+  // looks at part e; a run of parts of one request begins where the request
+  // changes, and the runs go round the warps.
   auto warp_part = [&](int e) {
     const int w = e >> 1;
     return (e & 1) ? reinterpret_cast<const float *>(smem + (size_t)w * S::kRing)
                    : reinterpret_cast<const float *>(smem + (size_t)W * S::kRing) + w * S::kPart;
   };
-  for (int e = 0; e < 2 * W;) {
-    if (!span_used[e]) {
-      ++e;
-      continue;
-    }
-    const Span first = spans[e];
-    int n = 0, last = e, f = e;
-    for (; f < 2 * W; ++f) {
-      if (!span_used[f]) continue;
-      if (spans[f].row != first.row || spans[f].kh != first.kh || spans[f].tile != first.tile) break;
-      if (tid == 0) members[n] = f;
-      ++n, last = f;
-    }
-    e = f;
-    __syncthreads();
-    const int kh = first.kh, h0 = first.tile * S::kHeads;
-    const int heads = min(S::kHeads, a.group - h0);
-    const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
-    auto finish = [&](int h, int d, const float (&x)[8], float m, float l) {
-      const float f = vs / l;
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i] * f;
-      if (d < a.dim) store_out8<Io>(a, first.row, kh * a.group + h0 + h, d, y);
-      if (d == 0 && a.lse != nullptr)
-        a.lse[(size_t)first.row * a.heads + kh * a.group + h0 + h] = m * kLn2 + logf(l);
-    };
-    const bool here = first.k0 == 0 && spans[last].k1 == first.units;
-    auto member = [&](int i) { return warp_part(members[i]); };
-    if (here) {
-      join_parts<D, S::kHeads>(heads, n, member, finish);
-    } else {
+  {
+    const bool used = lane < 2 * W && span_used[lane];
+    const Span mine = used ? spans[lane] : Span{0, -1, 0, 0, 0, 0, 0};
+    const uint32_t parts = __ballot_sync(0xffffffffu, used);
+    const uint32_t below = parts & ((1u << lane) - 1u);
+    const int prev = below ? 31 - __clz(below) : 0;
+    // (every lane takes part in every shuffle: no short-circuit around them)
+    const int prev_row = __shfl_sync(0xffffffffu, mine.row, prev), prev_kh = __shfl_sync(0xffffffffu, mine.kh, prev);
+    const int prev_tile = __shfl_sync(0xffffffffu, mine.tile, prev);
+    const bool other = prev_row != mine.row || prev_kh != mine.kh || prev_tile != mine.tile;
+    uint32_t begins = __ballot_sync(0xffffffffu, used && (below == 0 || other));
+    for (int r = 0; begins != 0; ++r) {
+      const int e0 = __ffs(begins) - 1;
+      begins &= begins - 1;
+      if (r % W != warp) continue;
+      const uint32_t members = parts & ~((1u << e0) - 1u) & (begins ? (begins & -begins) - 1u : ~0u);
+      const int e1 = 31 - __clz(members);
+      const Span first = spans[e0];
+      const int h0 = first.tile * S::kHeads, heads = min(S::kHeads, a.group - h0);
+      const int head0 = first.kh * a.group + h0;
+      const bool here = first.k0 == 0 && spans[e1].k1 == first.units;
       // across CTAs: place 1 holds the part of a request that begins in this
       // CTA, place 0 of one that began before
-      float *place = a.parts + ((size_t)blockIdx.x * 2 + (first.k0 == 0)) * kPartFloats;
-      join_parts<D, S::kHeads>(heads, n, member, [&](int h, int d, const float (&x)[8], float m, float l) {
-        __stcg(reinterpret_cast<float4 *>(place + h * D + d), make_float4(x[0], x[1], x[2], x[3]));
-        __stcg(reinterpret_cast<float4 *>(place + h * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
-        if (d == 0) __stcg(place + S::kHeads * D + 2 * h, m), __stcg(place + S::kHeads * D + 2 * h + 1, l);
-      });
-      // CTAs of the request's first and last unit
-      const long long b0 = first.unit0 - first.k0, b1 = b0 + first.units - 1;
-      const int c0 = (int)(((b0 + 1) * all_warps - 1) / line / W), c1 = (int)(((b1 + 1) * all_warps - 1) / line / W);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        is_last = atomicAdd(a.arrivals + c0, 1) == c1 - c0;
-        if (is_last) a.arrivals[c0] = 0;
-        __threadfence();
+      float *const place = a.parts + ((size_t)blockIdx.x * 2 + (first.k0 == 0)) * kPartFloats;
+      const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + first.kh) : 1.f;
+      for (int u = lane; u < heads * (D / 4); u += 32) {
+        const int h = u / (D / 4), d = 4 * (u % (D / 4)), ml = S::kHeads * D + 2 * h;
+        float m = -INFINITY;
+        for (uint32_t b = members; b; b &= b - 1) m = fmaxf(m, warp_part(__ffs(b) - 1)[ml]);
+        const float base = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t b = members; b; b &= b - 1) {
+          const float *p = warp_part(__ffs(b) - 1);
+          const float f = exp2_approx(p[ml] - base);
+          l += f * p[ml + 1];
+          add_scaled(x, f, *reinterpret_cast<const float4 *>(p + h * D + d));
+        }
+        if (here) {
+          if (d < a.dim) store_out4<Io>(a, first.row, head0 + h, d, x, vs / l);
+          if (d == 0 && a.lse != nullptr) a.lse[(size_t)first.row * a.heads + head0 + h] = m * kLn2 + logf(l);
+        } else {
+          __stcg(reinterpret_cast<float4 *>(place + h * D + d), x);
+          if (d == 0) __stcg(reinterpret_cast<float2 *>(place + ml), make_float2(m, l));
+        }
       }
+      if (!here) {
+        __threadfence();
+        if (lane == 0) {  // CTAs of the request's first and last unit
+          const long long b0 = first.unit0 - first.k0, b1 = b0 + first.units - 1;
+          crossing[atomicAdd(&n_crossing, 1)] = {first.row, first.kh, first.tile,
+                                                 (int)(((b0 + 1) * all_warps - 1) / line / W),
+                                                 (int)(((b1 + 1) * all_warps - 1) / line / W)};
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (n_crossing == 0) return;
+  if (tid < n_crossing) {
+    const Crossing c = crossing[tid];
+    __threadfence();
+    is_last[tid] = atomicAdd(a.arrivals + c.c0, 1) == c.c1 - c.c0;
+    if (is_last[tid]) a.arrivals[c.c0] = 0;
+    __threadfence();
+  }
+  __syncthreads();
+  // ---- the last CTA of a request joins the CTAs' parts: weights of the parts
+  // per head by a warp each, then 4 dimensions per thread, the parts shared
+  // out over the threads that are left
+  for (int x = 0; x < n_crossing; ++x) {
+    if (!is_last[x]) continue;
+    const Crossing c = crossing[x];
+    const int n = c.c1 - c.c0 + 1, h0 = c.tile * S::kHeads, heads = min(S::kHeads, a.group - h0);
+    const int head0 = c.kh * a.group + h0, tasks = heads * (D / 4);
+    const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + c.kh) : 1.f;
+    auto part = [&](int i) { return a.parts + ((size_t)(c.c0 + i) * 2 + (i == 0)) * kPartFloats; };
+    float4 *const sums = reinterpret_cast<float4 *>(smem);                     // [groups][tasks]
+    float *const inv = reinterpret_cast<float *>(sums + S::kThreads);          // [heads] v_scale / sum
+    float2 *const weight = reinterpret_cast<float2 *>(inv + S::kHeads);        // [heads][n]
+    for (int h = warp; h < heads; h += W) {
+      float m = -INFINITY;
+      for (int i = lane; i < n; i += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + S::kHeads * D + 2 * h));
+        weight[h * n + i] = ml;
+        m = fmaxf(m, ml.x);
+      }
+#pragma unroll
+      for (int y = 16; y; y >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      for (int i = lane; i < n; i += 32) {
+        const float f = exp2_approx(weight[h * n + i].x - base);
+        l += f * weight[h * n + i].y;
+        weight[h * n + i].x = f;
+      }
+#pragma unroll
+      for (int y = 16; y; y >>= 1) l += __shfl_xor_sync(0xffffffffu, l, y);
+      if (lane == 0) {
+        inv[h] = vs / l;
+        if (a.lse != nullptr) a.lse[(size_t)c.row * a.heads + head0 + h] = m * kLn2 + logf(l);
+      }
+    }
+    __syncthreads();
+    auto sum_parts = [&](int task, int i0, int step) {
+      const int h = task / (D / 4), d = 4 * (task % (D / 4));
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = i0; i < n; i += step)
+        add_scaled(y, weight[h * n + i].x, __ldcg(reinterpret_cast<const float4 *>(part(i) + h * D + d)));
+      return y;
+    };
+    auto finish = [&](int task, float4 y) {
+      const int h = task / (D / 4), d = 4 * (task % (D / 4));
+      if (d < a.dim) store_out4<Io>(a, c.row, head0 + h, d, y, inv[h]);
+    };
+    if (tasks >= S::kThreads) {
+      for (int task = tid; task < tasks; task += S::kThreads) finish(task, sum_parts(task, 0, 1));
+    } else {
+      const int groups = S::kThreads / tasks, group = tid / tasks;
+      if (group < groups) sums[tid] = sum_parts(tid % tasks, group, groups);
       __syncthreads();
-      if (is_last)
-        join_parts<D, S::kHeads>(heads, c1 - c0 + 1, [&](int i) {
-          return const_cast<const float *>(a.parts) + ((size_t)(c0 + i) * 2 + (i == 0)) * kPartFloats;
-        }, finish);
+      if (tid < tasks) {
+        float4 y = sums[tid];
+        for (int i = 1; i < groups; ++i) add_scaled(y, 1.f, sums[i * tasks + tid]);
+        finish(tid, y);
+      }
     }
     __syncthreads();
   }
