@@ -50,8 +50,10 @@ __device__ DeviceStatus g_attention_status;  // bad pages and lengths
 __device__ DeviceStatus g_attention_wait;    // a wait that gave up (it ends the waits of others, too)
 
 constexpr int kUnit = 16;              // keys of a unit
+constexpr int kMinShare = 4;           // units of a CTA at least
 constexpr int kMaxSplitHeads = 16;     // query heads of one pass over the keys
 constexpr int kMaxGrid = 1024;         // CTAs the workspace's counters are laid out for
+constexpr int kRowsPerLane = 8;        // requests per lane up to which a warp scans the lengths by itself
 constexpr int kPartFloats = kMaxSplitHeads * (128 + 2);
 
 struct AttnArgs {
@@ -95,7 +97,7 @@ struct Shape {
 
 // One part of a split request as a warp or CTA holds it.
 struct Span {
-  long long unit0;         // its first unit on the line
+  uint32_t unit0;          // its first unit on the line
   int row, kh, tile;       // request, kv head, pass over its query heads
   int k0, k1, units;       // its units of the request's `units`
 };
@@ -232,6 +234,12 @@ __device__ __forceinline__ void add_scaled(float4 &x, float f, float4 y) {
   x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
 }
 
+__device__ __forceinline__ int add_acq_rel(int *p, int v) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
 // The request part that a CTA shares with others, for the join across CTAs.
 struct Crossing {
   int row, kh, tile, c0, c1;  // and the first and last of its CTAs
@@ -251,12 +259,12 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   int *const ends = reinterpret_cast<int *>(smem + (size_t)W * S::kRing);
   __shared__ Span spans[2 * W];
   __shared__ Crossing crossing[2];
-  __shared__ int span_used[2 * W], scratch[32], any_empty, n_crossing, is_last[2];
+  __shared__ int span_used[2 * W], scratch[32], n_crossing, is_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int passes = a.kv_heads * a.tiles;
   pdl_launch_dependents();
   if (tid == 0) {
-    any_empty = n_crossing = 0;
+    n_crossing = 0;
     tma_prefetch_desc(&k_map);
     tma_prefetch_desc(&v_map);
   }
@@ -268,36 +276,46 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   __syncthreads();
   pdl_wait();
 
-  // ---- the line of units: prefix sums over the requests
-  const int per = (a.seqs + S::kThreads - 1) / S::kThreads;
-  int mine = 0;
-  for (int b = tid * per; b < min(a.seqs, (tid + 1) * per); ++b) {
-    const int len = row_len(a, b);
-    mine += (len + kUnit - 1) / kUnit;
-    if (len == 0) any_empty = 1;
+  // ---- the line of units: prefix sums over the requests, by every warp for
+  // itself (no barrier) up to 256 requests, by the CTA together above
+  const bool few = a.seqs <= 32 * kRowsPerLane;
+  const int per = few ? (a.seqs + 31) / 32 : (a.seqs + S::kThreads - 1) / S::kThreads;
+  const int first_row = (few ? lane : tid) * per;
+  int lens[kRowsPerLane], mine = 0, sum;
+  bool empty = false;
+  if (few) {
+#pragma unroll
+    for (int i = 0; i < kRowsPerLane; ++i) lens[i] = i < per && first_row + i < a.seqs ? row_len(a, first_row + i) : -1;
+#pragma unroll
+    for (int i = 0; i < kRowsPerLane; ++i) mine += (lens[i] + kUnit - 1) / kUnit, empty = empty || lens[i] == 0;
+    mine = warp_inclusive_sum(mine);
+    sum = __shfl_sync(0xffffffffu, mine, 31);
+  } else {
+    for (int b = first_row; b < min(a.seqs, first_row + per); ++b) {
+      const int len = row_len(a, b);
+      mine += (len + kUnit - 1) / kUnit;
+      empty = empty || len == 0;
+    }
+    ends[tid] = block_inclusive_sum(mine, scratch, sum);
   }
-  int sum;
-  ends[tid] = block_inclusive_sum(mine, scratch, sum);
-  __syncthreads();
-  if (any_empty) {
+  if (few ? __any_sync(0xffffffffu, empty) : __syncthreads_or(empty)) {
     const float zero[8] = {};
-    for (int b = blockIdx.x; b < a.seqs; b += gridDim.x) {
+    for (int b = blockIdx.x + gridDim.x * warp; b < a.seqs; b += gridDim.x * W) {
       if (row_len(a, b) != 0) continue;
-      for (int u = tid; u < a.heads * (a.dim >> 3); u += S::kThreads)
+      for (int u = lane; u < a.heads * (a.dim >> 3); u += 32)
         store_out8<Io>(a, b, u / (a.dim >> 3), 8 * (u % (a.dim >> 3)), zero);
-      for (int h = tid; a.lse != nullptr && h < a.heads; h += S::kThreads) a.lse[(size_t)b * a.heads + h] = -INFINITY;
+      for (int h = lane; a.lse != nullptr && h < a.heads; h += 32) a.lse[(size_t)b * a.heads + h] = -INFINITY;
     }
   }
-  // Shares of the line, per warp. Where there are fewer units than CTAs the
-  // last CTAs have none: each of the others has one at least, which the count
-  // of arrivals at a join relies on.
-  const long long line = (long long)sum * passes;
-  const long long ctas = min((long long)gridDim.x, line);
-  if ((long long)blockIdx.x >= ctas) return;
-  const long long all_warps = ctas * W;
-  const long long gw = (long long)blockIdx.x * W + warp;
-  const long long u0 = gw * line / all_warps, u1 = (gw + 1) * line / all_warps;
-  const int count = (int)(u1 - u0);
+  // Shares of the line: `share` units a CTA (the last may have less, and
+  // CTAs past the line's end none), spread evenly over its warps.
+  const uint32_t line = (uint32_t)sum * (uint32_t)passes;
+  const uint32_t share = max((line + gridDim.x - 1) / gridDim.x, (uint32_t)kMinShare);
+  const uint32_t cta0 = blockIdx.x * share;
+  if (cta0 >= line) return;
+  const uint32_t cta_units = min(share, line - cta0);
+  const uint32_t u0 = cta0 + (uint32_t)((uint64_t)cta_units * warp / W);
+  const int count = (int)(cta0 + (uint32_t)((uint64_t)cta_units * (warp + 1) / W) - u0);
 
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * S::kRing;
   float *const part0 = reinterpret_cast<float *>(smem + (size_t)W * S::kRing) + warp * S::kPart;
@@ -306,26 +324,46 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   // ---- where the share begins
   Cursor at = {0, 0, 0, 0, 0, 1};
   if (count > 0) {
-    int lo = 0, hi = S::kThreads - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if ((long long)ends[mid] * passes > u0) hi = mid; else lo = mid + 1;
-    }
-    long long before = lo > 0 ? ends[lo - 1] : 0;
-    const int last = min(a.seqs, (lo + 1) * per) - 1;
-    for (at.row = lo * per;; ++at.row) {
-      at.len = row_len(a, at.row);
-      at.units = (at.len + kUnit - 1) / kUnit;
-      if (at.row >= last || (before + at.units) * passes > u0) break;
-      before += at.units;
+    uint32_t before;
+    if (few) {
+      const uint32_t beyond = __ballot_sync(0xffffffffu, (uint64_t)(uint32_t)mine * passes > u0);
+      const int lo = beyond ? __ffs(beyond) - 1 : 31;
+      int units = 0, row = first_row, len = 0, sums = mine;
+#pragma unroll
+      for (int i = 0; i < kRowsPerLane; ++i) sums -= (lens[i] + kUnit - 1) / kUnit;  // before this lane's rows
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < kRowsPerLane; ++i) {
+        const int n = (lens[i] + kUnit - 1) / kUnit;
+        if (!found && n > 0) {
+          if ((uint64_t)(uint32_t)(sums + n) * passes > u0) found = true, units = n, row = first_row + i, len = lens[i];
+          else sums += n;
+        }
+      }
+      at.row = __shfl_sync(0xffffffffu, row, lo), at.len = __shfl_sync(0xffffffffu, len, lo);
+      at.units = __shfl_sync(0xffffffffu, units, lo), before = __shfl_sync(0xffffffffu, sums, lo);
+    } else {
+      int lo = 0, hi = S::kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if ((uint64_t)(uint32_t)ends[mid] * passes > u0) hi = mid; else lo = mid + 1;
+      }
+      before = lo > 0 ? ends[lo - 1] : 0;
+      const int last = min(a.seqs, (lo + 1) * per) - 1;
+      for (at.row = lo * per;; ++at.row) {
+        at.len = row_len(a, at.row);
+        at.units = (at.len + kUnit - 1) / kUnit;
+        if (at.row >= last || (uint64_t)(before + at.units) * passes > u0) break;
+        before += at.units;
+      }
     }
     at.units = max(1, at.units);
-    const long long in = u0 - before * passes;
-    const int pass = (int)min((long long)passes - 1, in / at.units);
+    const uint32_t in = u0 - before * (uint32_t)passes;
+    const int pass = (int)min((uint32_t)passes - 1, in / (uint32_t)at.units);
     at.kh = pass / a.tiles, at.tile = pass % a.tiles;
-    at.k = (int)(in - (long long)pass * at.units);
+    at.k = (int)(in - (uint32_t)pass * (uint32_t)at.units);
   }
-  __syncthreads();
+  if (!few) __syncthreads();  // `ends` gives way to the parts
 
   if (count > 0) {
     // Copies run ahead of the products by ST - 1 units, page lookups by one
@@ -373,6 +411,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       look_up();
     };
     look_up();
+#pragma unroll 1
     for (int s = 0; s < ST - 1; ++s) issue();
 
     // ---- the share
@@ -381,7 +420,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     float m[NT][2], l[NT][2];    // running maximum (base 2) and this lane's sum
     float o[NT][S::kVals / 2][4];
     int k0 = at.k;               // first unit of the current request part
-    long long start = u0;
+    uint32_t start = u0;
     bool fresh = true;
     // Row g of the products stands for key pi, row g + 8 for pi + 8.
     const int pi = g & 1 ? (g + 4) & 7 : g, pe = 2 * t, po = (2 * t + 5) & 7;  // pi of g, 2t, 2t + 1
@@ -659,49 +698,45 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     const int prev_row = __shfl_sync(0xffffffffu, mine.row, prev), prev_kh = __shfl_sync(0xffffffffu, mine.kh, prev);
     const int prev_tile = __shfl_sync(0xffffffffu, mine.tile, prev);
     const bool other = prev_row != mine.row || prev_kh != mine.kh || prev_tile != mine.tile;
-    uint32_t begins = __ballot_sync(0xffffffffu, used && (below == 0 || other));
-    for (int r = 0; begins != 0; ++r) {
-      const int e0 = __ffs(begins) - 1;
-      begins &= begins - 1;
-      if (r % W != warp) continue;
-      const uint32_t members = parts & ~((1u << e0) - 1u) & (begins ? (begins & -begins) - 1u : ~0u);
-      const int e1 = 31 - __clz(members);
-      const Span first = spans[e0];
-      const int h0 = first.tile * S::kHeads, heads = min(S::kHeads, a.group - h0);
-      const int head0 = first.kh * a.group + h0;
-      const bool here = first.k0 == 0 && spans[e1].k1 == first.units;
-      // across CTAs: place 1 holds the part of a request that begins in this
-      // CTA, place 0 of one that began before
-      float *const place = a.parts + ((size_t)blockIdx.x * 2 + (first.k0 == 0)) * kPartFloats;
-      const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + first.kh) : 1.f;
-      for (int u = lane; u < heads * (D / 4); u += 32) {
-        const int h = u / (D / 4), d = 4 * (u % (D / 4)), ml = S::kHeads * D + 2 * h;
-        float m = -INFINITY;
-        for (uint32_t b = members; b; b &= b - 1) m = fmaxf(m, warp_part(__ffs(b) - 1)[ml]);
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t b = members; b; b &= b - 1) {
-          const float *p = warp_part(__ffs(b) - 1);
-          const float f = exp2_approx(p[ml] - base);
-          l += f * p[ml + 1];
-          add_scaled(x, f, *reinterpret_cast<const float4 *>(p + h * D + d));
-        }
-        if (here) {
-          if (d < a.dim) store_out4<Io>(a, first.row, head0 + h, d, x, vs / l);
-          if (d == 0 && a.lse != nullptr) a.lse[(size_t)first.row * a.heads + head0 + h] = m * kLn2 + logf(l);
-        } else {
-          __stcg(reinterpret_cast<float4 *>(place + h * D + d), x);
-          if (d == 0) __stcg(reinterpret_cast<float2 *>(place + ml), make_float2(m, l));
-        }
+    const uint32_t begins = __ballot_sync(0xffffffffu, used && (below == 0 || other));
+    // 4 dimensions of a head of a run per thread
+    const int widest = min(S::kHeads, a.group), tasks = widest * (D / 4), all = __popc(begins) * tasks;
+    for (int u = tid; u < all; u += S::kThreads) {
+      uint32_t rest = begins;
+      for (int r = u / tasks; r > 0; --r) rest &= rest - 1;
+      const int e0 = __ffs(rest) - 1, h = u % tasks / (D / 4), d = 4 * (u % (D / 4)), ml = S::kHeads * D + 2 * h;
+      rest &= rest - 1;
+      const uint32_t members = parts & ~((1u << e0) - 1u) & (rest ? (rest & -rest) - 1u : ~0u);
+      const Span &first = spans[e0];
+      const int h0 = first.tile * S::kHeads, head = first.kh * a.group + h0 + h;
+      if (h0 + h >= a.group) continue;
+      float m = -INFINITY;
+      for (uint32_t b = members; b; b &= b - 1) m = fmaxf(m, warp_part(__ffs(b) - 1)[ml]);
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t b = members; b; b &= b - 1) {
+        const float *p = warp_part(__ffs(b) - 1);
+        const float f = exp2_approx(p[ml] - base);
+        l += f * p[ml + 1];
+        add_scaled(x, f, *reinterpret_cast<const float4 *>(p + h * D + d));
       }
-      if (!here) {
-        __threadfence();
-        if (lane == 0) {  // CTAs of the request's first and last unit
-          const long long b0 = first.unit0 - first.k0, b1 = b0 + first.units - 1;
-          crossing[atomicAdd(&n_crossing, 1)] = {first.row, first.kh, first.tile,
-                                                 (int)(((b0 + 1) * all_warps - 1) / line / W),
-                                                 (int)(((b1 + 1) * all_warps - 1) / line / W)};
+      if (first.k0 == 0 && spans[31 - __clz(members)].k1 == first.units) {
+        const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + first.kh) : 1.f;
+        if (d < a.dim) store_out4<Io>(a, first.row, head, d, x, vs / l);
+        if (d == 0 && a.lse != nullptr) a.lse[(size_t)first.row * a.heads + head] = m * kLn2 + logf(l);
+      } else {
+        // across CTAs: place 1 holds the part of a request that begins in this
+        // CTA, place 0 of one that began before
+        float *const place = a.parts + ((size_t)blockIdx.x * 2 + (first.k0 == 0)) * kPartFloats;
+        __stcg(reinterpret_cast<float4 *>(place + h * D + d), x);
+        if (d == 0) {
+          __stcg(reinterpret_cast<float2 *>(place + ml), make_float2(m, l));
+          if (h == 0) {  // CTAs of the request's first and last unit
+            const uint32_t b0 = first.unit0 - first.k0;
+            crossing[atomicAdd(&n_crossing, 1)] = {first.row, first.kh, first.tile, (int)(b0 / share),
+                                                   (int)((b0 + first.units - 1) / share)};
+          }
         }
       }
     }
@@ -709,11 +744,10 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   __syncthreads();
   if (n_crossing == 0) return;
   if (tid < n_crossing) {
+    // releases the CTA's part (written before the barrier) and acquires the others'
     const Crossing c = crossing[tid];
-    __threadfence();
-    is_last[tid] = atomicAdd(a.arrivals + c.c0, 1) == c.c1 - c.c0;
+    is_last[tid] = add_acq_rel(a.arrivals + c.c0, 1) == c.c1 - c.c0;
     if (is_last[tid]) a.arrivals[c.c0] = 0;
-    __threadfence();
   }
   __syncthreads();
   // ---- the last CTA of a request joins the CTAs' parts: weights of the parts
@@ -887,8 +921,6 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
              kv->type);
   CE_REQUIRE(heads >= 1 && heads % kv->kv_heads == 0, "heads must be a multiple of kv_heads (got %d, %d)", heads,
              kv->kv_heads);
-  CE_REQUIRE((int64_t)pt->seqs * ((int64_t)pt->max_pages * pt->page_size / kUnit + 1) < (1ll << 31),
-             "seqs x max_pages x page_size must be below 2^35");
   const int64_t row = (int64_t)heads * kv->head_dim;
   CE_REQUIRE(aligned16(q) && aligned16(out) && q_ld % 8 == 0 && out_ld % 8 == 0 && q_ld >= row && out_ld >= row,
              "q and out must be 16-byte aligned, their row strides multiples of 8 and at least heads * head_dim");
@@ -910,6 +942,10 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   a.group = heads / kv->kv_heads;
   a.tiles = a.group <= 8 ? 1 : (a.group + kMaxSplitHeads - 1) / kMaxSplitHeads;
   a.scale = scale;
+  const int64_t units = (int64_t)pt->max_pages * pt->page_size / kUnit + 1;  // of a full row
+  CE_REQUIRE(pt->seqs * units < (1ll << 31) && (double)pt->seqs * units * kv->kv_heads * a.tiles < 4294967296.0 - kMaxGrid,
+             "seqs x max_pages x page_size x kv_heads is too large (%d x %d x %d x %d)", pt->seqs, pt->max_pages,
+             pt->page_size, kv->kv_heads);
   a.arrivals = static_cast<int *>(workspace);
   a.parts = reinterpret_cast<float *>(a.arrivals + kMaxGrid);
   const cudaStream_t s = (cudaStream_t)stream;
