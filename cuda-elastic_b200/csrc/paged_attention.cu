@@ -81,9 +81,9 @@ struct Shape {
   static constexpr int kTiles = D * kItem > 128 ? 2 : 1;        // 128-byte wide tiles of 16 rows
   static constexpr int kTileBytes = 128 * kUnit;
   static constexpr int kStageBytes = 2 * kTiles * kTileBytes;   // keys, then values
-  static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : D == 128 ? 12 : 16)
+  static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : 12)
                                         : (kTiles == 2 ? 6 : D == 128 ? 8 : 12);
-  static constexpr int kStages = kTiles == 1 && D == 128 && NT == 2 ? 4 : 3;
+  static constexpr int kStages = kTiles == 2 || (D == 64) != (NT == 1) ? 3 : 4;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPart = kHeads * (D + 2);  // floats of one (O, max, sum) part
   static constexpr int kVals = D / 8;             // dimensions of a value row per lane
@@ -97,7 +97,7 @@ struct Shape {
 
 // One part of a split request as a warp or CTA holds it.
 struct Span {
-  uint32_t unit0;          // its first unit on the line
+  uint32_t slot;           // the place of its first unit on the line
   int row, kh, tile;       // request, kv head, pass over its query heads
   int k0, k1, units;       // its units of the request's `units`
 };
@@ -112,26 +112,15 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m
       : "memory");
 }
 
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
-
 template <bool BF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
   if constexpr (BF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -187,6 +176,8 @@ __device__ __forceinline__ int row_len(const AttnArgs &a, int b) {
   }
   return len;
 }
+
+__device__ __forceinline__ int slots_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit + 1 : 0; }
 
 // A place on the line of units. Requests of length 0 have none.
 struct Cursor {
@@ -276,7 +267,9 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   __syncthreads();
   pdl_wait();
 
-  // ---- the line of units: prefix sums over the requests, by every warp for
+  // ---- the line: for every request, kv head and pass over its query heads a
+  // slot for the change to it (fetching q, writing the output: about the time
+  // of a unit) and one for each of its units. Prefix sums over the requests, by every warp for
   // itself (no barrier) up to 256 requests, by the CTA together above
   const bool few = a.seqs <= 32 * kRowsPerLane;
   const int per = few ? (a.seqs + 31) / 32 : (a.seqs + S::kThreads - 1) / S::kThreads;
@@ -287,13 +280,13 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
     for (int i = 0; i < kRowsPerLane; ++i) lens[i] = i < per && first_row + i < a.seqs ? row_len(a, first_row + i) : -1;
 #pragma unroll
-    for (int i = 0; i < kRowsPerLane; ++i) mine += (lens[i] + kUnit - 1) / kUnit, empty = empty || lens[i] == 0;
+    for (int i = 0; i < kRowsPerLane; ++i) mine += slots_of(lens[i]), empty = empty || lens[i] == 0;
     mine = warp_inclusive_sum(mine);
     sum = __shfl_sync(0xffffffffu, mine, 31);
   } else {
     for (int b = first_row; b < min(a.seqs, first_row + per); ++b) {
       const int len = row_len(a, b);
-      mine += (len + kUnit - 1) / kUnit;
+      mine += slots_of(len);
       empty = empty || len == 0;
     }
     ends[tid] = block_inclusive_sum(mine, scratch, sum);
@@ -307,15 +300,15 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       for (int h = lane; a.lse != nullptr && h < a.heads; h += 32) a.lse[(size_t)b * a.heads + h] = -INFINITY;
     }
   }
-  // Shares of the line: `share` units a CTA (the last may have less, and
+  // Shares of the line: `share` slots a CTA (the last may have less, and
   // CTAs past the line's end none), spread evenly over its warps.
   const uint32_t line = (uint32_t)sum * (uint32_t)passes;
   const uint32_t share = max((line + gridDim.x - 1) / gridDim.x, (uint32_t)kMinShare);
   const uint32_t cta0 = blockIdx.x * share;
   if (cta0 >= line) return;
-  const uint32_t cta_units = min(share, line - cta0);
-  const uint32_t u0 = cta0 + (uint32_t)((uint64_t)cta_units * warp / W);
-  const int count = (int)(cta0 + (uint32_t)((uint64_t)cta_units * (warp + 1) / W) - u0);
+  const uint32_t cta_slots = min(share, line - cta0);
+  uint32_t slot = cta0 + (uint32_t)((uint64_t)cta_slots * warp / W);
+  int count = (int)(cta0 + (uint32_t)((uint64_t)cta_slots * (warp + 1) / W) - slot);  // slots left
 
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * S::kRing;
   float *const part0 = reinterpret_cast<float *>(smem + (size_t)W * S::kRing) + warp * S::kPart;
@@ -326,42 +319,42 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   if (count > 0) {
     uint32_t before;
     if (few) {
-      const uint32_t beyond = __ballot_sync(0xffffffffu, (uint64_t)(uint32_t)mine * passes > u0);
+      const uint32_t beyond = __ballot_sync(0xffffffffu, (uint64_t)(uint32_t)mine * passes > slot);
       const int lo = beyond ? __ffs(beyond) - 1 : 31;
-      int units = 0, row = first_row, len = 0, sums = mine;
+      int row = first_row, len = 0, sums = mine;
 #pragma unroll
-      for (int i = 0; i < kRowsPerLane; ++i) sums -= (lens[i] + kUnit - 1) / kUnit;  // before this lane's rows
+      for (int i = 0; i < kRowsPerLane; ++i) sums -= slots_of(lens[i]);  // before this lane's rows
       bool found = false;
 #pragma unroll
       for (int i = 0; i < kRowsPerLane; ++i) {
-        const int n = (lens[i] + kUnit - 1) / kUnit;
+        const int n = slots_of(lens[i]);
         if (!found && n > 0) {
-          if ((uint64_t)(uint32_t)(sums + n) * passes > u0) found = true, units = n, row = first_row + i, len = lens[i];
+          if ((uint64_t)(uint32_t)(sums + n) * passes > slot) found = true, row = first_row + i, len = lens[i];
           else sums += n;
         }
       }
       at.row = __shfl_sync(0xffffffffu, row, lo), at.len = __shfl_sync(0xffffffffu, len, lo);
-      at.units = __shfl_sync(0xffffffffu, units, lo), before = __shfl_sync(0xffffffffu, sums, lo);
+      before = __shfl_sync(0xffffffffu, sums, lo);
     } else {
       int lo = 0, hi = S::kThreads - 1;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if ((uint64_t)(uint32_t)ends[mid] * passes > u0) hi = mid; else lo = mid + 1;
+        if ((uint64_t)(uint32_t)ends[mid] * passes > slot) hi = mid; else lo = mid + 1;
       }
       before = lo > 0 ? ends[lo - 1] : 0;
       const int last = min(a.seqs, (lo + 1) * per) - 1;
       for (at.row = lo * per;; ++at.row) {
         at.len = row_len(a, at.row);
-        at.units = (at.len + kUnit - 1) / kUnit;
-        if (at.row >= last || (uint64_t)(before + at.units) * passes > u0) break;
-        before += at.units;
+        if (at.row >= last || (uint64_t)(before + slots_of(at.len)) * passes > slot) break;
+        before += slots_of(at.len);
       }
     }
-    at.units = max(1, at.units);
-    const uint32_t in = u0 - before * (uint32_t)passes;
-    const int pass = (int)min((uint32_t)passes - 1, in / (uint32_t)at.units);
+    at.units = max(1, (at.len + kUnit - 1) / kUnit);
+    const uint32_t in = slot - before * (uint32_t)passes, each = (uint32_t)at.units + 1;
+    const int pass = (int)min((uint32_t)passes - 1, in / each);
     at.kh = pass / a.tiles, at.tile = pass % a.tiles;
-    at.k = (int)(in - (uint32_t)pass * (uint32_t)at.units);
+    at.k = (int)(in - (uint32_t)pass * each) - 1;
+    if (at.k < 0) at.k = 0, --count, ++slot;
   }
   if (!few) __syncthreads();  // `ends` gives way to the parts
 
@@ -376,13 +369,14 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     int to_look = count;
     auto look_up = [&] {
       left = 0;
-      if (to_look == 0) return;
+      if (to_look <= 0) return;
       const int key = look.k * kUnit + sub;
       left = look.len - look.k * kUnit;
       head = look.kh;
       token = key & mask;
       page = sub < min(left, kUnit) ? __ldg(pages + (key >> a.shift)) : 0;
-      if (--to_look == 0) return;
+      to_look -= look.k + 1 == look.units ? 2 : 1;  // the unit's slot, and that of the change to the next request
+      if (to_look <= 0) return;
       const int row = look.row;
       look.step(a);
       if (look.row != row) pages = a.table + (size_t)look.row * a.max_pages;
@@ -414,14 +408,34 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll 1
     for (int s = 0; s < ST - 1; ++s) issue();
 
+    // q as it lies in memory, heads 8 nt + g of a pass, dimensions in the order
+    // of the keys' pieces. With one tile of heads it is fetched a request part
+    // ahead (two tiles leave no registers for that).
+    uint4 raw[NT][D / 32];
+    auto load_q = [&](const Cursor &c) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = c.tile * S::kHeads + 8 * nt + g;
+        const Io *src = static_cast<const Io *>(a.q) + c.row * a.q_ld + (long long)(c.kh * a.group + h) * a.dim;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          // runs of 8: for 16-bit caches piece t + 4i, for 8-bit ones half of a piece of 16
+          const int d = F8 ? 16 * (t + 4 * (i >> 1)) + 8 * (i & 1) : 8 * (t + 4 * i);
+          raw[nt][i] = h < a.group && d < a.dim ? __ldg(reinterpret_cast<const uint4 *>(src + d)) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    if constexpr (NT == 1) load_q(at);
+    const uint8_t *const ring_ptr = smem + (size_t)warp * S::kRing;
+
     // ---- the share
     uint32_t q[NT][D / 8];       // this lane's part of the contracted dimension, heads 8 nt + g
     float cs[NT][2];             // score factor (base 2) of heads 8 nt + 2t, + 1
     float m[NT][2], l[NT][2];    // running maximum (base 2) and this lane's sum
     float o[NT][S::kVals / 2][4];
     int k0 = at.k;               // first unit of the current request part
-    uint32_t start = u0;
-    bool fresh = true;
+    uint32_t start = slot;
+    bool fresh = true, first_part = true;
     // Row g of the products stands for key pi, row g + 8 for pi + 8.
     const int pi = g & 1 ? (g + 4) & 7 : g, pe = 2 * t, po = (2 * t + 5) & 7;  // pi of g, 2t, 2t + 1
     uint32_t key_at[2], val_at[2];  // this lane's pieces in a stage
@@ -434,22 +448,14 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     }
     int stage = 0, landed = 0;
     uint32_t parity = 0;
-    for (int it = 0; it < count; ++it) {
+    for (;;) {
       if (fresh) {
         fresh = false;
-        const int kh = at.kh, h0 = at.tile * S::kHeads;
+        if constexpr (NT > 1) load_q(at);
+        const int kh = at.kh;
         const float ks = a.k_scale != nullptr ? __ldg(a.k_scale + kh) : 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const int h = h0 + 8 * nt + g;
-          const Io *src = static_cast<const Io *>(a.q) + at.row * a.q_ld + (long long)(kh * a.group + h) * a.dim;
-          uint4 raw[D / 32];
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            // element run of 8: for 16-bit caches chunk t + 4c, for 8-bit ones half of a 16-element chunk
-            const int d = F8 ? 16 * (t + 4 * (c >> 1)) + 8 * (c & 1) : 8 * (t + 4 * c);
-            raw[c] = h < a.group && d < a.dim ? __ldg(reinterpret_cast<const uint4 *>(src + d)) : make_uint4(0, 0, 0, 0);
-          }
           float f = a.scale * kLog2e * ks;
           if constexpr (F8) {
             // The 8-bit cache's products are f16. q is brought into f16's
@@ -458,7 +464,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
             float x[D / 4], top = 0.f;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-              const Io *e = reinterpret_cast<const Io *>(&raw[c]);
+              const Io *e = reinterpret_cast<const Io *>(&raw[nt][c]);
 #pragma unroll
               for (int i = 0; i < 8; ++i) x[8 * c + i] = to_float(e[i]), top = fmaxf(top, fabsf(x[8 * c + i]));
             }
@@ -473,7 +479,8 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
           } else {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c)
-              q[nt][4 * c] = raw[c].x, q[nt][4 * c + 1] = raw[c].y, q[nt][4 * c + 2] = raw[c].z, q[nt][4 * c + 3] = raw[c].w;
+              q[nt][4 * c] = raw[nt][c].x, q[nt][4 * c + 1] = raw[nt][c].y, q[nt][4 * c + 2] = raw[nt][c].z,
+              q[nt][4 * c + 3] = raw[nt][c].w;
           }
           // the factor of head 8 nt + g lives in lanes 4g ..; this lane's columns are 2t, 2t + 1
           cs[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
@@ -483,22 +490,54 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
           for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
         }
+        if (NT == 1 && count - (at.units - at.k) > 1) {
+          Cursor next = at;
+          next.k = next.units - 1;
+          next.step(a);
+          load_q(next);
+        }
       }
       if (!warp_wait(&full[warp][stage], parity, &g_attention_wait, kSiteWait)) break;
       ++landed;
       issue();  // into the stage that the previous unit left
-      const uint32_t st = ring + (uint32_t)stage * S::kStageBytes;
-      // ---- scores: 16 keys x 8 NT heads
-      float s[NT][4], s2[NT][4];
+      const uint8_t *const st = ring_ptr + (uint32_t)stage * S::kStageBytes;
+      const bool tail = at.k + 1 == at.units;     // may have keys past the length
+      const int n_live = at.len - at.k * kUnit;
+      // ---- all of the unit into registers: the loads of the values are under way during the scores
+      uint4 kx[S::kKeyChunks][2];
+#pragma unroll
+      for (int c = 0; c < S::kKeyChunks; ++c)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          kx[c][r] = *reinterpret_cast<const uint4 *>(st + key_at[c & 1] + (c >> 1) * S::kTileBytes + r * (8 * 128));
+      constexpr int kWords = S::kValBytes * S::kValChunks / 4;
+      uint32_t x[4][kWords];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < S::kValChunks; ++c) {
+          const uint8_t *from = st + val_at[r & 1] + c * S::kTileBytes + (r >> 1) * (8 * 128);
+          if constexpr (S::kValBytes == 16) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(from);
+            x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
+          } else {
+            const uint2 y = *reinterpret_cast<const uint2 *>(from);
+            x[r][0] = y.x, x[r][1] = y.y;
+          }
+        }
+      // ---- scores: 16 keys x 8 NT heads, in sums of their own per 16 bytes of keys
+      constexpr int kSums = 2 * S::kKeyChunks > 4 ? 4 : 2 * S::kKeyChunks;
+      float part_s[NT][kSums][4], s[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.f;
+        for (int y = 0; y < kSums; ++y)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part_s[nt][y][i] = 0.f;
 #pragma unroll
       for (int c = 0; c < S::kKeyChunks; ++c) {
-        const uint32_t from = st + key_at[c & 1] + (c >> 1) * S::kTileBytes;
-        const uint4 x = lds16(from), y = lds16(from + 8 * 128);
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+        const uint32_t xw[4] = {kx[c][0].x, kx[c][0].y, kx[c][0].z, kx[c][0].w};
+        const uint32_t yw[4] = {kx[c][1].x, kx[c][1].y, kx[c][1].z, kx[c][1].w};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if constexpr (F8) {
@@ -507,44 +546,44 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
               uint32_t x0, x1, y0, y1;
               e4m3_to_f16(xw[j], x0, x1);
               e4m3_to_f16(yw[j], y0, y1);
-              mma<BF>((j & 1) ? s2[nt] : s[nt], x0, y0, x1, y1, q[nt][8 * c + 2 * j], q[nt][8 * c + 2 * j + 1]);
+              mma<BF>(part_s[nt][(4 * c + j) % kSums], x0, y0, x1, y1, q[nt][8 * c + 2 * j], q[nt][8 * c + 2 * j + 1]);
             }
           } else {
-            mma<BF>(s[nt], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
-            mma<BF>(s2[nt], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
+            mma<BF>(part_s[nt][2 * c % kSums], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
+            mma<BF>(part_s[nt][(2 * c + 1) % kSums], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
           }
         }
       }
-      // ---- softmax: keys g (elements 0, 1) and g + 8 (2, 3) of heads 2t, 2t + 1
+      // ---- softmax: keys of rows g (elements 0, 1) and g + 8 (2, 3), heads 2t, 2t + 1.
+      // The maximum that the weights refer to moves only when a score passes
+      // it by more than 8 (2^8 is far inside both 16-bit types' range), so
+      // that most units need a vote instead of a reduction and a rescaling.
       uint32_t big[NT][2], rest[NT][2];
-      float top[NT][2];
+      bool grew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * cs[nt][i & 1];
-        if (at.k + 1 == at.units) {  // the last unit may have keys past the length
-          const int n = at.len - at.k * kUnit;
+        for (int i = 0; i < 4; ++i) {
+          float y = part_s[nt][0][i] + part_s[nt][1][i];
+          if constexpr (kSums == 4) y += part_s[nt][2][i] + part_s[nt][3][i];
+          s[nt][i] = y * cs[nt][i & 1];
+        }
+        if (tail) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = pi + 8 * (i >> 1) < n ? s[nt][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[nt][i] = pi + 8 * (i >> 1) < n_live ? s[nt][i] : -INFINITY;
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(s[nt][j], s[nt][j + 2]);
+        for (int i = 0; i < 4; ++i) grew = grew || s[nt][i] > m[nt][i & 1] + 8.f;
       }
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
-      bool grew = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) grew = grew || top[nt][0] > m[nt][0] || top[nt][1] > m[nt][1];
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float mn = fmaxf(m[nt][j], top[nt][j]);
+            float top = fmaxf(s[nt][j], s[nt][j + 2]);
+#pragma unroll
+            for (int y = 4; y < 32; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            const float mn = fmaxf(m[nt][j], top);
             const float f = mn == -INFINITY ? 1.f : exp2_approx(m[nt][j] - mn);
             m[nt][j] = mn;
             l[nt][j] *= f;
@@ -567,26 +606,10 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
         for (int r = 0; r < 2; ++r) big[nt][r] = transpose8x8(big[nt][r]), rest[nt][r] = transpose8x8(rest[nt][r]);
       }
       // ---- values: rows of V^T are this lane's kVals dimensions, in pairs (i, i + kVals / 2)
-      constexpr int kWords = S::kValBytes * S::kValChunks / 4;
-      uint32_t x[4][kWords];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < S::kValChunks; ++c) {
-          const uint32_t from = st + val_at[r & 1] + c * S::kTileBytes + (r >> 1) * (8 * 128);
-          if constexpr (S::kValBytes == 16) {
-            const uint4 y = lds16(from);
-            x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
-          } else {
-            const uint2 y = lds8(from);
-            x[r][0] = y.x, x[r][1] = y.y;
-          }
-        }
-      if (at.k + 1 == at.units) {  // weights of 0 must meet values of 0, whatever the cache holds there
-        const int n = at.len - at.k * kUnit;
+      if (tail) {  // weights of 0 must meet values of 0, whatever the cache holds there
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if ((r & 1 ? po : pe) + 8 * (r >> 1) >= n)
+          if ((r & 1 ? po : pe) + 8 * (r >> 1) >= n_live)
 #pragma unroll
             for (int w = 0; w < kWords; ++w) x[r][w] = 0;
       }
@@ -618,13 +641,15 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 
       // ---- end of the request's keys, or of the share
       const bool ends_here = at.k + 1 == at.units;
-      if (ends_here || it + 1 == count) {
+      --count, ++slot;
+      const bool over = count == 0 || (ends_here && count == 1);
+      if (ends_here || over) {
         const int kh = at.kh, h0 = at.tile * S::kHeads;
         const bool whole = ends_here && k0 == 0;
         const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + kh) : 1.f;
-        const int slot = start == u0 ? 0 : 1;
-        float *part = slot ? part1 : part0;
-        if (slot && !whole) __syncwarp();  // the ring is the second part's place: every lane is done with the last unit
+        const int place = first_part ? 0 : 1;
+        float *part = place ? part1 : part0;
+        if (place && !whole) __syncwarp();  // the ring is the second part's place: every lane is done with the last unit
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -663,14 +688,16 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
             }
           }
         if (!whole && lane == 0) {
-          spans[2 * warp + slot] = {start, at.row, at.kh, at.tile, k0, at.k + 1, at.units};
-          span_used[2 * warp + slot] = 1;
+          spans[2 * warp + place] = {start, at.row, at.kh, at.tile, k0, at.k + 1, at.units};
+          span_used[2 * warp + place] = 1;
         }
-        fresh = true;
-        start = u0 + it + 1;
+        if (over) break;
+        fresh = true, first_part = false;
+        --count;
+        start = ++slot;
         k0 = 0;
       }
-      if (it + 1 < count) at.step(a);
+      at.step(a);
     }
     // After a wait that gave up: no copy may land in the memory of a CTA that has left.
     for (; landed < issued; ++landed) {
@@ -733,7 +760,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
         if (d == 0) {
           __stcg(reinterpret_cast<float2 *>(place + ml), make_float2(m, l));
           if (h == 0) {  // CTAs of the request's first and last unit
-            const uint32_t b0 = first.unit0 - first.k0;
+            const uint32_t b0 = first.slot - first.k0;
             crossing[atomicAdd(&n_crossing, 1)] = {first.row, first.kh, first.tile, (int)(b0 / share),
                                                    (int)((b0 + first.units - 1) / share)};
           }
@@ -942,8 +969,8 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   a.group = heads / kv->kv_heads;
   a.tiles = a.group <= 8 ? 1 : (a.group + kMaxSplitHeads - 1) / kMaxSplitHeads;
   a.scale = scale;
-  const int64_t units = (int64_t)pt->max_pages * pt->page_size / kUnit + 1;  // of a full row
-  CE_REQUIRE(pt->seqs * units < (1ll << 31) && (double)pt->seqs * units * kv->kv_heads * a.tiles < 4294967296.0 - kMaxGrid,
+  const int64_t slots = (int64_t)pt->max_pages * pt->page_size / kUnit + 2;  // slots of a full row at most
+  CE_REQUIRE(pt->seqs * slots < (1ll << 31) && (double)pt->seqs * slots * kv->kv_heads * a.tiles < 4294967296.0 - kMaxGrid,
              "seqs x max_pages x page_size x kv_heads is too large (%d x %d x %d x %d)", pt->seqs, pt->max_pages,
              pt->page_size, kv->kv_heads);
   a.arrivals = static_cast<int *>(workspace);
