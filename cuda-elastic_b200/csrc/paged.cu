@@ -50,69 +50,97 @@ __device__ __forceinline__ bool page_ok(const Tables &t, int page) {
   return false;
 }
 
-// This CTA's share [lo, hi) of the pages (a multiple of 32 pages each, so
-// that a word of the free map belongs to one CTA).
-struct Share {
-  int lo, hi;
+// The CTA's place in its cluster.
+struct Cluster {
+  int rank, ranks;
 };
-__device__ __forceinline__ Share page_share(int pages, int rank, int ranks) {
-  const int per = ((pages + ranks - 1) / ranks + 31) / 32 * 32;
-  const int lo = min(pages, rank * per);
-  return {lo, min(pages, lo + per)};
+__device__ __forceinline__ Cluster this_cluster() {
+  int n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return {(int)cluster_ctarank(), n};
 }
-
-// Free map of the CTA's share: bit p of word w is set when page lo + 32 w + p
-// has no holder. Returns the number of free pages (same value in all threads).
-__device__ __forceinline__ int map_free(const Tables &t, Share sh, uint32_t *map, int *scratch) {
-  const int lane = threadIdx.x & 31;
-  int mine = 0;
-  for (int p = sh.lo + (int)threadIdx.x; p - lane < sh.hi; p += blockDim.x) {
-    const bool free = p < sh.hi && __ldcg(t.refs + p) == 0;
-    const uint32_t word = __ballot_sync(0xffffffffu, free);
-    if (lane == 0) {
-      map[(p - sh.lo) >> 5] = word;
-      mine += __popc(word);
-    }
-  }
-  int total;
-  block_inclusive_sum(mine, scratch, total);
-  return total;
-}
-
-// Calls take(rank, page) for the free pages of the share whose rank (`base` +
-// the free pages of the share before it) is below `limit`.
-template <class F>
-__device__ __forceinline__ void each_free(Share sh, const uint32_t *map, int base, int limit, int *scratch, F &&take) {
-  const int words = (sh.hi - sh.lo + 31) >> 5;
-  for (int w0 = 0; w0 < words && base < limit; w0 += blockDim.x) {
-    const int w = w0 + threadIdx.x;
-    uint32_t bits = w < words ? map[w] : 0u;
-    int total;
-    int rank = base + block_inclusive_sum(__popc(bits), scratch, total) - __popc(bits);
-    for (; bits != 0u && rank < limit; bits &= bits - 1, ++rank) take(rank, sh.lo + 32 * w + __ffs(bits) - 1);
-    base += total;
-  }
-}
-
-// Free pages of the CTAs before this one, and of all.
-__device__ __forceinline__ void free_before(int *count, int rank, int ranks, int &before, int &total) {
-  before = total = 0;
-  const uint32_t here = smem_u32(count);
-  for (int r = 0; r < ranks; ++r) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_map(here, (uint32_t)r)) : "memory");
-    before += r < rank ? v : 0;
-    total += v;
-  }
-}
-
-__device__ __forceinline__ int cluster_ranks() {
-  int r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
+__device__ __forceinline__ void sync_all(Cluster c) {
+  if (c.ranks == 1) __syncthreads(); else cluster_sync();
 }
 
 __device__ __forceinline__ int clamp_int(long long v) { return v > 0x7fffffffll ? 0x7fffffff : (int)v; }
+
+// The map of free pages, one bit each, in shares: CTA r of the cluster keeps
+// the words of pages [r per, (r + 1) per), per a multiple of 32.
+struct FreeMap {
+  uint32_t *words;  // this CTA's
+  int *ends;        // prefix sums of their free pages, after count()
+  int per, lo, hi;
+  __device__ __forceinline__ FreeMap(uint32_t *w, int pages, Cluster c) : words(w) {
+    per = ((pages + c.ranks - 1) / c.ranks + 31) / 32 * 32;
+    lo = min(pages, c.rank * per);
+    hi = min(pages, lo + per);
+    ends = reinterpret_cast<int *>(w + per / 32);
+  }
+  // Reads refs once: the map, and the copy into `t.refs` where that is another buffer.
+  __device__ __forceinline__ void fill(const Tables &t) const {
+    const int lane = threadIdx.x & 31;
+    for (int p0 = lo + (int)threadIdx.x - lane; p0 < hi; p0 += blockDim.x * 4) {
+      int v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + i * (int)blockDim.x + lane;
+        v[i] = p < hi ? __ldcg(t.refs_in + p) : 1;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + i * (int)blockDim.x + lane;
+        const uint32_t word = __ballot_sync(0xffffffffu, v[i] == 0);
+        if (p < hi && t.refs != t.refs_in) t.refs[p] = v[i];
+        if (lane == 0 && p < hi) words[(p - lo) >> 5] = word;
+      }
+    }
+  }
+  // A page that has lost its last holder.
+  __device__ __forceinline__ void set(int page) const {
+    const int r = page / per, in = page - r * per;
+    const uint32_t word = cluster_map(smem_u32(words + (in >> 5)), (uint32_t)r);
+    asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(word), "r"(1u << (in & 31)) : "memory");
+  }
+  // Prefix sums over the words; the number of free pages of the share.
+  __device__ __forceinline__ int count(int *scratch) const {
+    const int n = (hi - lo + 31) >> 5;
+    int base = 0;
+    for (int w0 = 0; w0 < n; w0 += blockDim.x) {
+      const int w = w0 + threadIdx.x;
+      int total;
+      const int sum = block_inclusive_sum(w < n ? __popc(words[w]) : 0, scratch, total);
+      if (w < n) ends[w] = base + sum;
+      base += total;
+    }
+    return base;
+  }
+  // The r-th free page of the share (r from 0, below count()).
+  __device__ __forceinline__ int nth(int r) const {
+    const int w = first_above(ends, (hi - lo + 31) >> 5, r);
+    uint32_t bits = words[w];
+    r -= w ? ends[w - 1] : 0;
+    int at = 0;
+#pragma unroll
+    for (int half = 16; half; half >>= 1) {  // the half word that holds the r-th set bit
+      const int n = __popc(bits & ((1u << half) - 1u));
+      if (r >= n) r -= n, bits >>= half, at += half;
+    }
+    return lo + 32 * w + at;
+  }
+};
+
+// Free pages of the CTAs before this one, and of all.
+__device__ __forceinline__ void free_before(int *count, Cluster c, int &before, int &total) {
+  before = total = 0;
+  const uint32_t here = smem_u32(count);
+  for (int r = 0; r < c.ranks; ++r) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_map(here, (uint32_t)r)) : "memory");
+    before += r < c.rank ? v : 0;
+    total += v;
+  }
+}
 
 // ---------------------------------------------------------------------------
 // resize
@@ -125,71 +153,82 @@ struct ResizeArgs {
   int capacity;
 };
 
-// One cluster. Every CTA scans all rows (they are few) and a share of the
-// pages; the phases are parted by cluster barriers:
-//   1. shrinking rows give pages back (integer atomics on refs);
-//   2. each row's need of pages and tokens, their prefix sums; the free map;
-//   3. the free pages of rank below the need go to the row that the rank
-//      falls into (binary search in the prefix sums);
-//   4. slots and positions, token by token, the same way.
-__global__ void __launch_bounds__(kTableThreads) resize_kernel(ResizeArgs a) {
+// One cluster; its time is a chain of dependent reads and barriers, so each
+// input is read once, early, and phases that have nothing to do are skipped.
+// Every CTA goes over all rows (they are few, and sums over them are needed
+// everywhere) and over its share of the pages:
+//   1. lengths into shared memory, the free map (and copy) of refs;
+//   2. if a row gets shorter: its pages lose a holder (integer atomics), the
+//      last holder's loss sets the page's bit in the map;
+//   3. each row's need of pages and tokens, and their prefix sums;
+//   4. page r of those needed is the r-th free one: the rank is looked up in
+//      the map's prefix sums, its row and column in the rows';
+//   5. slots and positions, token by token, by the rows' prefix sums.
+__global__ void __launch_bounds__(kTableThreads) resize_kernel(const __grid_constant__ ResizeArgs a) {
   extern __shared__ int smem[];
   __shared__ long long scratch8[32];
   __shared__ int scratch4[32];
   __shared__ int s_free, s_pages, s_tokens, s_refused;
   const Tables &t = a.t;
-  const int n = t.n, tid = threadIdx.x, lane = tid & 31;
-  const int rank = (int)cluster_ctarank(), ranks = cluster_ranks();
-  int *need_end = smem, *tok_end = smem + n, *old_len = smem + 2 * n;
-  uint32_t *map = reinterpret_cast<uint32_t *>(smem + 3 * n);
-  const Share sh = page_share(t.pages, rank, ranks);
+  const int n = t.n, tid = threadIdx.x, lane = tid & 31, mask = (1 << t.shift) - 1;
+  const Cluster c = this_cluster();
+  int *need_end = smem, *tok_end = smem + n, *old_len = smem + 2 * n, *new_len = smem + 3 * n;
+  const FreeMap map(reinterpret_cast<uint32_t *>(smem + 4 * n), t.pages, c);
   pdl_launch_dependents();
+  if (tid == 0) s_pages = s_tokens = s_refused = 0;
   pdl_wait();
 
-  if (t.refs != t.refs_in)
-    for (int p = sh.lo + tid; p < sh.hi; p += blockDim.x) t.refs[p] = t.refs_in[p];
-  if (tid == 0) s_pages = s_tokens = s_refused = 0;
-  cluster_sync();
-  // 1. pages given back (and, with another table, the rows that stay)
-  const int warps = ranks * (int)(blockDim.x >> 5);
-  for (int i = rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
-    const int have = pages_of(held_len(t, i), t.shift);
-    const int want = a.new_lens[i] < 0 ? have : pages_of(a.new_lens[i], t.shift);
-    const int32_t *row = t.table_in + (size_t)i * t.max_pages;
-    for (int j = want + lane; j < have; j += 32)
-      if (page_ok(t, row[j])) atomicAdd(t.refs + row[j], -1);
-    if (t.table != t.table_in)
-      for (int j = lane; j < min(want, have); j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
+  // 1.
+  bool shorter = false;
+  for (int i = tid; i < n; i += blockDim.x) {
+    const int len = a.new_lens[i], old = held_len(t, i);
+    old_len[i] = old;
+    new_len[i] = len < 0 ? old : len;
+    shorter = shorter || (len >= 0 && len < old) || t.table != t.table_in;
   }
-  cluster_sync();
-  // 2. needs
-  const int free = map_free(t, sh, map, scratch4);
-  if (tid == 0) s_free = free;
-  cluster_sync();
-  int before, total_free;
-  free_before(&s_free, rank, ranks, before, total_free);
+  map.fill(t);
+  shorter = __syncthreads_or(shorter);
+  // 2. (with another table: the rows that stay, too)
+  if (shorter) {
+    sync_all(c);  // every CTA's share of refs is copied
+    const int warps = c.ranks * (int)(blockDim.x >> 5);
+    for (int i = c.rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
+      const int have = pages_of(old_len[i], t.shift), want = pages_of(new_len[i], t.shift);
+      const int32_t *row = t.table_in + (size_t)i * t.max_pages;
+      for (int j = want + lane; j < have; j += 32)
+        if (page_ok(t, row[j]) && atomicAdd(t.refs + row[j], -1) == 1) map.set(row[j]);
+      if (t.table != t.table_in)
+        for (int j = lane; j < min(want, have); j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
+    }
+  }
+  sync_all(c);
+  // 3.
   const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
   long long need_sum = 0, tok_sum = 0;
   int growing = 0, granted = 0;
   for (int i = r0; i < r1; ++i) {
-    const int old = held_len(t, i), len = a.new_lens[i];
+    const int old = old_len[i], len = new_len[i];
     const int have = pages_of(old, t.shift), want = pages_of(len, t.shift);
     bool fits = len > old && want <= t.max_pages;
     growing += len > old;
-    if (fits && (old & ((1 << t.shift) - 1)) != 0) {  // its last page is partly filled
+    if (fits && (old & mask) != 0) {  // its last page is partly filled
       const int tail = t.table_in[(size_t)i * t.max_pages + (old >> t.shift)];
       fits = page_ok(t, tail) && __ldcg(t.refs + tail) == 1;
     }
     need_sum += fits ? want - have : 0;
     tok_sum += fits ? len - old : 0;
-    old_len[i] = old;
     need_end[i] = clamp_int(need_sum);  // made absolute below
     tok_end[i] = fits ? clamp_int(tok_sum) : -1 - clamp_int(tok_sum);  // sign: does not fit
   }
+  const int free = map.count(scratch4);
+  if (tid == 0) s_free = free;
   long long all;
   const long long need0 = block_inclusive_sum(need_sum, scratch8, all) - need_sum;
   const long long tok0 = block_inclusive_sum(tok_sum, scratch8, all) - tok_sum;
+  sync_all(c);
+  int before, total_free;
+  free_before(&s_free, c, before, total_free);
   int pages_given = 0, tokens_given = 0;
   for (int i = r0; i < r1; ++i) {
     const bool fits = tok_end[i] >= 0;
@@ -199,37 +238,37 @@ __global__ void __launch_bounds__(kTableThreads) resize_kernel(ResizeArgs a) {
   }
   if (granted) atomicMax(&s_pages, pages_given), atomicMax(&s_tokens, tokens_given);
   if (growing != granted) atomicAdd(&s_refused, growing - granted);
-  cluster_sync();
+  __syncthreads();
   const int R = s_pages, T = s_tokens;
-  // 3. pages
-  each_free(sh, map, before, R, scratch4, [&](int r, int page) {
-    const int i = first_above(need_end, n, r);
+  // 4.
+  for (int r = before + tid; r < min(R, before + free); r += blockDim.x) {
+    const int page = map.nth(r - before), i = first_above(need_end, n, r);
     const int col = pages_of(old_len[i], t.shift) + r - (i ? need_end[i - 1] : 0);
     t.table[(size_t)i * t.max_pages + col] = page;
     t.refs[page] = 1;
-  });
-  cluster_sync();
-  // 4. slots; no CTA reads the old lengths any more
-  const int threads = ranks * (int)blockDim.x;
-  for (int j = rank * (int)blockDim.x + tid; j < a.capacity; j += threads) {
+  }
+  sync_all(c);
+  // 5. (no CTA reads the old lengths any more)
+  const int threads = c.ranks * (int)blockDim.x, first = c.rank * (int)blockDim.x + tid;
+  for (int j = first; j < a.capacity; j += threads) {
     long long slot = -1;
     int pos = -1;
     if (j < T) {
       const int i = first_above(tok_end, n, j);
       pos = old_len[i] + j - (i ? tok_end[i - 1] : 0);
       const int page = __ldcg(t.table + (size_t)i * t.max_pages + (pos >> t.shift));
-      slot = ((long long)page << t.shift) + (pos & ((1 << t.shift) - 1));
+      slot = ((long long)page << t.shift) + (pos & mask);
     }
     a.slots[j] = slot;
     a.pos[j] = pos;
   }
-  for (int i = rank * (int)blockDim.x + tid; i < n; i += threads) {
-    const int first = i ? tok_end[i - 1] : 0, old = old_len[i], len = a.new_lens[i];
-    const bool given = tok_end[i] > first && tok_end[i] <= T && need_end[i] <= R;
-    t.lens[i] = given || (len >= 0 && len < old) ? len : old;
-    if (a.starts != nullptr) a.starts[i] = min(first, T);
+  for (int i = first; i < n; i += threads) {
+    const int start = i ? tok_end[i - 1] : 0, old = old_len[i], len = new_len[i];
+    const bool given = tok_end[i] > start && tok_end[i] <= T && need_end[i] <= R;
+    t.lens[i] = given || len < old ? len : old;
+    if (a.starts != nullptr) a.starts[i] = min(start, T);
   }
-  if (rank == 0 && tid == 0) {
+  if (c.rank == 0 && tid == 0) {
     if (a.starts != nullptr) a.starts[n] = T;
     if (t.status != nullptr) {
       t.status[0] = R;
@@ -238,7 +277,6 @@ __global__ void __launch_bounds__(kTableThreads) resize_kernel(ResizeArgs a) {
       t.status[3] = T;
     }
   }
-  cluster_sync();  // no CTA leaves while another reads its free count
 }
 
 // ---------------------------------------------------------------------------
@@ -252,104 +290,105 @@ struct ReorderArgs {
 };
 
 // One cluster, in the manner of resize_kernel:
-//   1. refs of every page of old row i change by (children of i) - 1, and
-//      each new row's pages are those of its parent;
-//   2. rows whose partly filled last page is held by another row too need a
-//      page of their own, all but the first of the group when the group
-//      alone holds it; prefix sum over rows, free map over pages;
-//   3. the free pages of the lowest ranks go to those rows.
-__global__ void __launch_bounds__(kTableThreads) reorder_kernel(ReorderArgs a) {
+//   1. each new row's parent, length and partly filled last page, the
+//      children of each old row, the free map;
+//   2. refs of every page of old row i change by (children of i) - 1, and
+//      each new row's pages are those of its parent. A page comes to 0 only
+//      when every row that held it is without children, so whoever brings it
+//      there may set its bit, whatever the order;
+//   3. rows whose last page another row holds too need a page of their own,
+//      all but the first of the group when the group alone holds it;
+//   4. the free pages of the lowest ranks go to those rows.
+__global__ void __launch_bounds__(kTableThreads) reorder_kernel(const __grid_constant__ ReorderArgs a) {
   extern __shared__ int smem[];
   __shared__ int scratch4[32];
   __shared__ int s_free;
   const Tables &t = a.t;
-  const int n = t.n, K = a.beams, tid = threadIdx.x, lane = tid & 31;
-  const int rank = (int)cluster_ctarank(), ranks = cluster_ranks();
-  int *new_len = smem, *tail = smem + n, *copy_end = smem + 2 * n;
-  uint32_t *map = reinterpret_cast<uint32_t *>(smem + 3 * n);
-  const Share sh = page_share(t.pages, rank, ranks);
+  const int n = t.n, K = a.beams, tid = threadIdx.x, lane = tid & 31, mask = (1 << t.shift) - 1;
+  const Cluster c = this_cluster();
+  int *new_len = smem, *tail = smem + n, *copy_end = smem + 2 * n, *children = smem + 3 * n;
+  const FreeMap map(reinterpret_cast<uint32_t *>(smem + 4 * n), t.pages, c);
   pdl_launch_dependents();
+  for (int i = tid; i < n; i += blockDim.x) children[i] = 0;
+  __syncthreads();
   pdl_wait();
 
-  if (t.refs != t.refs_in)
-    for (int p = sh.lo + tid; p < sh.hi; p += blockDim.x) t.refs[p] = t.refs_in[p];
+  // 1.
   for (int i = tid; i < n; i += blockDim.x) {
     const int p = a.parents[i], src = i - i % K + p;
     const bool kept = p >= 0 && p < K;
     const int len = kept ? held_len(t, src) : 0;
-    new_len[i] = len;
     int page = -1;
-    if ((len & ((1 << t.shift) - 1)) != 0) {
+    if ((len & mask) != 0) {
       page = t.table_in[(size_t)src * t.max_pages + (len >> t.shift)];
       if (!page_ok(t, page)) page = -1;
     }
+    if (kept) atomicAdd(children + src, 1);
+    new_len[i] = len;
     tail[i] = page;
   }
-  cluster_sync();
-  // 1. references and rows
-  const int warps = ranks * (int)(blockDim.x >> 5);
-  for (int i = rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
-    const int g = i - i % K;
-    int children = 0;
-    for (int k = lane; k < K; k += 32) children += a.parents[g + k] == i - g;
-    children = __reduce_add_sync(0xffffffffu, children);
-    if (children != 1) {
-      const int have = pages_of(held_len(t, i), t.shift);
-      for (int j = lane; j < have; j += 32) {
-        const int page = t.table_in[(size_t)i * t.max_pages + j];
-        if (page_ok(t, page)) atomicAdd(t.refs + page, children - 1);
-      }
+  map.fill(t);
+  sync_all(c);
+  // 2.
+  const int warps = c.ranks * (int)(blockDim.x >> 5);
+  for (int i = c.rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
+    const int held = pages_of(new_len[i], t.shift), delta = children[i] - 1;
+    const int32_t *from = t.table_in + (size_t)(i - i % K + (held ? a.parents[i] : 0)) * t.max_pages;
+    const int32_t *mine = t.table_in + (size_t)i * t.max_pages;
+    const int have = delta != 0 ? pages_of(held_len(t, i), t.shift) : 0;
+    for (int j = lane; j < held; j += 32) t.table[(size_t)i * t.max_pages + j] = from[j];
+    for (int j = lane; j < have; j += 32) {
+      const int page = mine[j];
+      if (page_ok(t, page) && atomicAdd(t.refs + page, delta) + delta == 0) map.set(page);
     }
-    const int held = pages_of(new_len[i], t.shift);
-    const int32_t *row = t.table_in + (size_t)(g + (held ? a.parents[i] : 0)) * t.max_pages;
-    for (int j = lane; j < held; j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
   }
-  cluster_sync();
-  // 2. rows that need a page
-  const int free = map_free(t, sh, map, scratch4);
-  if (tid == 0) s_free = free;
+  sync_all(c);
+  // 3.
   const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
   const int r0 = min(n, tid * per), r1 = min(n, r0 + per);
   int want = 0;
   for (int i = r0; i < r1; ++i) {
     const int page = tail[i], g = i - i % K;
     if (page >= 0) {
+      const int refs = __ldcg(t.refs + page);
       int holders = 0, first = K;
       for (int k = K - 1; k >= 0; --k)
         if (tail[g + k] == page) ++holders, first = k;
-      want += !(first == i - g && __ldcg(t.refs + page) == holders);
+      want += !(first == i - g && refs == holders);
     }
     copy_end[i] = want;  // made absolute below
   }
+  const int free = map.count(scratch4);
+  if (tid == 0) s_free = free;
   int wanted;
   const int want0 = block_inclusive_sum(want, scratch4, wanted) - want;
   for (int i = r0; i < r1; ++i) copy_end[i] += want0;
-  cluster_sync();
+  sync_all(c);
   int before, total_free;
-  free_before(&s_free, rank, ranks, before, total_free);
+  free_before(&s_free, c, before, total_free);
   const int R = min(wanted, total_free);
-  // 3. pages
-  each_free(sh, map, before, R, scratch4, [&](int r, int page) {
-    const int i = first_above(copy_end, n, r);
+  // 4.
+  for (int r = before + tid; r < min(R, before + free); r += blockDim.x) {
+    const int page = map.nth(r - before), i = first_above(copy_end, n, r);
     t.table[(size_t)i * t.max_pages + (new_len[i] >> t.shift)] = page;
     t.refs[page] = 1;
     atomicAdd(t.refs + tail[i], -1);
     a.copies[2 * i] = tail[i];
     a.copies[2 * i + 1] = page;
-  });
-  const int threads = ranks * (int)blockDim.x;
-  for (int i = rank * (int)blockDim.x + tid; i < n; i += threads) {
+  }
+  const int threads = c.ranks * (int)blockDim.x;
+  for (int i = c.rank * (int)blockDim.x + tid; i < n; i += threads) {
     const int r = i ? copy_end[i - 1] : 0;
     if (copy_end[i] == r || r >= R) a.copies[2 * i] = a.copies[2 * i + 1] = -1;
     t.lens[i] = new_len[i];
   }
-  if (rank == 0 && tid == 0 && t.status != nullptr) {
+  if (c.rank == 0 && tid == 0 && t.status != nullptr) {
     t.status[0] = R;
     t.status[1] = wanted - R;
     t.status[2] = total_free - R;
     t.status[3] = R;
   }
-  cluster_sync();  // no CTA leaves while another reads its free count
+  if (c.ranks > 1) cluster_sync();  // no CTA leaves while another reads its free count
 }
 
 // The page copies of a reorder: 16-byte pieces of the lens % page_size tokens
@@ -432,74 +471,71 @@ __device__ __forceinline__ void store8(__nv_fp8_e4m3 *p, const float (&x)[8]) {
   *reinterpret_cast<uint2 *>(p) = o;
 }
 
-// One thread per 8 elements (4 rotary pairs) of a q, k or v head: in fp32,
-// rounded once where it is stored. Bound by memory: every element is read
-// and written once, the rotary row of a token comes from L1 for all heads
-// but the first.
+// One thread per 8 elements (4 rotary pairs) of a q, k or v head of a token,
+// in fp32, rounded once where it is stored. Bound by memory: every element
+// is read and written once; a token's slot, position and rotary row are read
+// by its block (one or a few) and served from L1 to all its heads.
+constexpr int kAppendThreads = 256;
 template <typename In, typename Out, typename Cache>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_launch_dependents();
+  const unsigned eighths = (unsigned)a.dim >> 3;
+  const unsigned q_units = a.heads * eighths, kv_units = a.kv_heads * eighths;
+  unsigned u = blockIdx.y * kAppendThreads + threadIdx.x;
+  if (u >= q_units + 2 * kv_units) return;
+  const int part = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;
+  u -= part == 0 ? 0 : part == 1 ? q_units : q_units + kv_units;
+  const int head = (int)(u / eighths), d = 8 * (int)(u % eighths), tok = blockIdx.x;
+  const In *src = part == 0 ? static_cast<const In *>(a.q) + tok * a.q_ld
+                : part == 1 ? static_cast<const In *>(a.k) + tok * a.k_ld
+                            : static_cast<const In *>(a.v) + tok * a.v_ld;
   pdl_wait();
-  const int eighths = a.dim >> 3;
-  const int q_units = a.q != nullptr ? a.heads * eighths : 0, kv_units = a.kv_heads * eighths;
-  const int units = q_units + 2 * kv_units;
-  const long long total = (long long)a.tokens * units;
-  for (long long w = (long long)blockIdx.x * blockDim.x + threadIdx.x; w < total; w += (long long)gridDim.x * blockDim.x) {
-    const int tok = (int)(w / units);
-    int u = (int)(w % units);
-    const long long slot = a.slots[tok];
-    bool live = slot >= 0;
-    if (live && slot >= a.slot_end) {
-      report_timeout(&g_paged_status, kSiteSlot);
+  float x[8];
+  load8(src + head * a.dim + d, x);  // on its way while the slot and position are looked up
+  const long long slot = a.slots[tok];
+  bool live = slot >= 0;
+  if (live && slot >= a.slot_end) {
+    report_timeout(&g_paged_status, kSiteSlot);
+    live = false;
+  }
+  int pos = 0;
+  if (live && a.rope != nullptr) {
+    pos = a.pos[tok];
+    if (pos < 0 || pos >= a.rope_len) {
+      report_timeout(&g_paged_status, kSitePos);
       live = false;
     }
-    int pos = 0;
-    if (live && a.rope != nullptr) {
-      pos = a.pos[tok];
-      if (pos < 0 || pos >= a.rope_len) {
-        report_timeout(&g_paged_status, kSitePos);
-        live = false;
-      }
-    }
-    const int part = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;
-    u -= part == 0 ? 0 : part == 1 ? q_units : q_units + kv_units;
-    const int head = u / eighths, d = 8 * (u % eighths);
-    if (!live) {
-      if (part == 0) {
-        const float zero[8] = {};
-        store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, zero);
-      }
-      continue;
-    }
-    const In *src = part == 0 ? static_cast<const In *>(a.q) + tok * a.q_ld
-                  : part == 1 ? static_cast<const In *>(a.k) + tok * a.k_ld
-                              : static_cast<const In *>(a.v) + tok * a.v_ld;
-    float x[8];
-    load8(src + head * a.dim + d, x);
-    if (part < 2 && a.rope != nullptr) {
-      const float4 *cs = reinterpret_cast<const float4 *>(a.rope + (long long)pos * a.dim + d);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {  // two pairs per 16 bytes of (cos, sin)
-        const float4 c = __ldg(cs + i);
-        const float x0 = x[4 * i], x1 = x[4 * i + 1], x2 = x[4 * i + 2], x3 = x[4 * i + 3];
-        x[4 * i] = x0 * c.x - x1 * c.y, x[4 * i + 1] = x0 * c.y + x1 * c.x;
-        x[4 * i + 2] = x2 * c.z - x3 * c.w, x[4 * i + 3] = x2 * c.w + x3 * c.z;
-      }
-    }
-    if (part == 0) {
-      store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, x);
-      continue;
-    }
-    const float *scale = part == 1 ? a.k_scale : a.v_scale;
-    if (scale != nullptr) {
-      const float s = __ldg(scale + head);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] / s;
-    }
-    Cache *base = reinterpret_cast<Cache *>(part == 1 ? a.kc : a.vc);
-    store8(base + (slot >> a.shift) * a.page_stride + head * a.head_stride +
-               (slot & ((1ll << a.shift) - 1)) * a.token_stride + d, x);
   }
+  if (!live) {
+    if (part == 0) {
+      const float zero[8] = {};
+      store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, zero);
+    }
+    return;
+  }
+  if (part < 2 && a.rope != nullptr) {
+    const float4 *cs = reinterpret_cast<const float4 *>(a.rope + (long long)pos * a.dim + d);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // two pairs per 16 bytes of (cos, sin)
+      const float4 c = __ldg(cs + i);
+      const float x0 = x[4 * i], x1 = x[4 * i + 1], x2 = x[4 * i + 2], x3 = x[4 * i + 3];
+      x[4 * i] = x0 * c.x - x1 * c.y, x[4 * i + 1] = x0 * c.y + x1 * c.x;
+      x[4 * i + 2] = x2 * c.z - x3 * c.w, x[4 * i + 3] = x2 * c.w + x3 * c.z;
+    }
+  }
+  if (part == 0) {
+    store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, x);
+    return;
+  }
+  const float *scale = part == 1 ? a.k_scale : a.v_scale;
+  if (scale != nullptr) {
+    const float s = __ldg(scale + head);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] / s;
+  }
+  Cache *base = reinterpret_cast<Cache *>(part == 1 ? a.kc : a.vc);
+  store8(base + (slot >> a.shift) * a.page_stride + head * a.head_stride +
+             (slot & ((1ll << a.shift) - 1)) * a.token_stride + d, x);
 }
 
 // Launches one cluster of `ranks` CTAs (a table kernel).
@@ -522,13 +558,13 @@ int launch_tables(void (*kernel)(Args), const Args &a, int ranks, size_t smem, c
   return e == cudaSuccess ? CE_OK : cuda_error(e, what);
 }
 
-// Dynamic shared memory of a table kernel: three words per row, and the free
-// map of a CTA's share of the pages.
+// Dynamic shared memory of a table kernel: four words per row, and the free
+// map and its sums of a CTA's share of the pages.
 size_t table_smem(const ce_page_table *t, int ranks) {
   const int words = ((t->pages + ranks - 1) / ranks + 31) / 32;
-  return 12ull * t->seqs + 4ull * words;
+  return 16ull * t->seqs + 8ull * words;
 }
-constexpr size_t kTableSmemMax = 12ull * kMaxRows + kMaxPages / 8 / 8 + 128;  // a cluster of 8
+constexpr size_t kTableSmemMax = 16ull * kMaxRows + kMaxPages / 8 / 4 + 128;  // a cluster of 8
 static_assert(kTableSmemMax <= 224 * 1024, "a table kernel's shared memory");
 
 // CTAs of a table kernel.
@@ -565,10 +601,10 @@ Tables tables_of(const ce_page_table *to, const ce_page_table *from, int32_t *st
 template <typename In, typename Out>
 int launch_append(int cache_type, const AppendArgs &a, dim3 grid, cudaStream_t s) {
   if (cache_type == CE_TYPE_BF16)
-    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, dim3(256), 0, s, true, "append_kernel", a);
+    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
   if (cache_type == CE_TYPE_F16)
-    return launch_kernel(append_kernel<In, Out, __half>, grid, dim3(256), 0, s, true, "append_kernel", a);
-  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, dim3(256), 0, s, true, "append_kernel", a);
+    return launch_kernel(append_kernel<In, Out, __half>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
+  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
 }
 
 template <typename In>
@@ -717,8 +753,9 @@ int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out, int q_out_typ
   a.slot_end = (long long)kv->pages * kv->page_size;
   a.tokens = tokens, a.heads = q != nullptr ? heads : 0, a.kv_heads = kv->kv_heads, a.dim = kv->head_dim;
   a.shift = log2_of(kv->page_size), a.rope_len = rope_len;
-  const long long units = (long long)tokens * (a.heads + 2 * a.kv_heads) * (a.dim / 8);
-  const dim3 grid((unsigned)std::min<long long>((units + 255) / 256, 8ll * sm_count()));
+  const long long units = (a.heads + 2ll * a.kv_heads) * (a.dim / 8);  // of a token
+  CE_REQUIRE(units <= 65535ll * kAppendThreads, "too many heads (%d + 2 x %d)", heads, kv->kv_heads);
+  const dim3 grid((unsigned)tokens, (unsigned)((units + kAppendThreads - 1) / kAppendThreads));
   const cudaStream_t s = (cudaStream_t)stream;
   if (in_type == CE_TYPE_F32) return launch_append<float>(q_out_type, kv->type, a, grid, s);
   if (in_type == CE_TYPE_F16) return launch_append<__half>(q_out_type, kv->type, a, grid, s);

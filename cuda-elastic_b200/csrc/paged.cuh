@@ -12,7 +12,7 @@
 namespace ce {
 namespace paged {
 
-constexpr int kMaxRows = 16384;      // rows of a block table
+constexpr int kMaxRows = 8192;       // rows of a block table
 constexpr int kMaxPages = 1 << 20;   // pages of a pool
 constexpr int kMaxPage = 1024;       // tokens of a page
 

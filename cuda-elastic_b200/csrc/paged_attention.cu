@@ -6,7 +6,7 @@
 // side. Every key and value is used once, G x 4 flops per element pair, so
 // the bound is the memory that K and V come from. The design serves that:
 //
-//   * The unit of work is 16 keys of one (request, kv head). All units of the
+//   * The unit of work is 16 or 32 keys of one (request, kv head). All units of the
 //     batch form one line, in which every warp of the grid (one CTA per SM)
 //     takes an equal contiguous share, whatever the lengths: a long request
 //     is split over many SMs, many short ones share a warp, and no SM ends
@@ -49,7 +49,9 @@ namespace {
 __device__ DeviceStatus g_attention_status;  // bad pages and lengths
 __device__ DeviceStatus g_attention_wait;    // a wait that gave up (it ends the waits of others, too)
 
-constexpr int kUnit = 16;              // keys of a unit
+// Keys of a unit: 16 where a row of a head takes more than 128 bytes, else 32,
+// so that a unit is 8 KB of keys and values at the common head sizes.
+constexpr int unit_of(int dim, int item) { return dim > 64 && item == 2 ? 16 : 32; }
 constexpr int kMinShare = 4;           // units of a CTA at least
 constexpr int kMaxSplitHeads = 16;     // query heads of one pass over the keys
 constexpr int kMaxGrid = 1024;         // CTAs the workspace's counters are laid out for
@@ -78,12 +80,14 @@ struct Shape {
   static constexpr int kKeyChunks = D * kItem / 64;           // 16-byte pieces of a key row per lane
   static constexpr int kValBytes = D * kItem / 8 >= 16 ? 16 : 8;
   static constexpr int kValChunks = D * kItem / 8 / kValBytes;  // pieces of a value row per lane
-  static constexpr int kTiles = D * kItem > 128 ? 2 : 1;        // 128-byte wide tiles of 16 rows
+  static constexpr int kTiles = D * kItem > 128 ? 2 : 1;        // 128-byte wide tiles of kUnit rows
+  static constexpr int kUnit = unit_of(D, kItem);
+  static constexpr int kHalves = kUnit / 16;                    // products of 16 keys
   static constexpr int kTileBytes = 128 * kUnit;
   static constexpr int kStageBytes = 2 * kTiles * kTileBytes;   // keys, then values
-  static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : 12)
-                                        : (kTiles == 2 ? 6 : D == 128 ? 8 : 12);
-  static constexpr int kStages = kTiles == 2 || (D == 64) != (NT == 1) ? 3 : 4;
+  static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : D == 128 ? 10 : 12)
+                                        : (kTiles == 2 ? 6 : D == 128 ? 8 : 10);
+  static constexpr int kStages = kTiles == 2 ? 3 : 2;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPart = kHeads * (D + 2);  // floats of one (O, max, sum) part
   static constexpr int kVals = D / 8;             // dimensions of a value row per lane
@@ -177,9 +181,11 @@ __device__ __forceinline__ int row_len(const AttnArgs &a, int b) {
   return len;
 }
 
-__device__ __forceinline__ int slots_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit + 1 : 0; }
+template <int UNIT>
+__device__ __forceinline__ int slots_of(int len) { return len > 0 ? (len + UNIT - 1) / UNIT + 1 : 0; }
 
 // A place on the line of units. Requests of length 0 have none.
+template <int UNIT>
 struct Cursor {
   int row, kh, tile, k, len, units;  // request, kv head, pass over its query heads, unit; the request's length and units
   __device__ __forceinline__ void next_row(const AttnArgs &a) {
@@ -190,7 +196,7 @@ struct Cursor {
       }
       len = row_len(a, row);
     } while (len == 0);
-    units = (len + kUnit - 1) / kUnit;
+    units = (len + UNIT - 1) / UNIT;
   }
   __device__ __forceinline__ void step(const AttnArgs &a) {
     if (++k < units) return;
@@ -242,7 +248,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
                  const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, NT, F8>;
   constexpr bool BF = !F8 && std::is_same<Io, __nv_bfloat16>::value;  // type of the products
-  constexpr int W = S::kWarps, ST = S::kStages;
+  constexpr int W = S::kWarps, ST = S::kStages, kUnit = S::kUnit, H = S::kHalves;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[W][ST];
   // units of the requests up to each thread's last, per kv head and pass; in
@@ -280,13 +286,13 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
 #pragma unroll
     for (int i = 0; i < kRowsPerLane; ++i) lens[i] = i < per && first_row + i < a.seqs ? row_len(a, first_row + i) : -1;
 #pragma unroll
-    for (int i = 0; i < kRowsPerLane; ++i) mine += slots_of(lens[i]), empty = empty || lens[i] == 0;
+    for (int i = 0; i < kRowsPerLane; ++i) mine += slots_of<kUnit>(lens[i]), empty = empty || lens[i] == 0;
     mine = warp_inclusive_sum(mine);
     sum = __shfl_sync(0xffffffffu, mine, 31);
   } else {
     for (int b = first_row; b < min(a.seqs, first_row + per); ++b) {
       const int len = row_len(a, b);
-      mine += slots_of(len);
+      mine += slots_of<kUnit>(len);
       empty = empty || len == 0;
     }
     ends[tid] = block_inclusive_sum(mine, scratch, sum);
@@ -315,7 +321,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   float *const part1 = reinterpret_cast<float *>(smem + (size_t)warp * S::kRing);
 
   // ---- where the share begins
-  Cursor at = {0, 0, 0, 0, 0, 1};
+  Cursor<kUnit> at = {0, 0, 0, 0, 0, 1};
   if (count > 0) {
     uint32_t before;
     if (few) {
@@ -323,11 +329,11 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       const int lo = beyond ? __ffs(beyond) - 1 : 31;
       int row = first_row, len = 0, sums = mine;
 #pragma unroll
-      for (int i = 0; i < kRowsPerLane; ++i) sums -= slots_of(lens[i]);  // before this lane's rows
+      for (int i = 0; i < kRowsPerLane; ++i) sums -= slots_of<kUnit>(lens[i]);  // before this lane's rows
       bool found = false;
 #pragma unroll
       for (int i = 0; i < kRowsPerLane; ++i) {
-        const int n = slots_of(lens[i]);
+        const int n = slots_of<kUnit>(lens[i]);
         if (!found && n > 0) {
           if ((uint64_t)(uint32_t)(sums + n) * passes > slot) found = true, row = first_row + i, len = lens[i];
           else sums += n;
@@ -345,8 +351,8 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       const int last = min(a.seqs, (lo + 1) * per) - 1;
       for (at.row = lo * per;; ++at.row) {
         at.len = row_len(a, at.row);
-        if (at.row >= last || (uint64_t)(before + slots_of(at.len)) * passes > slot) break;
-        before += slots_of(at.len);
+        if (at.row >= last || (uint64_t)(before + slots_of<kUnit>(at.len)) * passes > slot) break;
+        before += slots_of<kUnit>(at.len);
       }
     }
     at.units = max(1, (at.len + kUnit - 1) / kUnit);
@@ -361,8 +367,8 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   if (count > 0) {
     // Copies run ahead of the products by ST - 1 units, page lookups by one
     // more, so that no copy waits for its page id. A unit is one box of a
-    // page, or 16 / page_size boxes of as many pages, one per lane.
-    Cursor look = at;  // the unit whose pages are looked up next
+    // page, or kUnit / page_size boxes of as many pages, one per lane.
+    Cursor<kUnit> look = at;  // the unit whose pages are looked up next
     const int32_t *pages = a.table + (size_t)look.row * a.max_pages;
     const int rows = min(kUnit, 1 << a.shift), mask = (1 << a.shift) - 1, sub = lane * rows;  // of this lane's box
     int page = 0, token = 0, head = 0, left = 0;  // of the looked-up unit; left: live keys (less than 1: no unit)
@@ -412,7 +418,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     // of the keys' pieces. With one tile of heads it is fetched a request part
     // ahead (two tiles leave no registers for that).
     uint4 raw[NT][D / 32];
-    auto load_q = [&](const Cursor &c) {
+    auto load_q = [&](const Cursor<kUnit> &c) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int h = c.tile * S::kHeads + 8 * nt + g;
@@ -491,7 +497,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
           for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
         }
         if (NT == 1 && count - (at.units - at.k) > 1) {
-          Cursor next = at;
+          Cursor<kUnit> next = at;
           next.k = next.units - 1;
           next.step(a);
           load_q(next);
@@ -503,54 +509,74 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       const uint8_t *const st = ring_ptr + (uint32_t)stage * S::kStageBytes;
       const bool tail = at.k + 1 == at.units;     // may have keys past the length
       const int n_live = at.len - at.k * kUnit;
-      // ---- all of the unit into registers: the loads of the values are under way during the scores
-      uint4 kx[S::kKeyChunks][2];
-#pragma unroll
-      for (int c = 0; c < S::kKeyChunks; ++c)
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          kx[c][r] = *reinterpret_cast<const uint4 *>(st + key_at[c & 1] + (c >> 1) * S::kTileBytes + r * (8 * 128));
+      // The values of the first 16 keys are on their way from shared memory
+      // during the scores.
       constexpr int kWords = S::kValBytes * S::kValChunks / 4;
       uint32_t x[4][kWords];
+      auto load_values = [&](int hf) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < S::kValChunks; ++c) {
-          const uint8_t *from = st + val_at[r & 1] + c * S::kTileBytes + (r >> 1) * (8 * 128);
-          if constexpr (S::kValBytes == 16) {
-            const uint4 y = *reinterpret_cast<const uint4 *>(from);
-            x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
-          } else {
-            const uint2 y = *reinterpret_cast<const uint2 *>(from);
-            x[r][0] = y.x, x[r][1] = y.y;
+          for (int c = 0; c < S::kValChunks; ++c) {
+            const uint8_t *from = st + val_at[r & 1] + c * S::kTileBytes + (2 * hf + (r >> 1)) * (8 * 128);
+            if constexpr (S::kValBytes == 16) {
+              const uint4 y = *reinterpret_cast<const uint4 *>(from);
+              x[r][4 * c] = y.x, x[r][4 * c + 1] = y.y, x[r][4 * c + 2] = y.z, x[r][4 * c + 3] = y.w;
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2 *>(from);
+              x[r][0] = y.x, x[r][1] = y.y;
+            }
           }
+        if (tail) {  // weights of 0 must meet values of 0, whatever the cache holds there
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((r & 1 ? po : pe) + 8 * (r >> 1) + 16 * hf >= n_live)
+#pragma unroll
+              for (int w = 0; w < kWords; ++w) x[r][w] = 0;
         }
-      // ---- scores: 16 keys x 8 NT heads, in sums of their own per 16 bytes of keys
-      constexpr int kSums = 2 * S::kKeyChunks > 4 ? 4 : 2 * S::kKeyChunks;
-      float part_s[NT][kSums][4], s[NT][4];
+      };
+      // ---- scores: 16 keys x 8 NT heads per half, in sums of their own so that no product waits long
+      constexpr int kSums = 2 * S::kKeyChunks * H > 4 ? 4 / H : 2;
+      float s[NT][H][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int hf = 0; hf < H; ++hf) {
+        uint4 kx[S::kKeyChunks][2];
 #pragma unroll
-        for (int y = 0; y < kSums; ++y)
+        for (int c = 0; c < S::kKeyChunks; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) part_s[nt][y][i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < S::kKeyChunks; ++c) {
-        const uint32_t xw[4] = {kx[c][0].x, kx[c][0].y, kx[c][0].z, kx[c][0].w};
-        const uint32_t yw[4] = {kx[c][1].x, kx[c][1].y, kx[c][1].z, kx[c][1].w};
+          for (int r = 0; r < 2; ++r)
+            kx[c][r] = *reinterpret_cast<const uint4 *>(st + key_at[c & 1] + (c >> 1) * S::kTileBytes +
+                                                        (2 * hf + r) * (8 * 128));
+        if (hf == 0) load_values(0);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if constexpr (F8) {
+          float sums[kSums][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t x0, x1, y0, y1;
-              e4m3_to_f16(xw[j], x0, x1);
-              e4m3_to_f16(yw[j], y0, y1);
-              mma<BF>(part_s[nt][(4 * c + j) % kSums], x0, y0, x1, y1, q[nt][8 * c + 2 * j], q[nt][8 * c + 2 * j + 1]);
+          for (int y = 0; y < kSums; ++y)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[y][i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < S::kKeyChunks; ++c) {
+            const uint32_t xw[4] = {kx[c][0].x, kx[c][0].y, kx[c][0].z, kx[c][0].w};
+            const uint32_t yw[4] = {kx[c][1].x, kx[c][1].y, kx[c][1].z, kx[c][1].w};
+            if constexpr (F8) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint32_t x0, x1, y0, y1;
+                e4m3_to_f16(xw[j], x0, x1);
+                e4m3_to_f16(yw[j], y0, y1);
+                mma<BF>(sums[(4 * c + j) % kSums], x0, y0, x1, y1, q[nt][8 * c + 2 * j], q[nt][8 * c + 2 * j + 1]);
+              }
+            } else {
+              mma<BF>(sums[2 * c % kSums], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
+              mma<BF>(sums[(2 * c + 1) % kSums], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
             }
-          } else {
-            mma<BF>(part_s[nt][2 * c % kSums], xw[0], yw[0], xw[1], yw[1], q[nt][4 * c], q[nt][4 * c + 1]);
-            mma<BF>(part_s[nt][(2 * c + 1) % kSums], xw[2], yw[2], xw[3], yw[3], q[nt][4 * c + 2], q[nt][4 * c + 3]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float y = sums[0][i] + sums[1][i];
+            if constexpr (kSums == 4) y += sums[2][i] + sums[3][i];
+            s[nt][hf][i] = y * cs[nt][i & 1];
           }
         }
       }
@@ -558,29 +584,31 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       // The maximum that the weights refer to moves only when a score passes
       // it by more than 8 (2^8 is far inside both 16-bit types' range), so
       // that most units need a vote instead of a reduction and a rescaling.
-      uint32_t big[NT][2], rest[NT][2];
+      if (tail) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int hf = 0; hf < H; ++hf)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (pi + 8 * (i >> 1) + 16 * hf >= n_live) s[nt][hf][i] = -INFINITY;
+      }
       bool grew = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y = part_s[nt][0][i] + part_s[nt][1][i];
-          if constexpr (kSums == 4) y += part_s[nt][2][i] + part_s[nt][3][i];
-          s[nt][i] = y * cs[nt][i & 1];
+        for (int j = 0; j < 2; ++j) {
+          float top = fmaxf(s[nt][0][j], s[nt][0][j + 2]);
+          if constexpr (H == 2) top = fmaxf(top, fmaxf(s[nt][1][j], s[nt][1][j + 2]));
+          grew = grew || top > m[nt][j] + 8.f;
         }
-        if (tail) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] = pi + 8 * (i >> 1) < n_live ? s[nt][i] : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) grew = grew || s[nt][i] > m[nt][i & 1] + 8.f;
-      }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(s[nt][j], s[nt][j + 2]);
+            float top = fmaxf(s[nt][0][j], s[nt][0][j + 2]);
+            if constexpr (H == 2) top = fmaxf(top, fmaxf(s[nt][1][j], s[nt][1][j + 2]));
 #pragma unroll
             for (int y = 4; y < 32; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
             const float mn = fmaxf(m[nt][j], top);
@@ -591,51 +619,52 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
             for (int i = 0; i < S::kVals / 2; ++i) o[nt][i][j] *= f, o[nt][i][j + 2] *= f;
           }
       }
+      uint32_t big[NT][H][2], rest[NT][H][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p[4], base[2];
+        float base[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) base[j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[nt][i] - base[i & 1]);
-        l[nt][0] += p[0] + p[2];
-        l[nt][1] += p[1] + p[3];
-        split16<BF>(p[0], p[1], big[nt][0], rest[nt][0]);
-        split16<BF>(p[2], p[3], big[nt][1], rest[nt][1]);
+        for (int hf = 0; hf < H; ++hf) {
+          float p[4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) big[nt][r] = transpose8x8(big[nt][r]), rest[nt][r] = transpose8x8(rest[nt][r]);
+          for (int i = 0; i < 4; ++i) p[i] = exp2_approx(s[nt][hf][i] - base[i & 1]);
+          l[nt][0] += p[0] + p[2];
+          l[nt][1] += p[1] + p[3];
+          split16<BF>(p[0], p[1], big[nt][hf][0], rest[nt][hf][0]);
+          split16<BF>(p[2], p[3], big[nt][hf][1], rest[nt][hf][1]);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            big[nt][hf][r] = transpose8x8(big[nt][hf][r]), rest[nt][hf][r] = transpose8x8(rest[nt][hf][r]);
+        }
       }
       // ---- values: rows of V^T are this lane's kVals dimensions, in pairs (i, i + kVals / 2)
-      if (tail) {  // weights of 0 must meet values of 0, whatever the cache holds there
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if ((r & 1 ? po : pe) + 8 * (r >> 1) >= n_live)
+      for (int hf = 0; hf < H; ++hf) {
+        if (hf > 0) load_values(hf);
+        constexpr int kPer = 4 / S::kItem;  // elements of a word
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) x[r][w] = 0;
-      }
-      auto product = [&](int i, const uint32_t (&v)[4]) {  // v: (row g | g + 8) x (keys 2t, 2t + 1 | 2t + 8, 2t + 9)
+        for (int i = 0; i < S::kVals / 2; i += 2) {
+          uint32_t v[2][4];  // elements i and i + 1: (row g | g + 8) x (keys 2t, 2t + 1 | 2t + 8, 2t + 9)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], big[nt][0], big[nt][1]);
-          mma<BF>(o[nt][i], v[0], v[1], v[2], v[3], rest[nt][0], rest[nt][1]);
-        }
-      };
-      constexpr int kPer = 4 / S::kItem;  // elements of a word
-#pragma unroll
-      for (int i = 0; i < S::kVals / 2; i += 2) {
-        uint32_t v[2][4];  // elements i and i + 1
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int e = i + (r & 1) * (S::kVals / 2), w = e / kPer, pr = 2 * (r >> 1);
-          if constexpr (F8) {
-            e4m3_to_f16(__byte_perm(x[pr][w], x[pr + 1][w], e % kPer ? 0x7362 : 0x5140), v[0][r], v[1][r]);
-          } else {
-            v[0][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x5410);
-            v[1][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x7632);
+          for (int r = 0; r < 4; ++r) {
+            const int e = i + (r & 1) * (S::kVals / 2), w = e / kPer, pr = 2 * (r >> 1);
+            if constexpr (F8) {
+              e4m3_to_f16(__byte_perm(x[pr][w], x[pr + 1][w], e % kPer ? 0x7362 : 0x5140), v[0][r], v[1][r]);
+            } else {
+              v[0][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x5410);
+              v[1][r] = __byte_perm(x[pr][w], x[pr + 1][w], 0x7632);
+            }
           }
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma<BF>(o[nt][i + u], v[u][0], v[u][1], v[u][2], v[u][3], big[nt][hf][0], big[nt][hf][1]);
+              mma<BF>(o[nt][i + u], v[u][0], v[u][1], v[u][2], v[u][3], rest[nt][hf][0], rest[nt][hf][1]);
+            }
         }
-        product(i, v[0]);
-        product(i + 1, v[1]);
       }
       if (++stage == ST) stage = 0, parity ^= 1u;
 
@@ -876,8 +905,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // The map of one layer of a pool: [pages][heads][tokens][head_dim] with the
-// pool's strides; boxes of 128 bytes x min(16, page_size) tokens.
-int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer) {
+// pool's strides; boxes of 128 bytes x min(unit, page_size) tokens.
+int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer, int unit_keys) {
   const auto fn = encode_fn();
   if (fn == nullptr) return set_error(CE_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const int b = type_bytes(kv->type);
@@ -887,7 +916,7 @@ int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer
   auto stride = [&](int64_t elements, int size) { return size > 1 ? (cuuint64_t)elements * b : (cuuint64_t)16; };
   const cuuint64_t strides[3] = {stride(kv->token_stride, kv->page_size), stride(kv->head_stride, kv->kv_heads),
                                  stride(kv->page_stride, kv->pages)};
-  const cuuint32_t box[4] = {(cuuint32_t)(128 / b), (cuuint32_t)std::min(kUnit, kv->page_size), 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / b), (cuuint32_t)std::min(unit_keys, kv->page_size), 1, 1};
   const cuuint32_t unit[4] = {1, 1, 1, 1};
   char *base = static_cast<char *>(pool) + (long long)layer * kv->layer_stride * b;
   const CUresult r = fn(map, b == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims,
@@ -957,8 +986,9 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
              "the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
   AttnArgs a = {};
   CUtensorMap maps[2];
-  rc = make_page_map(&maps[0], kv, kv->k_dev, layer);
-  if (rc == CE_OK) rc = make_page_map(&maps[1], kv, kv->v_dev, layer);
+  const int unit = unit_of(kv->head_dim, type_bytes(kv->type));
+  rc = make_page_map(&maps[0], kv, kv->k_dev, layer, unit);
+  if (rc == CE_OK) rc = make_page_map(&maps[1], kv, kv->v_dev, layer, unit);
   if (rc != CE_OK) return rc;
   a.q = q, a.out = out, a.lse = lse;
   a.k_scale = kv->k_scale_dev, a.v_scale = kv->v_scale_dev;
@@ -969,7 +999,7 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
   a.group = heads / kv->kv_heads;
   a.tiles = a.group <= 8 ? 1 : (a.group + kMaxSplitHeads - 1) / kMaxSplitHeads;
   a.scale = scale;
-  const int64_t slots = (int64_t)pt->max_pages * pt->page_size / kUnit + 2;  // slots of a full row at most
+  const int64_t slots = (int64_t)pt->max_pages * pt->page_size / unit + 2;  // slots of a full row at most
   CE_REQUIRE(pt->seqs * slots < (1ll << 31) && (double)pt->seqs * slots * kv->kv_heads * a.tiles < 4294967296.0 - kMaxGrid,
              "seqs x max_pages x page_size x kv_heads is too large (%d x %d x %d x %d)", pt->seqs, pt->max_pages,
              pt->page_size, kv->kv_heads);

@@ -865,7 +865,7 @@ typedef struct ce_paged_kv {
 /* Block tables: row i holds the pages of request i in order, of which the
  * first ceil(lens[i] / page_size) count; what stands behind them means
  * nothing. refs[p] counts the rows that hold page p: 0 is a free page, and a
- * caller that adds 1 of its own keeps a page out of reuse. At most 16384
+ * caller that adds 1 of its own keeps a page out of reuse. At most 8192
  * rows and 2^20 pages. */
 typedef struct ce_page_table {
   int32_t *table_dev; /* [seqs][max_pages] */

@@ -30,7 +30,7 @@ def refused(ce, rc, word):
 
 
 BAD_TABLES = [(dict(table=None), "null buffer"), (dict(lens=None), "null buffer"), (dict(refs=None), "null buffer"),
-              (dict(seqs=0), "seqs"), (dict(seqs=16385), "seqs"), (dict(max_pages=0), "max_pages"),
+              (dict(seqs=0), "seqs"), (dict(seqs=8193), "seqs"), (dict(max_pages=0), "max_pages"),
               (dict(pages=0), "pages"), (dict(pages=(1 << 20) + 1), "pages"), (dict(page_size=24), "power of two"),
               (dict(page_size=0), "power of two"), (dict(page_size=2048), "power of two"),
               (dict(max_pages=1 << 28), "2^31")]
