@@ -130,6 +130,34 @@ struct FreeMap {
   }
 };
 
+// By one warp, four entries of a lane at a time so that their latencies overlap:
+// the pages of a row change their count of holders, or a row is copied.
+__device__ __forceinline__ void change_refs(const Tables &t, const FreeMap &map, const int32_t *row, int n, int delta) {
+  for (int j = threadIdx.x & 31; j < n; j += 128) {
+    int page[4], now[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) page[u] = j + 32 * u < n ? row[j + 32 * u] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool live = j + 32 * u < n && page_ok(t, page[u]);
+      now[u] = live ? atomicAdd(t.refs + page[u], delta) + delta : 1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (now[u] == 0) map.set(page[u]);
+  }
+}
+__device__ __forceinline__ void copy_row(int32_t *to, const int32_t *from, int n) {
+  for (int j = threadIdx.x & 31; j < n; j += 128) {
+    int page[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) page[u] = j + 32 * u < n ? from[j + 32 * u] : 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j + 32 * u < n) to[j + 32 * u] = page[u];
+  }
+}
+
 // Free pages of the CTAs before this one, and of all.
 __device__ __forceinline__ void free_before(int *count, Cluster c, int &before, int &total) {
   before = total = 0;
@@ -140,6 +168,21 @@ __device__ __forceinline__ void free_before(int *count, Cluster c, int &before, 
     before += r < c.rank ? v : 0;
     total += v;
   }
+}
+
+// Inclusive sums over the block of two values per thread.
+struct Pair {
+  long long a, b;
+};
+__device__ __forceinline__ Pair block_inclusive_sums(Pair v, Pair *scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v.a = warp_inclusive_sum(v.a), v.b = warp_inclusive_sum(v.b);
+  if (lane == 31) scratch[warp] = v;
+  __syncthreads();
+  Pair e = lane < warps ? scratch[lane] : Pair{0, 0};
+  e.a = warp_inclusive_sum(e.a), e.b = warp_inclusive_sum(e.b);
+  const long long a = __shfl_sync(0xffffffffu, e.a, max(0, warp - 1)), b = __shfl_sync(0xffffffffu, e.b, max(0, warp - 1));
+  return {v.a + (warp > 0 ? a : 0), v.b + (warp > 0 ? b : 0)};
 }
 
 // ---------------------------------------------------------------------------
@@ -166,7 +209,7 @@ struct ResizeArgs {
 //   5. slots and positions, token by token, by the rows' prefix sums.
 __global__ void __launch_bounds__(kTableThreads) resize_kernel(const __grid_constant__ ResizeArgs a) {
   extern __shared__ int smem[];
-  __shared__ long long scratch8[32];
+  __shared__ Pair scratch16[32];
   __shared__ int scratch4[32];
   __shared__ int s_free, s_pages, s_tokens, s_refused;
   const Tables &t = a.t;
@@ -195,10 +238,8 @@ __global__ void __launch_bounds__(kTableThreads) resize_kernel(const __grid_cons
     for (int i = c.rank * (int)(blockDim.x >> 5) + (tid >> 5); i < n; i += warps) {
       const int have = pages_of(old_len[i], t.shift), want = pages_of(new_len[i], t.shift);
       const int32_t *row = t.table_in + (size_t)i * t.max_pages;
-      for (int j = want + lane; j < have; j += 32)
-        if (page_ok(t, row[j]) && atomicAdd(t.refs + row[j], -1) == 1) map.set(row[j]);
-      if (t.table != t.table_in)
-        for (int j = lane; j < min(want, have); j += 32) t.table[(size_t)i * t.max_pages + j] = row[j];
+      change_refs(t, map, row + want, have - want, -1);
+      if (t.table != t.table_in) copy_row(t.table + (size_t)i * t.max_pages, row, min(want, have));
     }
   }
   sync_all(c);
@@ -223,9 +264,8 @@ __global__ void __launch_bounds__(kTableThreads) resize_kernel(const __grid_cons
   }
   const int free = map.count(scratch4);
   if (tid == 0) s_free = free;
-  long long all;
-  const long long need0 = block_inclusive_sum(need_sum, scratch8, all) - need_sum;
-  const long long tok0 = block_inclusive_sum(tok_sum, scratch8, all) - tok_sum;
+  const Pair ends = block_inclusive_sums(Pair{need_sum, tok_sum}, scratch16);
+  const long long need0 = ends.a - need_sum, tok0 = ends.b - tok_sum;
   sync_all(c);
   int before, total_free;
   free_before(&s_free, c, before, total_free);
@@ -250,17 +290,31 @@ __global__ void __launch_bounds__(kTableThreads) resize_kernel(const __grid_cons
   sync_all(c);
   // 5. (no CTA reads the old lengths any more)
   const int threads = c.ranks * (int)blockDim.x, first = c.rank * (int)blockDim.x + tid;
-  for (int j = first; j < a.capacity; j += threads) {
-    long long slot = -1;
-    int pos = -1;
-    if (j < T) {
-      const int i = first_above(tok_end, n, j);
-      pos = old_len[i] + j - (i ? tok_end[i - 1] : 0);
-      const int page = __ldcg(t.table + (size_t)i * t.max_pages + (pos >> t.shift));
-      slot = ((long long)page << t.shift) + (pos & mask);
+  // A warp takes 32 tokens, or 128 where there are more tokens than threads:
+  // mostly those of one request, whose row it then looks up once.
+  const int runs = a.capacity <= threads ? 1 : 4;
+  for (long long b = (long long)(first >> 5) * 32 * runs; b < a.capacity; b += (long long)threads * runs) {
+    const int base = (int)b, row = base < T ? first_above(tok_end, n, base) : 0;
+    const bool one = base < T && tok_end[row] >= min(T, base + 32 * runs);
+    int pos[4], page[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = base + 32 * u + lane;
+      pos[u] = -1, page[u] = 0;
+      if (u < runs && j < T) {
+        const int i = one ? row : first_above(tok_end, n, j);
+        pos[u] = old_len[i] + j - (i ? tok_end[i - 1] : 0);
+        page[u] = __ldcg(t.table + (size_t)i * t.max_pages + (pos[u] >> t.shift));
+      }
     }
-    a.slots[j] = slot;
-    a.pos[j] = pos;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = base + 32 * u + lane;
+      if (u < runs && j < a.capacity) {
+        a.slots[j] = pos[u] < 0 ? -1ll : ((long long)page[u] << t.shift) + (pos[u] & mask);
+        a.pos[j] = pos[u];
+      }
+    }
   }
   for (int i = first; i < n; i += threads) {
     const int start = i ? tok_end[i - 1] : 0, old = old_len[i], len = new_len[i];
@@ -304,7 +358,7 @@ __global__ void __launch_bounds__(kTableThreads) reorder_kernel(const __grid_con
   __shared__ int scratch4[32];
   __shared__ int s_free;
   const Tables &t = a.t;
-  const int n = t.n, K = a.beams, tid = threadIdx.x, lane = tid & 31, mask = (1 << t.shift) - 1;
+  const int n = t.n, K = a.beams, tid = threadIdx.x, mask = (1 << t.shift) - 1;
   const Cluster c = this_cluster();
   int *new_len = smem, *tail = smem + n, *copy_end = smem + 2 * n, *children = smem + 3 * n;
   const FreeMap map(reinterpret_cast<uint32_t *>(smem + 4 * n), t.pages, c);
@@ -336,11 +390,8 @@ __global__ void __launch_bounds__(kTableThreads) reorder_kernel(const __grid_con
     const int32_t *from = t.table_in + (size_t)(i - i % K + (held ? a.parents[i] : 0)) * t.max_pages;
     const int32_t *mine = t.table_in + (size_t)i * t.max_pages;
     const int have = delta != 0 ? pages_of(held_len(t, i), t.shift) : 0;
-    for (int j = lane; j < held; j += 32) t.table[(size_t)i * t.max_pages + j] = from[j];
-    for (int j = lane; j < have; j += 32) {
-      const int page = mine[j];
-      if (page_ok(t, page) && atomicAdd(t.refs + page, delta) + delta == 0) map.set(page);
-    }
+    copy_row(t.table + (size_t)i * t.max_pages, from, held);
+    change_refs(t, map, mine, have, delta);
   }
   sync_all(c);
   // 3.
@@ -391,31 +442,72 @@ __global__ void __launch_bounds__(kTableThreads) reorder_kernel(const __grid_con
   if (c.ranks > 1) cluster_sync();  // no CTA leaves while another reads its free count
 }
 
-// The page copies of a reorder: 16-byte pieces of the lens % page_size tokens
-// of every copied row, in all layers, K and V. Grid: (pieces, rows, layers).
+// The page copies of a reorder: 16-byte pieces of the len % page_size tokens
+// of every copied row, in all layers, K and V: read and written once. Each
+// CTA lists the rows that copy (the host does not know them), then takes
+// (row, layer) pairs in turn; blockIdx.y shares out the pieces of a pair
+// where pairs alone would not fill the GPU.
 struct CopyArgs {
   const int32_t *copies, *lens;
   char *k, *v;
   long long layer_stride, page_stride, head_stride, token_stride;  // bytes
-  int kv_heads, pieces, page_size;                                 // pieces: 16-byte pieces of a head's row
+  int rows, layers, kv_heads, pieces, page_size;                   // pieces: 16-byte pieces of a head's row
 };
+constexpr int kCopyThreads = 256;
 
-__global__ void __launch_bounds__(256) copy_pages_kernel(CopyArgs a) {
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {
+  __shared__ unsigned short list[kMaxRows];
+  __shared__ int scratch[32];
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.y;
-  const int src = a.copies[2 * row], dst = a.copies[2 * row + 1];
-  if (src < 0) return;
-  const int tokens = a.lens[row] & (a.page_size - 1);
-  const int total = tokens * a.kv_heads * a.pieces;
-  const long long layer = (long long)blockIdx.z * a.layer_stride;
-  for (int u = blockIdx.x * blockDim.x + threadIdx.x; u < total; u += gridDim.x * blockDim.x) {
-    const int piece = u % a.pieces, rest = u / a.pieces;
-    const long long at = layer + (rest / tokens) * a.head_stride + (rest % tokens) * a.token_stride + 16ll * piece;
-    const uint4 x = *reinterpret_cast<const uint4 *>(a.k + at + src * a.page_stride);
-    const uint4 y = *reinterpret_cast<const uint4 *>(a.v + at + src * a.page_stride);
-    *reinterpret_cast<uint4 *>(a.k + at + dst * a.page_stride) = x;
-    *reinterpret_cast<uint4 *>(a.v + at + dst * a.page_stride) = y;
+  int listed = 0;
+  uint32_t few = 0;  // up to 32 rows a warp lists by itself, in a word
+  if (a.rows <= 32) {
+    const int lane = threadIdx.x & 31;
+    few = __ballot_sync(0xffffffffu, lane < a.rows && a.copies[2 * lane] >= 0);
+    listed = __popc(few);
+  }
+  for (int r0 = 0; a.rows > 32 && r0 < a.rows; r0 += kCopyThreads) {
+    const int r = r0 + threadIdx.x;
+    const int copied = r < a.rows && a.copies[2 * r] >= 0;
+    int total;
+    const int at = listed + block_inclusive_sum(copied, scratch, total) - 1;
+    if (copied) list[at] = (unsigned short)r;
+    listed += total;
+  }
+  if (a.rows > 32) __syncthreads();
+  const int step = gridDim.y * kCopyThreads;
+  for (long long p = blockIdx.x; p < (long long)listed * a.layers; p += gridDim.x) {
+    const int at_row = (int)(p / a.layers), layer = (int)(p % a.layers);
+    int row;
+    if (a.rows <= 32) {
+      uint32_t rest = few;
+      for (int i = 0; i < at_row; ++i) rest &= rest - 1;
+      row = __ffs(rest) - 1;
+    } else {
+      row = list[at_row];
+    }
+    const int src = a.copies[2 * row], dst = a.copies[2 * row + 1], tokens = a.lens[row] & (a.page_size - 1);
+    const int total = tokens * a.kv_heads * a.pieces;
+    char *const k = a.k + layer * a.layer_stride, *const v = a.v + layer * a.layer_stride;
+    for (int u0 = blockIdx.y * kCopyThreads + threadIdx.x; u0 < total; u0 += 2 * step) {
+      uint4 x[2], y[2];
+      long long at[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const unsigned u = min(u0 + i * step, total - 1), rest = u / (unsigned)a.pieces;
+        at[i] = (rest / (unsigned)tokens) * a.head_stride + (rest % (unsigned)tokens) * a.token_stride +
+                16ll * (u % (unsigned)a.pieces);
+        x[i] = *reinterpret_cast<const uint4 *>(k + at[i] + src * a.page_stride);
+        y[i] = *reinterpret_cast<const uint4 *>(v + at[i] + src * a.page_stride);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (u0 + i * step < total) {
+          *reinterpret_cast<uint4 *>(k + at[i] + dst * a.page_stride) = x[i];
+          *reinterpret_cast<uint4 *>(v + at[i] + dst * a.page_stride) = y[i];
+        }
+    }
   }
 }
 
@@ -567,8 +659,17 @@ size_t table_smem(const ce_page_table *t, int ranks) {
 constexpr size_t kTableSmemMax = 16ull * kMaxRows + kMaxPages / 8 / 4 + 128;  // a cluster of 8
 static_assert(kTableSmemMax <= 224 * 1024, "a table kernel's shared memory");
 
-// CTAs of a table kernel.
-int table_ranks(const ce_page_table *t) { return t->pages <= 32768 && t->seqs <= 4096 ? 1 : 8; }
+// CTAs of a resize: one, whose barriers are cheap, or a cluster of 16 (the
+// non-portable size), which costs about 5,500 cycles more in barriers and
+// divides the rest: 0.25 cycles per page and 1.4 per token on one CTA. 64
+// requests, 4,096 pages: 6.7 us against 10.0; 1,021 requests, 98,304 pages,
+// 61,000 tokens: 83 us against 23.
+int resize_ranks(const ce_page_table *t, int capacity) {
+  return t->pages + 6ll * capacity > 26000 || t->seqs > kTableThreads ? 16 : 1;
+}
+// Of a reorder: its rows are a warp's work each, 32 of them at once in a CTA.
+// 4 rows: 8.4 us on one CTA, 10.2 on eight; 128 rows of 41 pages: 18.6 and 15.0.
+int reorder_ranks(const ce_page_table *t) { return t->seqs > 32 || t->pages > 26000 ? 8 : 1; }
 
 // Opts the table kernels into their shared memory, once per device.
 int configure_tables() {
@@ -579,6 +680,7 @@ int configure_tables() {
   CE_CUDA_TRY(cudaFuncSetAttribute(resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTableSmemMax));
   CE_CUDA_TRY(cudaFuncSetAttribute(reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)kTableSmemMax));
+  CE_CUDA_TRY(cudaFuncSetAttribute(resize_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   if (dev >= 0 && dev < 64) done[dev] = true;
   return CE_OK;
 }
@@ -686,7 +788,7 @@ int ce_paged_resize(const ce_page_table *to, const ce_page_table *from, const in
              "slots and pos are required for a capacity of %d", capacity);
   rc = configure_tables();
   if (rc != CE_OK) return rc;
-  const int ranks = table_ranks(from);
+  const int ranks = resize_ranks(from, capacity);
   const ResizeArgs a = {tables_of(to, from, status), new_lens, slots, pos, starts, capacity};
   return launch_tables(resize_kernel, a, ranks, table_smem(from, ranks), (cudaStream_t)stream, "resize_kernel");
 }
@@ -708,18 +810,20 @@ int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const i
   rc = configure_tables();
   if (rc != CE_OK) return rc;
   const cudaStream_t s = (cudaStream_t)stream;
-  const int ranks = table_ranks(from);
+  const int ranks = reorder_ranks(from);
   const ReorderArgs a = {tables_of(to, from, status), parents, beams, copies};
   rc = launch_tables(reorder_kernel, a, ranks, table_smem(from, ranks), s, "reorder_kernel");
   if (rc != CE_OK || kv == nullptr || kv->page_size == 1) return rc;
   const int b = type_bytes(kv->type);
   const CopyArgs c = {copies, to->lens_dev, static_cast<char *>(kv->k_dev), static_cast<char *>(kv->v_dev),
                       kv->layer_stride * b, kv->page_stride * b, kv->head_stride * b, kv->token_stride * b,
-                      kv->kv_heads, kv->head_dim * b / 16, kv->page_size};
-  const int most = (kv->page_size - 1) * c.kv_heads * c.pieces;  // pieces of a row in one layer
-  const dim3 grid((unsigned)((most + 1023) / 1024), (unsigned)from->seqs, (unsigned)kv->layers);
-  CE_REQUIRE(kv->layers <= 65535, "layers must be below 65536 (got %d)", kv->layers);
-  return launch_kernel(copy_pages_kernel, grid, dim3(256), 0, s, true, "copy_pages_kernel", c);
+                      from->seqs, kv->layers, kv->kv_heads, kv->head_dim * b / 16, kv->page_size};
+  const long long pairs = (long long)from->seqs * kv->layers, ctas = 8ll * sm_count();
+  const long long most = (kv->page_size - 1ll) * c.kv_heads * c.pieces;  // pieces of a pair
+  CE_REQUIRE(most < (1ll << 30), "a page of a layer is too large (%d tokens, %d heads)", kv->page_size, kv->kv_heads);
+  const unsigned x = (unsigned)std::min(pairs, ctas);
+  const unsigned y = (unsigned)std::max(1ll, std::min(ctas / x, most / (4 * kCopyThreads)));
+  return launch_kernel(copy_pages_kernel, dim3(x, y), dim3(kCopyThreads), 0, s, true, "copy_pages_kernel", c);
 }
 
 int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out, int q_out_type, const void *q, const void *k,
