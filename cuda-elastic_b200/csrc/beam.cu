@@ -7,9 +7,9 @@
 // the slice's `beams` best keys. A tile's candidates are found by a threshold
 // that is a lower bound of its beams-th best value: for the first tile the
 // beams-th largest of a warp's 32 lane maxima (the largest such over the
-// warps), later the worst key kept. On real logits a handful of values pass
-// it, and their ranks among themselves and the keys kept (counted, each
-// against all) put them in order. Keys are (logit, token) pairs as 64-bit
+// warps), later the first tile's beams-th best. On real logits a handful of
+// values pass it; they are collected without a barrier, and at the end their
+// ranks (counted, each against all) put them in order. Keys are (logit, token) pairs as 64-bit
 // integers, all different, so the order is total and independent of the
 // order in which threads append.
 //
@@ -60,7 +60,7 @@ __device__ __forceinline__ float logit_of(T v) {
 
 // Keys order tokens by (logit descending, token ascending) as integers.
 __device__ __forceinline__ unsigned long long key_of(float x, int token) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);  // -0 is +0
   const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
   return ((unsigned long long)o << 32) | (uint32_t)~token;
 }
@@ -103,29 +103,27 @@ __device__ __forceinline__ void add_sum(float &m, float &l, float m1, float l1) 
 
 struct Shared {
   unsigned long long buffer[kWarps * kListKeys];  // candidates; at the join the lists, per warp
-  unsigned long long top[kMaxBeams], next[kMaxBeams];
+  unsigned long long top[kMaxBeams];
   float kth[kWarps];
   float2 sums[kWarps];
   unsigned long long round[kWarps];
   float score[kMaxBeams][kMaxBeams];  // [beam][rank]
   int token[kMaxBeams][kMaxBeams];
-  int count[2], last;  // candidates of even and odd tiles
+  int count, last;
 };
 static_assert(kBuffer + kMaxBeams <= kWarps * kListKeys, "candidates and keys kept");
 
-// A tile's `beams` best by taking the best that is below the last taken, once
-// per rank: for tiles where the threshold leaves too much (rows of equal
-// logits) or none (rows banned but for a few tokens).
-template <class Key>
-__device__ __forceinline__ int take_in_rounds(Shared &sh, int beams, Key &&key) {
+// The `beams` best keys of the slice's tokens [t0, t1) by taking the best that
+// is below the last taken, once per rank, from memory: for slices where too
+// many values pass the threshold (equal or ascending logits).
+template <typename T>
+__device__ __noinline__ void take_in_rounds(Shared &sh, const T *x, int t0, int t1, int beams) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long last = ~0ull;
-  int n = 0;
-  for (; n < beams; ++n) {
+  for (int r = 0; r < beams; ++r) {
     unsigned long long k = 0;
-#pragma unroll
-    for (int i = 0; i <= kElems; ++i) {
-      const unsigned long long c = key(i);
+    for (int i = t0 + (int)threadIdx.x; i < t1; i += kThreads) {
+      const unsigned long long c = key_of(logit_of(x[i]), i);
       k = c < last && c > k ? c : k;
     }
 #pragma unroll
@@ -137,16 +135,50 @@ __device__ __forceinline__ int take_in_rounds(Shared &sh, int beams, Key &&key) 
     __syncthreads();
     for (int w = 0; w < kWarps; ++w) k = sh.round[w] > k ? sh.round[w] : k;
     __syncthreads();
-    if (k == 0) break;
-    if (threadIdx.x == 0) sh.buffer[n] = k;
+    if (threadIdx.x == 0) sh.top[r] = k;  // 0: no more
     last = k;
   }
-  return n;
+  __syncthreads();
+}
+
+// The `beams` best of the n keys in the buffer, in order, by their ranks
+// among all; 0 past the n-th.
+__device__ __forceinline__ void rank_buffer(Shared &sh, int n, int beams) {
+  if ((int)threadIdx.x < beams) sh.top[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long k = sh.buffer[i];
+    int rank = 0;
+    for (int q = 0; q < n; ++q) rank += sh.buffer[q] > k;
+    if (rank < beams) sh.top[rank] = k;
+  }
+  __syncthreads();
+}
+
+// The largest float below a finite x (so that y > it means y >= x).
+__device__ __forceinline__ float just_below(float x) {
+  const int b = __float_as_int(x);
+  return x == 0.f ? -__int_as_float(1) : __int_as_float(x > 0.f ? b - 1 : b + 1);
+}
+
+// The sum of e^(x - base) over N values, none above a finite base: one
+// multiply-add and one 2^y a value, relative to the rounded base log2 e, whose
+// rounding is taken back at the end.
+template <int N>
+__device__ __forceinline__ float sum_exp(const float (&x)[N], float base) {
+  const float b = base * kLog2e;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    s0 += exp2_approx(fmaf(x[i], kLog2e, -b));
+    s1 += exp2_approx(fmaf(x[i + 1], kLog2e, -b));
+  }
+  return (s0 + s1) * exp2_approx(-fmaf(base, kLog2e, -b));
 }
 
 template <typename T>
 __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int row, int slice) {
-  constexpr int kPerVec = 16 / sizeof(T), kVecs = kElems / kPerVec;
+  constexpr int kPerVec = 16 / sizeof(T), kVecs = kElems / kPerVec, kTile = kThreads * kVecs;  // in vectors
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
   const T *x = static_cast<const T *>(a.logits) + row * a.ld;
   // 16-byte vectors of the row from its first aligned element on; the few
@@ -160,79 +192,103 @@ __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int 
   if (slice == 0 && tid < head) extra = tid;
   if (slice == a.slices - 1 && tid >= 128 && tid < 128 + tail) extra = a.vocab - tail + tid - 128;
 
-  float m = -INFINITY, l = 0.f;
-  if (tid < K) sh.top[tid] = 0;
-  if (tid == 0) sh.count[0] = sh.count[1] = 0;
-  const int tiles = max(1, (v1 - v0 + kThreads * kVecs - 1) / (kThreads * kVecs));
+  uint4 raw[kVecs];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      if (at + v * kThreads < v1) raw[v] = __ldcs(xv + at + v * kThreads);
+  };
+  load(v0 + tid);
+  float ex = extra >= 0 ? logit_of(x[extra]) : -INFINITY;
+  float m = ex, l = ex > -INFINITY ? 1.f : 0.f;
+  if (tid == 0) sh.count = 0;
+  float bar = -INFINITY;
+  const int tiles = max(1, (v1 - v0 + kTile - 1) / kTile);
   for (int tile = 0; tile < tiles; ++tile) {
-    float e[kElems + 1];
-    const int at = v0 + tile * kThreads * kVecs + tid;
+    float e[kElems];
+    const int at = v0 + tile * kTile + tid;
+    const bool whole = v0 + (tile + 1) * kTile <= v1;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      const bool live = at + v * kThreads < v1;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (live) raw = __ldcs(xv + at + v * kThreads);
-      const T *p = reinterpret_cast<const T *>(&raw);
+      const T *p = reinterpret_cast<const T *>(&raw[v]);
 #pragma unroll
-      for (int i = 0; i < kPerVec; ++i) e[v * kPerVec + i] = live ? logit_of(p[i]) : -INFINITY;
+      for (int i = 0; i < kPerVec; ++i) e[v * kPerVec + i] = to_float(p[i]);
     }
-    const bool single = tile == 0 && extra >= 0;
-    e[kElems] = single ? logit_of(x[extra]) : -INFINITY;
-    auto token = [&](int i) { return i == kElems ? extra : head + (at + i / kPerVec * kThreads) * kPerVec + i % kPerVec; };
-    auto live = [&](int i) { return i == kElems ? single : at + i / kPerVec * kThreads < v1; };
-    float top = e[0];
+    if (!whole) {
 #pragma unroll
-    for (int i = 1; i <= kElems; ++i) top = fmaxf(top, e[i]);
-    if (top > -INFINITY) {
-      float s = 0.f;
-      const float base = fmaxf(top, m);
+      for (int v = 0; v < kVecs; ++v)
+        if (at + v * kThreads >= v1)
 #pragma unroll
-      for (int i = 0; i <= kElems; ++i) s += exp2_approx((e[i] - base) * kLog2e);  // a difference cannot overflow upwards
-      l = l * exp2_approx((m - base) * kLog2e) + s;
-      m = base;
+          for (int i = 0; i < kPerVec; ++i) e[v * kPerVec + i] = -INFINITY;
     }
-    // candidates
-    bool rounds = false, full = false;
-    float bar;
+    if (tile + 1 < tiles) load(at + kTile);  // under way during this tile
+    float top = e[0];  // of the numbers: a NaN is passed over
+#pragma unroll
+    for (int i = 1; i < kElems; ++i) top = fmaxf(top, e[i]);
+    if (!(top <= -INFINITY)) {
+      float base = fmaxf(top, m), s = sum_exp(e, base);
+      if (!(s <= kElems * 1.001f)) {  // a NaN, +inf, or values so large that their product with log2 e is not finite
+        top = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) e[i] = logit_of(e[i]), top = fmaxf(top, e[i]);
+        base = fmaxf(top, m);
+        if (base > -INFINITY)
+#pragma unroll
+          for (int i = 0; i < kElems; ++i) s += exp2_approx((e[i] - base) * kLog2e);  // a difference cannot overflow upwards
+      }
+      if (base > -INFINITY) l = l * exp2_approx((m - base) * kLog2e) + s, m = base;
+    }
+    // candidates: values above `bar`
     if (tile == 0) {
+      top = fmaxf(top, ex);
       const float kth = warp_kth(top, K);
       if (lane == 0) sh.kth[warp] = kth;
       __syncthreads();
       bar = sh.kth[0];
       for (int w = 1; w < kWarps; ++w) bar = fmaxf(bar, sh.kth[w]);
-      rounds = bar == -INFINITY;
-    } else {
-      full = sh.top[K - 1] != 0;  // then an equal value of a later token is no better
-      bar = full ? key_logit(sh.top[K - 1]) : -INFINITY;
-      rounds = !full;
+      if (bar > -INFINITY) bar = just_below(bar);
     }
-    if (!rounds && (full ? top > bar : top >= bar)) {
+    if (top > bar) {
+      auto offer = [&](float y, int token) {
+        const int n = atomicAdd(&sh.count, 1);
+        if (n < kBuffer) sh.buffer[n] = key_of(y, token);
+      };
 #pragma unroll
-      for (int i = 0; i <= kElems; ++i)
-        if (full ? e[i] > bar : e[i] >= bar) {
-          const int n = atomicAdd(&sh.count[tile & 1], 1);
-          if (n < kBuffer) sh.buffer[n] = key_of(e[i], token(i));
-        }
+      for (int i = 0; i < kElems; ++i)
+        if (e[i] > bar) offer(e[i], head + (at + i / kPerVec * kThreads) * kPerVec + i % kPerVec);
+      if (tile == 0 && ex > bar) offer(ex, extra);
     }
-    __syncthreads();
-    int n = sh.count[tile & 1];
-    if (n == 0 && !rounds) continue;  // no barrier: the next tile counts in the other word
-    if (rounds || n > kBuffer)
-      n = take_in_rounds(sh, K, [&](int i) { return live(i) ? key_of(e[i], token(i)) : 0ull; });
-    // ranks among the candidates and the keys kept
-    if (tid < K) sh.buffer[n + tid] = sh.top[tid], sh.next[tid] = 0;
-    __syncthreads();
-    n += K;
-    for (int i = tid; i < n; i += kThreads) {
-      const unsigned long long k = sh.buffer[i];
-      int rank = 0;
-      for (int q = 0; q < n; ++q) rank += sh.buffer[q] > k;
-      if (k != 0 && rank < K) sh.next[rank] = k;
+    if (tile == 0 && tiles > 1) {  // the first tile's beams-th best is the later ones' threshold
+      __syncthreads();
+      const int n = sh.count;
+      if (n > kBuffer) {
+        bar = INFINITY;  // too many: no more are taken, the rounds below decide
+      } else {
+        rank_buffer(sh, n, K);
+        if (tid < K) sh.buffer[tid] = sh.top[tid];
+        if (tid == 0) sh.count = min(n, K);
+        // an equal value of a later token is no better
+        bar = sh.top[K - 1] != 0 ? key_logit(sh.top[K - 1]) : -INFINITY;
+        __syncthreads();
+      }
     }
-    __syncthreads();
-    if (tid < K) sh.top[tid] = sh.next[tid];
-    if (tid == 0) sh.count[tile & 1] = 0;
-    __syncthreads();
+  }
+  __syncthreads();
+  const int t0 = slice == 0 ? 0 : head + v0 * kPerVec, t1 = slice == a.slices - 1 ? a.vocab : head + v1 * kPerVec;
+  int n = sh.count;
+  if (n > kBuffer) {
+    take_in_rounds(sh, x, t0, t1, K);
+  } else {
+    if (n < K) {
+      // Fewer than K values are finite: tokens of logit -inf follow, the
+      // lowest first. K of them, or all, stand among the first 2 K tokens.
+      __syncthreads();
+      if (tid < min(2 * K, t1 - t0) && logit_of(x[t0 + tid]) == -INFINITY)
+        sh.buffer[atomicAdd(&sh.count, 1)] = key_of(-INFINITY, t0 + tid);
+      __syncthreads();
+      n = sh.count;
+    }
+    rank_buffer(sh, n, K);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
@@ -298,12 +354,10 @@ __global__ void __launch_bounds__(kThreads, 4) select_kernel(BeamArgs a) {
   pdl_wait();
   const int row = group * K + blockIdx.y;
   if (!a.finished[row]) slice_of_row<T>(a, sh, row, blockIdx.x);
-  __threadfence();
   __syncthreads();
-  if (tid == 0) {
-    sh.last = atomicAdd(a.arrivals + group, 1) == K * a.slices - 1;
+  if (tid == 0) {  // releases this CTA's list and acquires the others'
+    sh.last = add_acq_rel(a.arrivals + group, 1) == K * a.slices - 1;
     if (sh.last) a.arrivals[group] = 0;
-    __threadfence();
   }
   __syncthreads();
   if (!sh.last) return;
@@ -330,11 +384,11 @@ __global__ void __launch_bounds__(kThreads, 4) select_kernel(BeamArgs a) {
   }
 }
 
-// Slices of a row: enough CTAs for about six on every SM, no slice below one
+// Slices of a row: enough CTAs for about three on every SM, no slice below one
 // tile of a CTA, and lists that fit the join.
 int slices_of(int rows, int beams, int vocab, int sms) {
   const int most = std::min({32, kListKeys / beams, (vocab + kThreads * kElems - 1) / (kThreads * kElems)});
-  return std::max(1, std::min(most, (6 * sms + rows - 1) / rows));
+  return std::max(1, std::min(most, (3 * sms + rows - 1) / rows));
 }
 
 }  // namespace

@@ -65,6 +65,12 @@ __device__ __forceinline__ T block_inclusive_sum(T v, T *scratch, T &total) {
   return (warp > 0 ? before : T(0)) + x;
 }
 
+__device__ __forceinline__ int add_acq_rel(int *p, int v) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
+}
+
 // First index of [0, n) whose value is above x (n if none); a ascending.
 __device__ __forceinline__ int first_above(const int *a, int n, int x) {
   int lo = 0, hi = n;

@@ -231,12 +231,6 @@ __device__ __forceinline__ void add_scaled(float4 &x, float f, float4 y) {
   x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
 }
 
-__device__ __forceinline__ int add_acq_rel(int *p, int v) {
-  int old;
-  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
-  return old;
-}
-
 // The request part that a CTA shares with others, for the join across CTAs.
 struct Crossing {
   int row, kh, tile, c0, c1;  // and the first and last of its CTAs
