@@ -5,13 +5,14 @@
 // each, so that a few rows still occupy many SMs; a CTA reads its slice once,
 // in tiles held in registers, and keeps a running (max, sum) per thread and
 // the slice's `beams` best keys. A tile's candidates are found by a threshold
-// that is a lower bound of its beams-th best value: for the first tile the
-// beams-th largest of a warp's 32 lane maxima (the largest such over the
-// warps), later the first tile's beams-th best. On real logits a handful of
-// values pass it; they are collected without a barrier, and at the end their
-// ranks (counted, each against all) put them in order. Keys are (logit, token) pairs as 64-bit
-// integers, all different, so the order is total and independent of the
-// order in which threads append.
+// that is a lower bound of its beams-th best value: for the first tile from
+// the sorted lane maxima of the warps, later the first tile's beams-th best
+// (few values pass it then: without that step, and so with some 17 candidates
+// a tile in the place of 8 / tile, 64 x 8 beams take 31 us in the place of
+// 22). They are collected without a barrier, and at the end their ranks
+// (counted, each against all) put them in order. Keys are (logit, token)
+// pairs as 64-bit integers, all different, so the order is total and
+// independent of the order in which threads append.
 //
 // The last CTA of a batch element to arrive joins the slices: a warp per
 // beam plays the sorted lists of its slices off against one another (a lane
@@ -76,8 +77,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// The k-th largest of the warp's 32 values (k from 1).
-__device__ __forceinline__ float warp_kth(float v, int k) {
+// The warp's 32 values in descending order of lanes.
+__device__ __forceinline__ float warp_sorted(float v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
@@ -87,7 +88,7 @@ __device__ __forceinline__ float warp_kth(float v, int k) {
       const bool up = ((lane & step) != 0) == ((lane & size) != 0);  // this lane keeps the larger one
       v = up ? fmaxf(v, y) : fminf(v, y);
     }
-  return __shfl_sync(0xffffffffu, v, k - 1);
+  return v;
 }
 
 // Joins (max, sum of e^(x - max)) pairs.
@@ -104,7 +105,7 @@ __device__ __forceinline__ void add_sum(float &m, float &l, float m1, float l1) 
 struct Shared {
   unsigned long long buffer[kWarps * kListKeys];  // candidates; at the join the lists, per warp
   unsigned long long top[kMaxBeams];
-  float kth[kWarps];
+  float2 kth[kWarps];
   float2 sums[kWarps];
   unsigned long long round[kWarps];
   float score[kMaxBeams][kMaxBeams];  // [beam][rank]
@@ -176,10 +177,12 @@ __device__ __forceinline__ float sum_exp(const float (&x)[N], float base) {
   return (s0 + s1) * exp2_approx(-fmaf(base, kLog2e, -b));
 }
 
+// open: the batch element's unfinished beams, read behind the first loads.
 template <typename T>
-__device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int row, int slice) {
+__device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int group, int beam, int slice, uint32_t &open) {
   constexpr int kPerVec = 16 / sizeof(T), kVecs = kElems / kPerVec, kTile = kThreads * kVecs;  // in vectors
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams;
+  const int row = group * K + beam;
   const T *x = static_cast<const T *>(a.logits) + row * a.ld;
   // 16-byte vectors of the row from its first aligned element on; the few
   // elements before and after them go to the first and last slice, one per thread
@@ -199,6 +202,8 @@ __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int 
       if (at + v * kThreads < v1) raw[v] = __ldcs(xv + at + v * kThreads);
   };
   load(v0 + tid);
+  open = __ballot_sync(0xffffffffu, lane < K && !a.finished[group * K + min(lane, K - 1)]);
+  if (!(open >> beam & 1)) return false;
   float ex = extra >= 0 ? logit_of(x[extra]) : -INFINITY;
   float m = ex, l = ex > -INFINITY ? 1.f : 0.f;
   if (tid == 0) sh.count = 0;
@@ -241,11 +246,16 @@ __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int 
     // candidates: values above `bar`
     if (tile == 0) {
       top = fmaxf(top, ex);
-      const float kth = warp_kth(top, K);
-      if (lane == 0) sh.kth[warp] = kth;
+      // At least K of the block's lane maxima reach the K-th of any warp, and
+      // as many reach the ceil(K / 8)-th of every one of the 8 warps.
+      const float sorted = warp_sorted(top), few = __shfl_sync(0xffffffffu, sorted, (K + kWarps - 1) / kWarps - 1),
+                  kth = __shfl_sync(0xffffffffu, sorted, K - 1);
+      if (lane == 0) sh.kth[warp] = make_float2(few, kth);
       __syncthreads();
-      bar = sh.kth[0];
-      for (int w = 1; w < kWarps; ++w) bar = fmaxf(bar, sh.kth[w]);
+      float every = sh.kth[0].x;
+      bar = sh.kth[0].y;
+      for (int w = 1; w < kWarps; ++w) every = fminf(every, sh.kth[w].x), bar = fmaxf(bar, sh.kth[w].y);
+      bar = fmaxf(bar, every);
       if (bar > -INFINITY) bar = just_below(bar);
     }
     if (top > bar) {
@@ -258,7 +268,7 @@ __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int 
         if (e[i] > bar) offer(e[i], head + (at + i / kPerVec * kThreads) * kPerVec + i % kPerVec);
       if (tile == 0 && ex > bar) offer(ex, extra);
     }
-    if (tile == 0 && tiles > 1) {  // the first tile's beams-th best is the later ones' threshold
+    if (tile == 0 && tiles > 1) {  // the first tile's K-th best is the later ones' threshold
       __syncthreads();
       const int n = sh.count;
       if (n > kBuffer) {
@@ -300,6 +310,7 @@ __device__ __forceinline__ void slice_of_row(const BeamArgs &a, Shared &sh, int 
     for (int w = 1; w < kWarps; ++w) add_sum(m, l, sh.sums[w].x, sh.sums[w].y);
     __stcg(a.sums + list, make_float2(m, l));
   }
+  return true;
 }
 
 // The best key of the warp's lanes, and which lane holds it (keys differ).
@@ -345,22 +356,27 @@ __device__ __forceinline__ int offers_of_row(const BeamArgs &a, Shared &sh, int 
   return n;
 }
 
-// Grid (slices, beams, batch).
+// Grid (slices, beams, batch). Finished beams have no logits to read: their
+// CTAs leave, and the join waits for the others (the first CTA joins where
+// all are finished).
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) select_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) select_kernel(const __grid_constant__ BeamArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.beams, group = blockIdx.z;
   pdl_launch_dependents();
   pdl_wait();
-  const int row = group * K + blockIdx.y;
-  if (!a.finished[row]) slice_of_row<T>(a, sh, row, blockIdx.x);
-  __syncthreads();
-  if (tid == 0) {  // releases this CTA's list and acquires the others'
-    sh.last = add_acq_rel(a.arrivals + group, 1) == K * a.slices - 1;
-    if (sh.last) a.arrivals[group] = 0;
+  uint32_t open;
+  if (slice_of_row<T>(a, sh, group, blockIdx.y, blockIdx.x, open)) {
+    __syncthreads();
+    if (tid == 0) {  // releases this CTA's list and acquires the others'
+      sh.last = add_acq_rel(a.arrivals + group, 1) == __popc(open) * a.slices - 1;
+      if (sh.last) a.arrivals[group] = 0;
+    }
+    __syncthreads();
+    if (!sh.last) return;
+  } else if (open != 0 || blockIdx.x + blockIdx.y != 0) {
+    return;
   }
-  __syncthreads();
-  if (!sh.last) return;
   for (int beam = warp; beam < K; beam += kWarps) {
     offers_of_row(a, sh, group, beam);
     __syncwarp();
