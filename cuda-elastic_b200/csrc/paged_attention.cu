@@ -813,13 +813,12 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     float4 *const sums = reinterpret_cast<float4 *>(smem);                     // [groups][tasks]
     float *const inv = reinterpret_cast<float *>(sums + S::kThreads);          // [heads] v_scale / sum
     float2 *const weight = reinterpret_cast<float2 *>(inv + S::kHeads);        // [heads][n]
+    for (int u = tid; u < heads * n; u += S::kThreads)
+      weight[u] = __ldcg(reinterpret_cast<const float2 *>(part(u % n) + S::kHeads * D + 2 * (u / n)));
+    __syncthreads();
     for (int h = warp; h < heads; h += W) {
       float m = -INFINITY;
-      for (int i = lane; i < n; i += 32) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part(i) + S::kHeads * D + 2 * h));
-        weight[h * n + i] = ml;
-        m = fmaxf(m, ml.x);
-      }
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, weight[h * n + i].x);
 #pragma unroll
       for (int y = 16; y; y >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
       const float base = m == -INFINITY ? 0.f : m;
@@ -837,29 +836,43 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
       }
     }
     __syncthreads();
-    auto sum_parts = [&](int task, int i0, int step) {
-      const int h = task / (D / 4), d = 4 * (task % (D / 4));
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int i = i0; i < n; i += step)
-        add_scaled(y, weight[h * n + i].x, __ldcg(reinterpret_cast<const float4 *>(part(i) + h * D + d)));
-      return y;
-    };
-    auto finish = [&](int task, float4 y) {
-      const int h = task / (D / 4), d = 4 * (task % (D / 4));
-      if (d < a.dim) store_out4<Io>(a, c.row, head0 + h, d, y, inv[h]);
-    };
-    if (tasks >= S::kThreads) {
-      for (int task = tid; task < tasks; task += S::kThreads) finish(task, sum_parts(task, 0, 1));
-    } else {
-      const int groups = S::kThreads / tasks, group = tid / tasks;
-      if (group < groups) sums[tid] = sum_parts(tid % tasks, group, groups);
-      __syncthreads();
-      if (tid < tasks) {
-        float4 y = sums[tid];
-        for (int i = 1; i < groups; ++i) add_scaled(y, 1.f, sums[i * tasks + tid]);
-        finish(tid, y);
+    // kOwn tasks of a thread side by side, so that enough reads are under way
+    constexpr int kOwn = (S::kHeads * D / 4 + S::kThreads - 1) / S::kThreads;
+    const int groups = max(1, S::kThreads / tasks), group = groups > 1 ? tid / tasks : 0;
+    const int task0 = groups > 1 ? tid % tasks : tid;
+    float4 y[kOwn];
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) y[o] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (group < groups) {
+      // (reads past the last part or task are of the last one, with weight 0)
+      for (int i0 = group; i0 < n; i0 += 4 * groups) {
+        float4 x[4][kOwn];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float4 *const from = reinterpret_cast<const float4 *>(part(min(i0 + u * groups, n - 1)));
+#pragma unroll
+          for (int o = 0; o < kOwn; ++o) x[u][o] = __ldcg(from + min(task0 + o * S::kThreads, tasks - 1));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int o = 0; o < kOwn; ++o) {
+            const int i = i0 + u * groups, task = task0 + o * S::kThreads;
+            const float w = weight[min(task, tasks - 1) / (D / 4) * n + min(i, n - 1)].x;
+            add_scaled(y[o], i < n ? w : 0.f, x[u][o]);
+          }
       }
+    }
+    if (groups > 1) {
+      if (group < groups) sums[tid] = y[0];
+      __syncthreads();
+      if (tid < tasks)
+        for (int i = 1; i < groups; ++i) add_scaled(y[0], 1.f, sums[i * tasks + tid]);
+    }
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      const int task = tid + o * S::kThreads, h = task / (D / 4), d = 4 * (task % (D / 4));
+      if (task < tasks && d < a.dim) store_out4<Io>(a, c.row, head0 + h, d, y[o], inv[h]);
     }
     __syncthreads();
   }
