@@ -564,20 +564,21 @@ __device__ __forceinline__ void store8(__nv_fp8_e4m3 *p, const float (&x)[8]) {
 }
 
 // One thread per 8 elements (4 rotary pairs) of a q, k or v head of a token,
-// in fp32, rounded once where it is stored. Bound by memory: every element
-// is read and written once; a token's slot, position and rotary row are read
-// by its block (one or a few) and served from L1 to all its heads.
+// in fp32, rounded once where it is stored. Blocks are (head_dim / 8, heads):
+// no index is divided, since the threads are many and short (with divided
+// indices and divisions by the scales 206 instructions a thread, and the
+// issue slots, not the memory, were the bound). Every element is read and
+// written once; a token's slot, position and rotary row are served from L1
+// to all its heads.
 constexpr int kAppendThreads = 256;
 template <typename In, typename Out, typename Cache>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_launch_dependents();
-  const unsigned eighths = (unsigned)a.dim >> 3;
-  const unsigned q_units = a.heads * eighths, kv_units = a.kv_heads * eighths;
-  unsigned u = blockIdx.y * kAppendThreads + threadIdx.x;
-  if (u >= q_units + 2 * kv_units) return;
-  const int part = u < q_units ? 0 : u < q_units + kv_units ? 1 : 2;
-  u -= part == 0 ? 0 : part == 1 ? q_units : q_units + kv_units;
-  const int head = (int)(u / eighths), d = 8 * (int)(u % eighths), tok = blockIdx.x;
+  int head = blockIdx.y * blockDim.y + threadIdx.y;  // q heads, then k heads, then v heads
+  if (head >= a.heads + 2 * a.kv_heads) return;
+  const int part = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : 2;
+  head -= part == 0 ? 0 : part == 1 ? a.heads : a.heads + a.kv_heads;
+  const int d = 8 * threadIdx.x, tok = blockIdx.x;
   const In *src = part == 0 ? static_cast<const In *>(a.q) + tok * a.q_ld
                 : part == 1 ? static_cast<const In *>(a.k) + tok * a.k_ld
                             : static_cast<const In *>(a.v) + tok * a.v_ld;
@@ -621,9 +622,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
   }
   const float *scale = part == 1 ? a.k_scale : a.v_scale;
   if (scale != nullptr) {
-    const float s = __ldg(scale + head);
+    const float inv = 1.f / __ldg(scale + head);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] / s;
+    for (int i = 0; i < 8; ++i) x[i] *= inv;
   }
   Cache *base = reinterpret_cast<Cache *>(part == 1 ? a.kc : a.vc);
   store8(base + (slot >> a.shift) * a.page_stride + head * a.head_stride +
@@ -701,18 +702,18 @@ Tables tables_of(const ce_page_table *to, const ce_page_table *from, int32_t *st
 }
 
 template <typename In, typename Out>
-int launch_append(int cache_type, const AppendArgs &a, dim3 grid, cudaStream_t s) {
+int launch_append(int cache_type, const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
   if (cache_type == CE_TYPE_BF16)
-    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
+    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, block, 0, s, true, "append_kernel", a);
   if (cache_type == CE_TYPE_F16)
-    return launch_kernel(append_kernel<In, Out, __half>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
-  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, dim3(kAppendThreads), 0, s, true, "append_kernel", a);
+    return launch_kernel(append_kernel<In, Out, __half>, grid, block, 0, s, true, "append_kernel", a);
+  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, block, 0, s, true, "append_kernel", a);
 }
 
 template <typename In>
-int launch_append(int out_type, int cache_type, const AppendArgs &a, dim3 grid, cudaStream_t s) {
-  return out_type == CE_TYPE_F16 ? launch_append<In, __half>(cache_type, a, grid, s)
-                                 : launch_append<In, __nv_bfloat16>(cache_type, a, grid, s);
+int launch_append(int out_type, int cache_type, const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
+  return out_type == CE_TYPE_F16 ? launch_append<In, __half>(cache_type, a, grid, block, s)
+                                 : launch_append<In, __nv_bfloat16>(cache_type, a, grid, block, s);
 }
 
 }  // namespace
@@ -857,13 +858,14 @@ int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out, int q_out_typ
   a.slot_end = (long long)kv->pages * kv->page_size;
   a.tokens = tokens, a.heads = q != nullptr ? heads : 0, a.kv_heads = kv->kv_heads, a.dim = kv->head_dim;
   a.shift = log2_of(kv->page_size), a.rope_len = rope_len;
-  const long long units = (a.heads + 2ll * a.kv_heads) * (a.dim / 8);  // of a token
-  CE_REQUIRE(units <= 65535ll * kAppendThreads, "too many heads (%d + 2 x %d)", heads, kv->kv_heads);
-  const dim3 grid((unsigned)tokens, (unsigned)((units + kAppendThreads - 1) / kAppendThreads));
+  const unsigned x = (unsigned)a.dim / 8, y = kAppendThreads / x;
+  const long long all = a.heads + 2ll * a.kv_heads;
+  CE_REQUIRE(all <= 65535ll * y, "too many heads (%d + 2 x %d)", heads, kv->kv_heads);
+  const dim3 grid((unsigned)tokens, (unsigned)((all + y - 1) / y)), block(x, y);
   const cudaStream_t s = (cudaStream_t)stream;
-  if (in_type == CE_TYPE_F32) return launch_append<float>(q_out_type, kv->type, a, grid, s);
-  if (in_type == CE_TYPE_F16) return launch_append<__half>(q_out_type, kv->type, a, grid, s);
-  return launch_append<__nv_bfloat16>(q_out_type, kv->type, a, grid, s);
+  if (in_type == CE_TYPE_F32) return launch_append<float>(q_out_type, kv->type, a, grid, block, s);
+  if (in_type == CE_TYPE_F16) return launch_append<__half>(q_out_type, kv->type, a, grid, block, s);
+  return launch_append<__nv_bfloat16>(q_out_type, kv->type, a, grid, block, s);
 }
 
 }  // extern "C"

@@ -906,7 +906,7 @@ int ce_paged_resize(const ce_page_table *to, const ce_page_table *from, const in
  * [rope_len][head_dim / 2][2]; NULL: no turn, pos may then be NULL), in fp32.
  * q goes to q_out [tokens][heads][head_dim] of q_out_type (16 bits), k and v
  * to slot slots[t] of `layer`, rounded to the nearest value of the pool's
- * type (E4M3: of x / scale, saturating at 448). A token whose slot is
+ * type (E4M3: of x * (1 / scale), saturating at 448). A token whose slot is
  * negative writes no cache, and zeros to q_out. Slots past the pool and
  * positions past rope_len are left out the same way and reported by
  * ce_device_status (CE_ERR_USAGE). q_dev and q_out_dev may both be NULL. */
