@@ -1019,7 +1019,8 @@ def _paged_setup():
     _I32, _I64, _F32, _BOOL = torch.int32, torch.int64, torch.float32, torch.bool
     _TYPES.update({torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16,
                    torch.float8_e4m3fn: TYPE_E4M3})
-    _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+    torch.cuda.init()
+    _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
     _L = lib()
 
 

@@ -87,7 +87,7 @@ struct Shape {
   static constexpr int kStageBytes = 2 * kTiles * kTileBytes;   // keys, then values
   static constexpr int kWarps = NT == 1 ? (kTiles == 2 ? 8 : D == 128 ? 10 : 12)
                                         : (kTiles == 2 ? 6 : D == 128 ? 8 : 10);
-  static constexpr int kStages = kTiles == 2 ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kHeads = 8 * NT;
   static constexpr int kPart = kHeads * (D + 2);  // floats of one (O, max, sum) part
   static constexpr int kVals = D / 8;             // dimensions of a value row per lane
