@@ -112,7 +112,8 @@ struct Shared {
   int token[kMaxBeams][kMaxBeams];
   int count, last;
 };
-static_assert(kBuffer + kMaxBeams <= kWarps * kListKeys, "candidates and keys kept");
+static_assert(kBuffer + 3 * kMaxBeams <= kWarps * kListKeys, "candidates and what follows them");
+static_assert(kElems == 16, "four tops of four");
 
 // The `beams` best keys of the slice's tokens [t0, t1) by taking the best that
 // is below the last taken, once per rank, from memory: for slices where too
@@ -227,15 +228,20 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
           for (int i = 0; i < kPerVec; ++i) e[v * kPerVec + i] = -INFINITY;
     }
     if (tile + 1 < tiles) load(at + kTile);  // under way during this tile
-    float top = e[0];  // of the numbers: a NaN is passed over
+    float tops[kElems / 4];  // of four numbers each: a NaN is passed over
 #pragma unroll
-    for (int i = 1; i < kElems; ++i) top = fmaxf(top, e[i]);
+    for (int i = 0; i < kElems; i += 4) tops[i / 4] = fmaxf(fmaxf(e[i], e[i + 1]), fmaxf(e[i + 2], e[i + 3]));
+    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     if (!(top <= -INFINITY)) {
       float base = fmaxf(top, m), s = sum_exp(e, base);
       if (!(s <= kElems * 1.001f)) {  // a NaN, +inf, or values so large that their product with log2 e is not finite
         top = -INFINITY, s = 0.f;
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) e[i] = logit_of(e[i]), top = fmaxf(top, e[i]);
+        for (int i = 0; i < kElems; ++i) {
+          e[i] = logit_of(e[i]);
+          tops[i / 4] = i % 4 ? fmaxf(tops[i / 4], e[i]) : e[i];
+          top = fmaxf(top, e[i]);
+        }
         base = fmaxf(top, m);
         if (base > -INFINITY)
 #pragma unroll
@@ -264,8 +270,12 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
         if (n < kBuffer) sh.buffer[n] = key_of(y, token);
       };
 #pragma unroll
-      for (int i = 0; i < kElems; ++i)
-        if (e[i] > bar) offer(e[i], head + (at + i / kPerVec * kThreads) * kPerVec + i % kPerVec);
+      for (int i = 0; i < kElems; i += 4)  // four at a time: hardly any of them has one
+        if (tops[i / 4] > bar) {
+#pragma unroll
+          for (int y = i; y < i + 4; ++y)
+            if (e[y] > bar) offer(e[y], head + (at + y / kPerVec * kThreads) * kPerVec + y % kPerVec);
+        }
       if (tile == 0 && ex > bar) offer(ex, extra);
     }
     if (tile == 0 && tiles > 1) {  // the first tile's K-th best is the later ones' threshold
