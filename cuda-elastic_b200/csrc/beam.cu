@@ -7,7 +7,7 @@
 // the slice's `beams` best keys. A tile's candidates are found by a threshold
 // that is a lower bound of its beams-th best value: for the first tile from
 // the sorted lane maxima of the warps, later the first tile's beams-th best
-// (few values pass it then: without that step, and so with some 17 candidates
+// (without that step, with some 17 candidates
 // a tile in the place of 8 / tile, 64 x 8 beams take 31 us in the place of
 // 22). They are collected without a barrier, and at the end their ranks
 // (counted, each against all) put them in order. Keys are (logit, token)
@@ -38,7 +38,8 @@ constexpr int kMaxGroups = 16384;  // batch elements: arrival counters at the fr
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kElems = 16;         // logits per thread and tile
-constexpr int kBuffer = 1024;      // candidates of a tile
+constexpr int kFirst = 1024;       // candidates of the first tile
+constexpr int kLater = 768;        // of the later ones
 constexpr int kListKeys = 256;     // keys of one beam's lists at the join: slices x beams
 
 struct BeamArgs {
@@ -116,9 +117,10 @@ struct Shared {
   unsigned long long round[kWarps];
   float score[kMaxBeams][kMaxBeams];  // [beam][rank]
   int token[kMaxBeams][kMaxBeams];
-  int count, last;
+  int first, later, passed, last;  // candidates; warps past the first tile
+  float bar;                       // what a later tile's candidates exceed
 };
-static_assert(kBuffer + 3 * kMaxBeams <= kWarps * kListKeys, "candidates and what follows them");
+static_assert(kFirst + kLater + 2 * kMaxBeams <= kWarps * kListKeys, "candidates and what follows them");
 static_assert(kElems == 16, "four tops of four");
 
 // The `beams` best keys of the slice's tokens [t0, t1) by taking the best that
@@ -149,18 +151,37 @@ __device__ __noinline__ void take_in_rounds(Shared &sh, const T *x, int t0, int 
   __syncthreads();
 }
 
-// The `beams` best of the n keys in the buffer, in order, by their ranks
-// among all; 0 past the n-th.
-__device__ __forceinline__ void rank_buffer(Shared &sh, int n, int beams) {
+// The `beams` best of the candidates, buffer[0, n0) and buffer[kFirst, kFirst
+// + n1), in order, by their ranks among all; 0 past the last.
+__device__ __forceinline__ void rank_candidates(Shared &sh, int n0, int n1, int beams) {
   if ((int)threadIdx.x < beams) sh.top[threadIdx.x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const unsigned long long k = sh.buffer[i];
+  for (int i = threadIdx.x; i < n0 + n1; i += kThreads) {
+    const unsigned long long k = sh.buffer[i < n0 ? i : kFirst + i - n0];
     int rank = 0;
-    for (int q = 0; q < n; ++q) rank += sh.buffer[q] > k;
+    for (int q = 0; q < n0; ++q) rank += sh.buffer[q] > k;
+    for (int q = kFirst; q < kFirst + n1; ++q) rank += sh.buffer[q] > k;
     if (rank < beams) sh.top[rank] = k;
   }
   __syncthreads();
+}
+
+// By one warp: the beams-th best logit of the first tile's n candidates (no
+// bar if there are fewer).
+__device__ __forceinline__ float later_bar(const Shared &sh, int n, int beams) {
+  unsigned long long last = ~0ull;
+  if (n < beams) return -INFINITY;
+  for (int r = 0; r < beams; ++r) {
+    unsigned long long k = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+      const unsigned long long c = sh.buffer[i];
+      k = c < last && c > k ? c : k;
+    }
+    const uint32_t hi = (uint32_t)(k >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+    const uint32_t low = __reduce_max_sync(0xffffffffu, hi == top ? (uint32_t)k : 0u);
+    last = (unsigned long long)top << 32 | low;
+  }
+  return key_logit(last);
 }
 
 // The largest float below a finite x (so that y > it means y >= x).
@@ -213,7 +234,7 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
   if (!(open >> beam & 1)) return false;
   float ex = extra >= 0 ? logit_of(x[extra]) : -INFINITY;
   float m = ex, l = ex > -INFINITY ? 1.f : 0.f;
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.first = sh.later = sh.passed = 0, sh.bar = -INFINITY;
   float bar = -INFINITY;
   const int tiles = max(1, (v1 - v0 + kTile - 1) / kTile);
   for (int tile = 0; tile < tiles; ++tile) {
@@ -257,7 +278,7 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
     }
     // candidates: values above `bar`
     if (tile == 0) {
-      top = fmaxf(top, ex);
+      if (extra < head) top = fmaxf(top, ex);
       // At least K of the block's lane maxima reach the K-th of any warp, and
       // as many reach the ceil(K / 8)-th of every one of the 8 warps.
       const float sorted = warp_sorted(top), few = __shfl_sync(0xffffffffu, sorted, (K + kWarps - 1) / kWarps - 1),
@@ -269,52 +290,61 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
       for (int w = 1; w < kWarps; ++w) every = fminf(every, sh.kth[w].x), bar = fmaxf(bar, sh.kth[w].y);
       bar = fmaxf(bar, every);
       if (bar > -INFINITY) bar = just_below(bar);
+    } else {
+      bar = fmaxf(bar, *(volatile float *)&sh.bar);
     }
+    auto offer = [&](bool first, float y, int token) {
+      const int n = atomicAdd(first ? &sh.first : &sh.later, 1);
+      if (n < (first ? kFirst : kLater)) sh.buffer[(first ? 0 : kFirst) + n] = key_of(y, token);
+    };
     if (top > bar) {
-      auto offer = [&](float y, int token) {
-        const int n = atomicAdd(&sh.count, 1);
-        if (n < kBuffer) sh.buffer[n] = key_of(y, token);
-      };
 #pragma unroll
       for (int i = 0; i < kElems; i += 4)  // four at a time: hardly any of them has one
         if (tops[i / 4] > bar) {
 #pragma unroll
           for (int y = i; y < i + 4; ++y)
-            if (e[y] > bar) offer(e[y], head + (at + y / kPerVec * kThreads) * kPerVec + y % kPerVec);
+            if (e[y] > bar) offer(tile == 0, e[y], head + (at + y / kPerVec * kThreads) * kPerVec + y % kPerVec);
         }
-      if (tile == 0 && ex > bar) offer(ex, extra);
     }
-    if (tile == 0 && tiles > 1) {  // the first tile's K-th best is the later ones' threshold
-      __syncthreads();
-      const int n = sh.count;
-      if (n > kBuffer) {
-        bar = INFINITY;  // too many: no more are taken, the rounds below decide
-      } else {
-        rank_buffer(sh, n, K);
-        if (tid < K) sh.buffer[tid] = sh.top[tid];
-        if (tid == 0) sh.count = min(n, K);
-        // an equal value of a later token is no better
-        bar = sh.top[K - 1] != 0 ? key_logit(sh.top[K - 1]) : -INFINITY;
-        __syncthreads();
+    // the row's last elements, behind all tiles by their tokens, count with the later ones
+    if (tile == 0 && ex > bar) offer(extra < head, ex, extra);
+    if (tile == 0 && tiles > 1) {
+      // The last warp to have offered its part of the first tile takes the
+      // K-th best of these as the later tiles' bar; nobody waits for it. (An
+      // equal value of a later token is no better.)
+      __syncwarp();
+      int passed = 0;
+      if (lane == 0) {
+        __threadfence_block();
+        passed = atomicAdd(&sh.passed, 1);
+        __threadfence_block();
+      }
+      passed = __shfl_sync(0xffffffffu, passed, 0);
+      __syncwarp();
+      if (passed == kWarps - 1) {
+        const int n = *(volatile int *)&sh.first;
+        const float kth = n > kFirst ? INFINITY : later_bar(sh, n, K);  // too many: the rounds below decide
+        if (lane == 0) *(volatile float *)&sh.bar = kth;
       }
     }
   }
   __syncthreads();
   const int t0 = slice == 0 ? 0 : head + v0 * kPerVec, t1 = slice == a.slices - 1 ? a.vocab : head + v1 * kPerVec;
-  int n = sh.count;
-  if (n > kBuffer) {
+  int n0 = sh.first;
+  const int n1 = sh.later;
+  if (n0 > kFirst || n1 > kLater) {
     take_in_rounds(sh, x, t0, t1, K);
   } else {
-    if (n < K) {
+    if (n0 + n1 < K) {
       // Fewer than K values are finite: tokens of logit -inf follow, the
       // lowest first. K of them, or all, stand among the first 2 K tokens.
       __syncthreads();
       if (tid < min(2 * K, t1 - t0) && logit_of(x[t0 + tid]) == -INFINITY)
-        sh.buffer[atomicAdd(&sh.count, 1)] = key_of(-INFINITY, t0 + tid);
+        sh.buffer[atomicAdd(&sh.first, 1)] = key_of(-INFINITY, t0 + tid);
       __syncthreads();
-      n = sh.count;
+      n0 = sh.first;
     }
-    rank_buffer(sh, n, K);
+    rank_candidates(sh, n0, n1, K);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));

@@ -56,6 +56,20 @@ def test_ties_go_to_the_lowest_token_and_beam(ce, dev):
     assert (got[3] == [False, False, True, False, False, False]).all()
 
 
+def test_ties_across_tiles_of_long_rows(ce, dev):
+    """So many rows that each is one CTA's: ties between the first tile, later
+    ones and the row's last elements (odd vocabulary) go to the lowest token;
+    16-bit logits are full of them."""
+    rng = np.random.default_rng(8)
+    B, K, V = 100, 6, 12007
+    x = torch.from_numpy((rng.standard_normal((B * K, V)) * 2).astype(np.float32)).to(dev).to(torch.bfloat16)
+    x[::3, [5, 4100, 8200, V - 1, V - 2]] = 9.0
+    x[1::3] = x[1::3].clamp(max=5.0)  # a plateau of the largest value
+    x[2::12] = -1.5  # nothing but ties: 12,007 candidates
+    scores, finished = -rng.random((B, K)).astype(np.float32), rng.random((B, K)) < 0.1
+    check(run(ce, dev, x, scores, finished), R.beam_select(x.float().cpu().numpy(), scores, finished, 2, 0), V)
+
+
 @pytest.mark.parametrize("V", [50, 9000])
 def test_infinities_and_nan(ce, dev, V):
     """Banned (-inf) and NaN logits are never taken before a finite one; a row
