@@ -39,8 +39,9 @@
 //     rounded value and what the rounding lost): rounded once to 16 bits they
 //     would err as much as the output's own rounding.
 //   * A request split over warps or CTAs is joined from (max, sum, O) parts:
-//     within a CTA from shared memory, across CTAs by the last to arrive, in
-//     the order of the keys, so the result does not depend on who is last.
+//     within a CTA from shared memory, across CTAs by the last to arrive or,
+//     where parts are many, by a launch of their own; in the order of the
+//     keys, so the result does not depend on who is last.
 //
 // Measured (B200, measured copy rate 6.45 TB/s): 64 requests of 32 heads of
 // 128, 805 MB of bf16 keys and values, 127 us = 6.2 TB/s; six documents with
@@ -74,6 +75,11 @@ constexpr int kMaxGrid = 1024;         // CTAs the workspace's counters are laid
 constexpr int kRowsPerLane = 8;        // requests per lane up to which a warp scans the lengths by itself
 constexpr int kPartFloats = kMaxSplitHeads * (128 + 2);
 
+// The request part that a CTA shares with others, for the join across CTAs.
+struct Crossing {
+  int row, kh, tile, c0, c1;  // and the first and last of its CTAs
+};
+
 struct AttnArgs {
   const void *q;
   void *out;
@@ -85,6 +91,7 @@ struct AttnArgs {
   int group, tiles;  // query heads per kv head; passes over them
   float scale;
   int *arrivals;  // [kMaxGrid], zero between calls
+  Crossing *crossings;  // [grid], of the requests that begin in a CTA and end in another; null: joined here
   float *parts;   // [grid][2][kPartFloats]
 };
 
@@ -248,11 +255,6 @@ __device__ __forceinline__ void add_scaled(float4 &x, float f, float4 y) {
   x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
 }
 
-// The request part that a CTA shares with others, for the join across CTAs.
-struct Crossing {
-  int row, kh, tile, c0, c1;  // and the first and last of its CTAs
-};
-
 template <int D, int NT, bool F8, typename Io>
 __global__ void __launch_bounds__(Shape<D, NT, F8>::kThreads, 1)
 attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -283,6 +285,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   }
   __syncthreads();
   pdl_wait();
+  if (a.crossings != nullptr && tid == 0) a.crossings[blockIdx.x].row = -1;
 
   // ---- the line: for every request, kv head and pass over its query heads a
   // slot for the change to it (fetching q, writing the output: about the time
@@ -810,6 +813,10 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   }
   __syncthreads();
   if (n_crossing == 0) return;
+  if (a.crossings != nullptr) {  // join_kernel does the rest
+    if (tid < n_crossing && crossing[tid].c0 == (int)blockIdx.x) a.crossings[blockIdx.x] = crossing[tid];
+    return;
+  }
   if (tid < n_crossing) {
     // releases the CTA's part (written before the barrier) and acquires the others'
     const Crossing c = crossing[tid];
@@ -895,6 +902,54 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
   }
 }
 
+// The join across CTAs as a launch of its own: block (c, h) joins the parts of
+// query head h of the request that begins in CTA c and ends in a later one.
+constexpr int kJoinThreads = 256;
+template <int D, int HEADS, typename Io>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnArgs a) {
+  __shared__ float2 weight[kMaxGrid];
+  __shared__ float4 sums[kJoinThreads];
+  const int tid = threadIdx.x, lane = tid & 31, h = blockIdx.y;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Crossing c = a.crossings[blockIdx.x];
+  if (c.row < 0 || h >= a.group - c.tile * HEADS) return;
+  const int n = c.c1 - c.c0 + 1, head = c.kh * a.group + c.tile * HEADS + h;
+  auto part = [&](int i) { return a.parts + ((size_t)(c.c0 + i) * 2 + (i == 0)) * kPartFloats; };
+  for (int i = tid; i < n; i += kJoinThreads)
+    weight[i] = __ldcg(reinterpret_cast<const float2 *>(part(i) + HEADS * D + 2 * h));
+  __syncthreads();
+  float m = -INFINITY, l = 0.f;  // by every warp for itself
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, weight[i].x);
+#pragma unroll
+  for (int y = 16; y; y >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, y));
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int i = lane; i < n; i += 32) l += exp2_approx(weight[i].x - base) * weight[i].y;
+#pragma unroll
+  for (int y = 16; y; y >>= 1) l += __shfl_xor_sync(0xffffffffu, l, y);
+  constexpr int kGroups = kJoinThreads / (D / 4);
+  const int d = 4 * (tid % (D / 4)), group = tid / (D / 4);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = group; i0 < n; i0 += 4 * kGroups) {
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      x[u] = __ldcg(reinterpret_cast<const float4 *>(part(min(i0 + u * kGroups, n - 1)) + h * D + d));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kGroups;
+      add_scaled(sum, i < n ? exp2_approx(weight[min(i, n - 1)].x - base) : 0.f, x[u]);
+    }
+  }
+  sums[tid] = sum;
+  __syncthreads();
+  if (group > 0) return;
+  for (int i = 1; i < kGroups; ++i) add_scaled(sum, 1.f, sums[i * (D / 4) + tid]);
+  const float vs = a.v_scale != nullptr ? __ldg(a.v_scale + c.kh) : 1.f;
+  if (d < a.dim) store_out4<Io>(a, c.row, head, d, sum, vs / l);
+  if (tid == 0 && a.lse != nullptr) a.lse[(size_t)c.row * a.heads + head] = m * kLn2 + logf(l);
+}
+
 template <int D, int NT, bool F8, typename Io>
 int launch_attention(const AttnArgs &a, const CUtensorMap (&maps)[2], int grid, cudaStream_t s) {
   using S = Shape<D, NT, F8>;
@@ -906,8 +961,11 @@ int launch_attention(const AttnArgs &a, const CUtensorMap (&maps)[2], int grid, 
                                      (int)S::kSmem));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return launch_kernel(attention_kernel<D, NT, F8, Io>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, s, true,
-                       "attention_kernel", a, maps[0], maps[1]);
+  const int rc = launch_kernel(attention_kernel<D, NT, F8, Io>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, s,
+                               true, "attention_kernel", a, maps[0], maps[1]);
+  if (rc != CE_OK || a.crossings == nullptr) return rc;
+  return launch_kernel(join_kernel<D, S::kHeads, Io>, dim3((unsigned)grid, (unsigned)std::min(S::kHeads, a.group)),
+                       dim3(kJoinThreads), 0, s, true, "join_kernel", a);
 }
 
 template <bool F8, typename Io>
@@ -949,7 +1007,24 @@ int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer
   return r == CUDA_SUCCESS ? CE_OK : set_error(CE_ERR_CUDA, format("cuTensorMapEncodeTiled failed (%d)", (int)r));
 }
 
-size_t workspace_bytes_of(int grid) { return 4ull * kMaxGrid + (size_t)grid * 2 * kPartFloats * 4; }
+size_t workspace_bytes_of(int grid) {
+  return 4ull * kMaxGrid + (size_t)grid * (2 * kPartFloats * 4 + sizeof(Crossing));
+}
+
+// Whether the joins across CTAs are a launch of their own. One CTA reads the
+// parts of a request at about 40 bytes a cycle; where few requests share the
+// whole grid these are many. 30,000 tokens, 2 kv heads of 128, one request:
+// 16 query heads each (600 KB of parts a kv head) 41.5 us joined by the last
+// CTA, 20.6 with the launch; 4 heads (150 KB) 17.0 and 14.7; four requests
+// of 4,000 tokens, 2 kv heads of 96, 8 query heads each (55 KB) 15.8 and
+// 11.2. Below that the launch's 2 us of host time weigh more than the 0.5 to
+// 1 us of the device's that it saves (one request, 12 heads of 64, 3 KB: 8.7
+// and 8.2 us on the device, 6.8 and 9 on the host).
+bool join_apart(const AttnArgs &a, int grid) {
+  const long long items = (long long)a.seqs * a.kv_heads * a.tiles;
+  const long long bytes = grid / items * std::min(a.group, kMaxSplitHeads) * a.dim * 4;  // of a request's parts, at most
+  return bytes > 32 * 1024;
+}
 
 }  // namespace
 }  // namespace paged
@@ -1029,6 +1104,7 @@ int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pt
              pt->page_size, kv->kv_heads);
   a.arrivals = static_cast<int *>(workspace);
   a.parts = reinterpret_cast<float *>(a.arrivals + kMaxGrid);
+  a.crossings = join_apart(a, grid) ? reinterpret_cast<Crossing *>(a.parts + (size_t)grid * 2 * kPartFloats) : nullptr;
   const cudaStream_t s = (cudaStream_t)stream;
   if (kv->type == CE_TYPE_BF16) return dispatch_attention<false, __nv_bfloat16>(a, maps, grid, s);
   if (kv->type == CE_TYPE_F16) return dispatch_attention<false, __half>(a, maps, grid, s);
