@@ -1059,11 +1059,10 @@ def _dense(t, name, dtype, count=None):
 
 def _heads_of(t, name, tokens, heads, dim):
     """(pointer, token stride) of a [tokens][heads][dim] tensor whose heads are contiguous."""
-    if t.shape != (tokens, heads, dim) or not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor [{tokens}][{heads}][{dim}] (got {tuple(t.shape)})")
-    ld, sh, sd = t.stride()
-    if sd != 1 or (sh != dim and heads > 1):
-        raise ValueError(f"{name}: the heads of a token must be contiguous (strides {t.stride()})")
+    ld, sh, sd = st = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if sd != 1 or (sh != dim and heads > 1) or not t.is_cuda or t.shape != (tokens, heads, dim):
+        raise ValueError(f"{name} must be a device tensor [{tokens}][{heads}][{dim}] whose heads are contiguous within a "
+                         f"token (got {tuple(t.shape)}, strides {st})")
     return t.data_ptr(), ld if tokens > 1 else max(ld, heads * dim)
 
 
@@ -1139,22 +1138,31 @@ def paged_append(kv, q_out, q, k, v, slots, pos=None, rope=None, layer=0, stream
     """Rotary positions on q [tokens][heads][dim] and k, then k and v
     [tokens][kv_heads][dim] into their slots of `layer`; rope float32
     [positions][dim / 2][2] of (cos, sin), or None (ce_paged_append)."""
-    T, D = slots.numel(), kv.head_dim
-    kp, k_ld = _heads_of(k, "k", T, kv.kv_heads, D)
-    vp, v_ld = _heads_of(v, "v", T, kv.kv_heads, D)
-    qp, q_ld, qo, qt, heads = None, 0, None, TYPE_BF16, 0
+    T, D, Hk = slots.numel(), kv.head_dim, kv.kv_heads
+    kt = k.dtype
+    kp, k_ld = _heads_of(k, "k", T, Hk, D)
+    vp, v_ld = _heads_of(v, "v", T, Hk, D)
+    qp = qo = None
+    q_ld = heads = 0
+    qt = TYPE_BF16
     if q is not None:
         heads = q.shape[1]
         qp, q_ld = _heads_of(q, "q", T, heads, D)
-        qo, qt = _dense(q_out, "q_out", q_out.dtype, T * heads * D), _type(q_out, "q_out")
-    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+        qt = _type(q_out, "q_out")
+        qo = _dense(q_out, "q_out", q_out.dtype, T * heads * D)
+    if v.dtype is not kt or (q is not None and q.dtype is not kt):
         raise TypeError("q, k and v must have one dtype")
-    if rope is not None and (rope.dim() != 3 or rope.shape[1] * 2 != D or rope.shape[2] != 2):
-        raise ValueError(f"rope must be [positions][{D // 2}][2] (got {tuple(rope.shape)})")
-    check(_L.ce_paged_append(kv._p, layer, qo, qt, qp, kp, vp, _type(k, "k"), q_ld, k_ld, v_ld,
-                                _dense(slots, "slots", _I64), _dense(pos, "pos", _I32, T), T, heads,
-                                _dense(rope, "rope", _F32), 0 if rope is None else rope.shape[0],
-                                _stream_of(stream)))
+    rp, rope_len = None, 0
+    if rope is not None:
+        rope_len = rope.shape[0]
+        if rope.shape != (rope_len, D >> 1, 2):
+            raise ValueError(f"rope must be [positions][{D // 2}][2] (got {tuple(rope.shape)})")
+        rp = _dense(rope, "rope", _F32)
+    rc = _L.ce_paged_append(kv._p, layer, qo, qt, qp, kp, vp, _type(k, "k"), q_ld, k_ld, v_ld,
+                            _dense(slots, "slots", _I64), _dense(pos, "pos", _I32, T), T, heads, rp, rope_len,
+                            _raw_stream(_device()) if stream is None else _stream(stream))
+    if rc:
+        check(rc)
     return q_out
 
 
