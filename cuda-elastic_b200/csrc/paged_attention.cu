@@ -44,11 +44,11 @@
 //     keys, so the result does not depend on who is last.
 //
 // Measured (B200, measured copy rate 6.45 TB/s): 64 requests of 32 heads of
-// 128, 805 MB of bf16 keys and values, 127 us = 6.2 TB/s; six documents with
-// 8 kv heads of 128, 1.99 GB, 294 us = 6.8 TB/s; 96 requests over an E4M3
-// cache with 3 kv heads of 96, 123 MB, 40 us = 3.1 TB/s, where the bound is
+// 128, 782 MB of bf16 keys and values, 128 us = 6.1 TB/s; six documents with
+// 8 kv heads of 128, 1.99 GB, 297 us = 6.7 TB/s; 96 requests over an E4M3
+// cache with 3 kv heads of 96, 123 MB, 36.6 us = 3.4 TB/s, where the bound is
 // the chain of instructions per unit (two conversions per four cached bytes,
-// 43% of the issue slots used by 10 warps); one request of 512 tokens, 12
+// a third of the issue slots used by 10 warps); one request of 512 tokens, 12
 // heads of 64: 8.6 us, of which the lengths and pages take 2, the unit 1.5,
 // the joins 4.
 #include <algorithm>
@@ -1001,9 +1001,16 @@ int make_page_map(CUtensorMap *map, const ce_paged_kv *kv, void *pool, int layer
   const cuuint32_t box[4] = {(cuuint32_t)(128 / b), (cuuint32_t)std::min(unit_keys, kv->page_size), 1, 1};
   const cuuint32_t unit[4] = {1, 1, 1, 1};
   char *base = static_cast<char *>(pool) + (long long)layer * kv->layer_stride * b;
+  // Fetches widened to 256 bytes suit rows of whole 128-byte pieces, and rows
+  // of one head that follow one another; beside others they bring other heads'
+  // rows (3 heads of 96 bytes, token-major: 39.7 us with 256, 36.6 with 64; 32
+  // heads of 256 bytes: 127.9 and 128.4; 12 heads of 224 bytes, head-major:
+  // 112 and 117).
+  const bool apart = kv->head_dim * b % 128 != 0 && kv->token_stride != kv->head_dim;
+  const CUtensorMapL2promotion fetch = apart ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B;
   const CUresult r = fn(map, b == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims,
                         strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? CE_OK : set_error(CE_ERR_CUDA, format("cuTensorMapEncodeTiled failed (%d)", (int)r));
 }
 
