@@ -1063,7 +1063,7 @@ def _heads_of(t, name, tokens, heads, dim):
     if sd != 1 or (sh != dim and heads > 1) or not t.is_cuda or t.shape != (tokens, heads, dim):
         raise ValueError(f"{name} must be a device tensor [{tokens}][{heads}][{dim}] whose heads are contiguous within a "
                          f"token (got {tuple(t.shape)}, strides {st})")
-    return t.data_ptr(), ld if tokens > 1 else max(ld, heads * dim)
+    return t.data_ptr(), ld if tokens > 1 else heads * dim
 
 
 class PagedKV:

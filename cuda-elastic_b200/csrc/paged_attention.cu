@@ -49,7 +49,7 @@
 // cache with 3 kv heads of 96, 123 MB, 36.6 us = 3.4 TB/s, where the bound is
 // the chain of instructions per unit (two conversions per four cached bytes,
 // a third of the issue slots used by 10 warps); one request of 512 tokens, 12
-// heads of 64: 8.6 us, of which the lengths and pages take 2, the unit 1.5,
+// heads of 64: 8.7 us, of which the lengths and pages take 2, the unit 1.5,
 // the joins 4.
 #include <algorithm>
 #include <type_traits>

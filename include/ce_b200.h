@@ -916,8 +916,9 @@ int ce_paged_append(const ce_paged_kv *kv, int layer, void *q_out_dev, int q_out
                     const float *rope_dev, int rope_len, ce_stream_t stream);
 
 /* Bytes of ce_paged_attention's workspace on the current device. Zero it once
- * before the first call; every call leaves it ready for the next. Calls that
- * may run at the same time need a workspace each. */
+ * before the first call; every call leaves it ready for the next (but zero it
+ * again after a CE_ERR_TIMEOUT). Calls that may run at the same time need a
+ * workspace each. */
 int ce_paged_attention_workspace(size_t *bytes);
 
 /* Attention of one new token per request over its pages: for each of `heads`

@@ -576,3 +576,71 @@ def test_beam_histories_survive(ce, dev, cache, layout, page, dim):
         verify()
         grow([len(h) + 1 + (i // K == 2) for i, h in enumerate(histories)])
         verify()
+
+
+# ---------------------------------------------------------------------------
+# the Python side's refusals
+
+def test_wrappers_refuse_wrong_tensors(ce, dev):
+    rng = np.random.default_rng(11)
+    k, v = (pool(rng, dev, "bf16", 1, 6, 2, 16, 64, "hnd") for _ in "kv")
+    with pytest.raises(ValueError):
+        ce.PagedKV(k, v[:, :5])
+    with pytest.raises(ValueError):
+        ce.PagedKV(k.cpu(), v.cpu())
+    with pytest.raises(TypeError):
+        ce.PagedKV(k.double(), v.double())
+    with pytest.raises(ValueError):  # head rows apart
+        ce.PagedKV(k.transpose(3, 4), v.transpose(3, 4))
+    kv = ce.PagedKV(k, v)
+    pt = ce.PageTable.empty(3, 4, 6, 16)
+    with pytest.raises(TypeError):
+        ce.PageTable(pt.table.long(), pt.lens, pt.refs, 16)
+    with pytest.raises(ValueError):
+        ce.PageTable(pt.table, pt.lens[:2], pt.refs, 16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev)
+    out = torch.empty_like(q)
+    for bad in (q[:2], q[:, :, :32], q.transpose(0, 1), q.cpu()):
+        with pytest.raises(ValueError):
+            ce.paged_attention(kv, out, bad, pt)
+    with pytest.raises(TypeError):
+        ce.paged_attention(kv, out, q.half(), pt)
+    with pytest.raises(ce.CeError):  # f16 queries over a bf16 cache
+        ce.paged_attention(kv, out.half(), q.half(), pt)
+    with pytest.raises(ce.CeError):
+        ce.paged_attention(kv, out, q, pt, layer=1)
+    with pytest.raises(ValueError):
+        ce.paged_attention(kv, out, q, pt, lse=torch.empty(3, 3, device=dev))
+    slots, pos = torch.zeros(3, dtype=torch.int64, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    n = torch.zeros(3, 2, 64, device=dev)
+    with pytest.raises(TypeError):
+        ce.paged_append(kv, None, None, n, n.half(), slots, pos)
+    with pytest.raises(TypeError):
+        ce.paged_append(kv, None, None, n, n, slots.int(), pos)
+    with pytest.raises(ValueError):
+        ce.paged_append(kv, None, None, n, n, slots, pos, torch.zeros(4, 16, 2, device=dev))
+    with pytest.raises(ValueError):
+        ce.paged_append(kv, None, None, n[:2], n[:2], slots, pos)
+    with pytest.raises(TypeError):
+        ce.paged_resize(pt, torch.zeros(3, device=dev), slots, pos)
+    with pytest.raises(ValueError):
+        ce.paged_resize(pt, pos[:2], slots, pos)
+    with pytest.raises(ce.CeError, match="must differ"):
+        ce.paged_reorder(pt, pos, 3, pt)
+    ce.device_status()
+
+
+def test_one_row_with_any_stride(ce, dev):
+    """The stride between tokens means nothing where there is one."""
+    rng = np.random.default_rng(12)
+    k, v = (pool(rng, dev, "f16", 1, 2, 1, 16, 32, "hnd") for _ in "kv")
+    pt = ce.PageTable(torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.full((1,), 7, dtype=torch.int32, device=dev),
+                      torch.zeros(2, dtype=torch.int32, device=dev), 16)
+    q = torch.randn(2 * 32 * 3, device=dev).half()
+    a = q.as_strided((1, 2, 32), (33, 32, 1))
+    out, want = torch.empty(1, 2, 32, dtype=torch.float16, device=dev), torch.empty(1, 2, 32, dtype=torch.float16, device=dev)
+    kv = ce.PagedKV(k, v)
+    ce.paged_attention(kv, out, a, pt)
+    ce.paged_attention(kv, want, a.clone().contiguous(), pt)
+    ce.device_status()
+    assert torch.equal(out, want)
