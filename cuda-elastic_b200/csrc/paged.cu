@@ -536,18 +536,20 @@ struct AppendArgs {
   int tokens, heads, kv_heads, dim, shift, rope_len;
 };
 
-__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-  const float4 a = __ldcs(reinterpret_cast<const float4 *>(p));
-  const float4 b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
+// Eight elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
-  const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(p));
-  const T *e = reinterpret_cast<const T *>(&a);
+struct Row8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
-}
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+  }
+  __device__ __forceinline__ void widen(float (&x)[8]) const {
+    const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
+  }
+};
 
 __device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
   uint4 o;
@@ -571,72 +573,89 @@ __device__ __forceinline__ void store8(__nv_fp8_e4m3 *p, const float (&x)[8]) {
   *reinterpret_cast<uint2 *>(p) = o;
 }
 
-// One thread per 8 elements (4 rotary pairs) of a q, k or v head of a token,
-// in fp32, rounded once where it is stored. Blocks are (head_dim / 8, heads):
-// no index is divided, since the threads are many and short (with divided
-// indices and divisions by the scales 206 instructions a thread, and the
-// issue slots, not the memory, were the bound). Every element is read and
-// written once; a token's slot, position and rotary row are served from L1
-// to all its heads.
+// A thread has 8 elements (4 rotary pairs) at one place of up to Heads heads of
+// a token (q, k and v heads numbered one after the other), in fp32, rounded
+// once where they are stored. Blocks are (head_dim / 8, heads): no index is
+// divided and the scales are multiplied by their reciprocals, since the
+// threads are short and issue slots count beside the memory (206 instructions
+// a thread with the divisions, 159 without). The slot and the position are
+// fetched at once, behind the heads: one link less in the chain from the slot
+// to the rotary row is 42 -> 40 us at 8,190 tokens of 32 + 2 x 8 heads of 128,
+// bf16 into E4M3, and three heads for one look-up 34.6 us = 5.4 TB/s. Every
+// element is read and written once.
 constexpr int kAppendThreads = 256;
-template <typename In, typename Out, typename Cache>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+template <typename In, typename Out, typename Cache, int Heads>
+__global__ void __launch_bounds__(kAppendThreads, Heads == 1 ? 8 : 6) append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_launch_dependents();
-  int head = blockIdx.y * blockDim.y + threadIdx.y;  // q heads, then k heads, then v heads
-  if (head >= a.heads + 2 * a.kv_heads) return;
-  const int part = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : 2;
-  head -= part == 0 ? 0 : part == 1 ? a.heads : a.heads + a.kv_heads;
+  const int all = a.heads + 2 * a.kv_heads, step = gridDim.y * blockDim.y;
+  const int first = blockIdx.y * blockDim.y + threadIdx.y;
+  if (first >= all) return;
   const int d = 8 * threadIdx.x, tok = blockIdx.x;
-  const In *src = part == 0 ? static_cast<const In *>(a.q) + tok * a.q_ld
-                : part == 1 ? static_cast<const In *>(a.k) + tok * a.k_ld
-                            : static_cast<const In *>(a.v) + tok * a.v_ld;
+  const In *q = static_cast<const In *>(a.q) + tok * a.q_ld + d;
+  const In *k = static_cast<const In *>(a.k) + tok * a.k_ld + d;
+  const In *v = static_cast<const In *>(a.v) + tok * a.v_ld + d;
+  Out *q_out = static_cast<Out *>(a.q_out) + (long long)tok * a.heads * a.dim + d;
   pdl_wait();
-  float x[8];
-  load8(src + head * a.dim + d, x);  // on its way while the slot and position are looked up
+  Row8<In> in[Heads];
+#pragma unroll
+  for (int i = 0; i < Heads; ++i) {  // on their way while the slot and position are looked up
+    int h = first + i * step;
+    if (h >= all) break;
+    const In *src = h < a.heads ? q : h < a.heads + a.kv_heads ? k : v;
+    h -= h < a.heads ? 0 : h < a.heads + a.kv_heads ? a.heads : a.heads + a.kv_heads;
+    in[i].load(src + h * a.dim);
+  }
   const long long slot = a.slots[tok];
+  const int pos = a.rope != nullptr ? a.pos[tok] : 0;
   bool live = slot >= 0;
   if (live && slot >= a.slot_end) {
     report_timeout(&g_paged_status, kSiteSlot);
     live = false;
   }
-  int pos = 0;
-  if (live && a.rope != nullptr) {
-    pos = a.pos[tok];
-    if (pos < 0 || pos >= a.rope_len) {
-      report_timeout(&g_paged_status, kSitePos);
-      live = false;
-    }
+  if (live && a.rope != nullptr && (pos < 0 || pos >= a.rope_len)) {
+    report_timeout(&g_paged_status, kSitePos);
+    live = false;
   }
   if (!live) {
-    if (part == 0) {
-      const float zero[8] = {};
-      store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, zero);
-    }
+    const float zero[8] = {};
+    for (int h = first; h < a.heads; h += step) store8(q_out + h * a.dim, zero);
     return;
   }
-  if (part < 2 && a.rope != nullptr) {
+  float4 c[2] = {{1, 0, 1, 0}, {1, 0, 1, 0}};  // (cos, sin) of four pairs
+  if (a.rope != nullptr) {
     const float4 *cs = reinterpret_cast<const float4 *>(a.rope + (long long)pos * a.dim + d);
+    c[0] = __ldg(cs), c[1] = __ldg(cs + 1);
+  }
+  const long long at = (slot >> a.shift) * a.page_stride + (slot & ((1ll << a.shift) - 1)) * a.token_stride + d;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {  // two pairs per 16 bytes of (cos, sin)
-      const float4 c = __ldg(cs + i);
-      const float x0 = x[4 * i], x1 = x[4 * i + 1], x2 = x[4 * i + 2], x3 = x[4 * i + 3];
-      x[4 * i] = x0 * c.x - x1 * c.y, x[4 * i + 1] = x0 * c.y + x1 * c.x;
-      x[4 * i + 2] = x2 * c.z - x3 * c.w, x[4 * i + 3] = x2 * c.w + x3 * c.z;
+  for (int i = 0; i < Heads; ++i) {
+    int h = first + i * step;
+    if (h >= all) break;
+    float x[8];
+    in[i].widen(x);
+    if (h < a.heads + a.kv_heads && a.rope != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float x0 = x[4 * j], x1 = x[4 * j + 1], x2 = x[4 * j + 2], x3 = x[4 * j + 3];
+        x[4 * j] = x0 * c[j].x - x1 * c[j].y, x[4 * j + 1] = x0 * c[j].y + x1 * c[j].x;
+        x[4 * j + 2] = x2 * c[j].z - x3 * c[j].w, x[4 * j + 3] = x2 * c[j].w + x3 * c[j].z;
+      }
     }
-  }
-  if (part == 0) {
-    store8(static_cast<Out *>(a.q_out) + ((long long)tok * a.heads + head) * a.dim + d, x);
-    return;
-  }
-  const float *scale = part == 1 ? a.k_scale : a.v_scale;
-  if (scale != nullptr) {
-    const float inv = 1.f / __ldg(scale + head);
+    if (h < a.heads) {
+      store8(q_out + h * a.dim, x);
+      continue;
+    }
+    h -= a.heads;
+    const bool is_v = h >= a.kv_heads;
+    if (is_v) h -= a.kv_heads;
+    const float *scale = is_v ? a.v_scale : a.k_scale;
+    if (scale != nullptr) {
+      const float inv = 1.f / __ldg(scale + h);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= inv;
+      for (int j = 0; j < 8; ++j) x[j] *= inv;
+    }
+    store8(reinterpret_cast<Cache *>(is_v ? a.vc : a.kc) + at + h * a.head_stride, x);
   }
-  Cache *base = reinterpret_cast<Cache *>(part == 1 ? a.kc : a.vc);
-  store8(base + (slot >> a.shift) * a.page_stride + head * a.head_stride +
-             (slot & ((1ll << a.shift) - 1)) * a.token_stride + d, x);
 }
 
 // Launches one cluster of `ranks` CTAs (a table kernel).
@@ -709,13 +728,28 @@ Tables tables_of(const ce_page_table *to, const ce_page_table *from, int32_t *st
           from->seqs, from->max_pages, from->pages, log2_of(from->page_size)};
 }
 
+// Three heads a thread where 16-bit rows fill more than two waves of CTAs
+// three times over (4,096 tokens of 32 + 2 x 32 heads of 128: 40.6 us with one
+// head, 36.0 with three; 256 tokens: 3.4 and 3.7). Fp32 rows have as many bytes
+// in flight with one (48.2 and 48.9 us), and fewer than three heads to a
+// thread leave lanes idle (4,096 tokens of 28 + 2 x 4 heads of 96: 13.2, 14.3).
+template <typename In, typename Out, typename Cache>
+int launch_append(const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
+  if constexpr (sizeof(In) == 2) {
+    constexpr long long kWave = 148 * (2048 / kAppendThreads);
+    if (grid.y >= 3 && (long long)grid.x * grid.y > 2 * kWave) {
+      grid.y = (grid.y + 2) / 3;
+      return launch_kernel(append_kernel<In, Out, Cache, 3>, grid, block, 0, s, true, "append_kernel", a);
+    }
+  }
+  return launch_kernel(append_kernel<In, Out, Cache, 1>, grid, block, 0, s, true, "append_kernel", a);
+}
+
 template <typename In, typename Out>
 int launch_append(int cache_type, const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
-  if (cache_type == CE_TYPE_BF16)
-    return launch_kernel(append_kernel<In, Out, __nv_bfloat16>, grid, block, 0, s, true, "append_kernel", a);
-  if (cache_type == CE_TYPE_F16)
-    return launch_kernel(append_kernel<In, Out, __half>, grid, block, 0, s, true, "append_kernel", a);
-  return launch_kernel(append_kernel<In, Out, __nv_fp8_e4m3>, grid, block, 0, s, true, "append_kernel", a);
+  if (cache_type == CE_TYPE_BF16) return launch_append<In, Out, __nv_bfloat16>(a, grid, block, s);
+  if (cache_type == CE_TYPE_F16) return launch_append<In, Out, __half>(a, grid, block, s);
+  return launch_append<In, Out, __nv_fp8_e4m3>(a, grid, block, s);
 }
 
 template <typename In>

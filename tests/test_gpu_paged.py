@@ -293,8 +293,21 @@ def test_attention_offsets_past_32_bits(ce, dev):
 @pytest.mark.parametrize("cache,out", [("bf16", "bf16"), ("f16", "f16"), ("e4m3", "f16"), ("bf16", "f16")])
 @pytest.mark.parametrize("dim,heads,kv_heads,layout", [(64, 6, 3, "hnd"), (16, 1, 1, "nhd"), (128, 8, 1, "nhd")])
 def test_append(ce, dev, io, cache, out, dim, heads, kv_heads, layout):
+    check_append(ce, dev, io, cache, out, dim, heads, kv_heads, layout, 37, 9)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cache,out", [("bf16", "bf16"), ("f16", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("dim,heads,kv_heads,layout", [(128, 33, 8, "hnd"), (80, 40, 11, "nhd"), (128, 46, 1, "nhd")])
+def test_append_of_many_tokens(ce, dev, io, cache, out, dim, heads, kv_heads, layout):
+    """Enough tokens and heads for a thread to take several heads, with and
+    without a remainder."""
+    check_append(ce, dev, io, cache, out, dim, heads, kv_heads, layout, 901, 115)
+
+
+def check_append(ce, dev, io, cache, out, dim, heads, kv_heads, layout, T, pages):
     rng = np.random.default_rng(dim + heads)
-    T, page, pages, layers = 37, 8, 9, 2
+    page, layers = 8, 2
     k, v = (pool(rng, dev, cache, layers, pages, kv_heads, page, dim, layout) for _ in "kv")
     before = [host(x) for x in (k, v)]
     qkv = torch.from_numpy(rng.standard_normal((T, (heads + 2 * kv_heads) * dim)).astype(np.float32) * 3).to(dev).to(DT[io])
