@@ -38,8 +38,11 @@ constexpr int kMaxGroups = 16384;  // batch elements: arrival counters at the fr
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kElems = 16;         // logits per thread and tile
-constexpr int kFirst = 1024;       // candidates of the first tile
-constexpr int kLater = 768;        // of the later ones
+// Epochs of a slice: the first tile, then 2, 4, 8, 16, 32 tiles, then the rest.
+constexpr int kEpochs = 7;
+constexpr int kFirst = 512;        // candidates of the first epoch
+constexpr int kLater = 256;        // of each later one
+constexpr int kKept = 512;         // candidates that are ranked
 constexpr int kListKeys = 256;     // keys of one beam's lists at the join: slices x beams
 
 struct BeamArgs {
@@ -98,6 +101,21 @@ __device__ __forceinline__ float warp_sorted(float v) {
   return v;
 }
 
+// The 32 largest of two lists, in descending order of lanes: `a` in that order,
+// `b` in the opposite one. Their lane maxima are those 32, first rising, then
+// falling or a turn of it, which five steps sort.
+template <typename T>
+__device__ __forceinline__ T warp_merged(T a, T b) {
+  const int lane = threadIdx.x & 31;
+  T v = a > b ? a : b;
+#pragma unroll
+  for (int step = 16; step; step >>= 1) {
+    const T y = __shfl_xor_sync(0xffffffffu, v, step);
+    v = (lane & step ? y < v : y > v) ? y : v;
+  }
+  return v;
+}
+
 // Joins (max, sum of e^(x - max)) pairs.
 __device__ __forceinline__ void add_sum(float &m, float &l, float m1, float l1) {
   if (m1 > m) {
@@ -115,12 +133,15 @@ struct Shared {
   float2 kth[kWarps];
   float2 sums[kWarps];
   unsigned long long round[kWarps];
-  float score[kMaxBeams][kMaxBeams];  // [beam][rank]
-  int token[kMaxBeams][kMaxBeams];
-  int first, later, passed, last;  // candidates; warps past the first tile
+  unsigned long long kept[kKept];  // candidates not below the last bar; at the join 32 per warp
+  int token[kMaxBeams][kMaxBeams];  // [beam][rank]
+  int count[kEpochs], passed[kEpochs];  // candidates; warps past the epoch
+  int keep, last;
+  float best[32];                  // of the epochs that all warps have passed, sorted
   float bar;                       // what a later tile's candidates exceed
 };
-static_assert(kFirst + kLater + 2 * kMaxBeams <= kWarps * kListKeys, "candidates and what follows them");
+static_assert(kFirst + (kEpochs - 1) * kLater == kWarps * kListKeys && kFirst >= 3 * kMaxBeams, "candidates by epochs");
+static_assert(kKept >= 32 * kWarps, "a list per warp");
 static_assert(kElems == 16, "four tops of four");
 
 // The `beams` best keys of the slice's tokens [t0, t1) by taking the best that
@@ -151,37 +172,36 @@ __device__ __noinline__ void take_in_rounds(Shared &sh, const T *x, int t0, int 
   __syncthreads();
 }
 
-// The `beams` best of the candidates, buffer[0, n0) and buffer[kFirst, kFirst
-// + n1), in order, by their ranks among all; 0 past the last.
-__device__ __forceinline__ void rank_candidates(Shared &sh, int n0, int n1, int beams) {
+__device__ __forceinline__ int epoch_start(int epoch) { return epoch == 0 ? 0 : kFirst + (epoch - 1) * kLater; }
+__device__ __forceinline__ int epoch_size(int epoch) { return epoch == 0 ? kFirst : kLater; }
+
+// The `beams` best of n keys, in order, by their ranks among all; 0 past the last.
+__device__ __forceinline__ void rank_candidates(Shared &sh, const unsigned long long *keys, int n, int beams) {
   if ((int)threadIdx.x < beams) sh.top[threadIdx.x] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < n0 + n1; i += kThreads) {
-    const unsigned long long k = sh.buffer[i < n0 ? i : kFirst + i - n0];
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long k = keys[i];
     int rank = 0;
-    for (int q = 0; q < n0; ++q) rank += sh.buffer[q] > k;
-    for (int q = kFirst; q < kFirst + n1; ++q) rank += sh.buffer[q] > k;
+    for (int q = 0; q < n; ++q) rank += keys[q] > k;
     if (rank < beams) sh.top[rank] = k;
   }
   __syncthreads();
 }
 
-// By one warp: the beams-th best logit of the first tile's n candidates (no
-// bar if there are fewer).
-__device__ __forceinline__ float later_bar(const Shared &sh, int n, int beams) {
-  unsigned long long last = ~0ull;
-  if (n < beams) return -INFINITY;
-  for (int r = 0; r < beams; ++r) {
-    unsigned long long k = 0;
-    for (int i = threadIdx.x & 31; i < n; i += 32) {
-      const unsigned long long c = sh.buffer[i];
-      k = c < last && c > k ? c : k;
-    }
-    const uint32_t hi = (uint32_t)(k >> 32), top = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t low = __reduce_max_sync(0xffffffffu, hi == top ? (uint32_t)k : 0u);
-    last = (unsigned long long)top << 32 | low;
+// By one warp, when all have passed an epoch: takes its candidates into the 32
+// best logits so far and returns the beams-th (-inf if there are fewer).
+__device__ __forceinline__ float later_bar(Shared &sh, int epoch, int beams) {
+  const int lane = threadIdx.x & 31, n = *(volatile int *)&sh.count[epoch];
+  if (n > epoch_size(epoch)) return INFINITY;  // too many: the rounds decide
+  float best = epoch == 0 ? -INFINITY : *(volatile float *)&sh.best[lane];
+  for (int i = lane; i - lane < n; i += 32) {
+    const float v = i < n ? key_logit(sh.buffer[epoch_start(epoch) + i]) : -INFINITY;
+    const float least = __shfl_sync(0xffffffffu, best, 31);
+    if (!__any_sync(0xffffffffu, v > least)) continue;
+    best = warp_merged(best, __shfl_sync(0xffffffffu, warp_sorted(v), 31 - lane));
   }
-  return key_logit(last);
+  *(volatile float *)&sh.best[lane] = best;
+  return __shfl_sync(0xffffffffu, best, beams - 1);
 }
 
 // The largest float below a finite x (so that y > it means y >= x).
@@ -234,7 +254,8 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
   if (!(open >> beam & 1)) return false;
   float ex = extra >= 0 ? logit_of(x[extra]) : -INFINITY;
   float m = ex, l = ex > -INFINITY ? 1.f : 0.f;
-  if (tid == 0) sh.first = sh.later = sh.passed = 0, sh.bar = -INFINITY;
+  if (tid < kEpochs) sh.count[tid] = sh.passed[tid] = 0;
+  if (tid == 0) sh.keep = 0, sh.bar = -INFINITY;
   float bar = -INFINITY;
   const int tiles = max(1, (v1 - v0 + kTile - 1) / kTile);
   for (int tile = 0; tile < tiles; ++tile) {
@@ -293,9 +314,10 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
     } else {
       bar = fmaxf(bar, *(volatile float *)&sh.bar);
     }
-    auto offer = [&](bool first, float y, int token) {
-      const int n = atomicAdd(first ? &sh.first : &sh.later, 1);
-      if (n < (first ? kFirst : kLater)) sh.buffer[(first ? 0 : kFirst) + n] = key_of(y, token);
+    const int epoch = min(31 - __clz(tile + 1), kEpochs - 1);
+    auto offer = [&](int to, float y, int token) {
+      const int n = atomicAdd(&sh.count[to], 1);
+      if (n < epoch_size(to)) sh.buffer[epoch_start(to) + n] = key_of(y, token);
     };
     if (top > bar) {
 #pragma unroll
@@ -303,49 +325,64 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
         if (tops[i / 4] > bar) {
 #pragma unroll
           for (int y = i; y < i + 4; ++y)
-            if (e[y] > bar) offer(tile == 0, e[y], head + (at + y / kPerVec * kThreads) * kPerVec + y % kPerVec);
+            if (e[y] > bar) offer(epoch, e[y], head + (at + y / kPerVec * kThreads) * kPerVec + y % kPerVec);
         }
     }
-    // the row's last elements, behind all tiles by their tokens, count with the later ones
-    if (tile == 0 && ex > bar) offer(extra < head, ex, extra);
-    if (tile == 0 && tiles > 1) {
-      // The last warp to have offered its part of the first tile takes the
-      // K-th best of these as the later tiles' bar; nobody waits for it. (An
-      // equal value of a later token is no better.)
+    // the row's last elements, behind all tiles by their tokens, count with the last epoch
+    if (tile == 0 && ex > bar) offer(extra < head ? 0 : kEpochs - 1, ex, extra);
+    if (tile + 1 < tiles && epoch < kEpochs - 1 && tile == (2 << epoch) - 2) {
+      // The last warp to have offered its part of the epoch takes the K-th
+      // best so far as the later tiles' bar; nobody waits for it. (An equal
+      // value of a later token is no better.) So each epoch, with as many
+      // tiles as all before it, has about K candidates.
       __syncwarp();
       int passed = 0;
       if (lane == 0) {
         __threadfence_block();
-        passed = atomicAdd(&sh.passed, 1);
+        passed = atomicAdd(&sh.passed[epoch], 1);
         __threadfence_block();
       }
       passed = __shfl_sync(0xffffffffu, passed, 0);
       __syncwarp();
       if (passed == kWarps - 1) {
-        const int n = *(volatile int *)&sh.first;
-        const float kth = n > kFirst ? INFINITY : later_bar(sh, n, K);  // too many: the rounds below decide
+        const float kth = later_bar(sh, epoch, K);
         if (lane == 0) *(volatile float *)&sh.bar = kth;
       }
     }
   }
   __syncthreads();
   const int t0 = slice == 0 ? 0 : head + v0 * kPerVec, t1 = slice == a.slices - 1 ? a.vocab : head + v1 * kPerVec;
-  int n0 = sh.first;
-  const int n1 = sh.later;
-  if (n0 > kFirst || n1 > kLater) {
-    take_in_rounds(sh, x, t0, t1, K);
-  } else {
-    if (n0 + n1 < K) {
-      // Fewer than K values are finite: tokens of logit -inf follow, the
-      // lowest first. K of them, or all, stand among the first 2 K tokens.
-      __syncthreads();
-      if (tid < min(2 * K, t1 - t0) && logit_of(x[t0 + tid]) == -INFINITY)
-        sh.buffer[atomicAdd(&sh.first, 1)] = key_of(-INFINITY, t0 + tid);
-      __syncthreads();
-      n0 = sh.first;
-    }
-    rank_candidates(sh, n0, n1, K);
+  int n = 0, first = sh.count[0];
+  bool over = false;
+#pragma unroll
+  for (int i = 0; i < kEpochs; ++i) n += sh.count[i], over |= sh.count[i] > epoch_size(i);
+  if (!over && n < K) {
+    // Fewer than K values are finite: tokens of logit -inf follow, the
+    // lowest first. K of them, or all, stand among the first 2 K tokens.
+    __syncthreads();
+    if (tid < min(2 * K, t1 - t0) && logit_of(x[t0 + tid]) == -INFINITY)
+      sh.buffer[atomicAdd(&sh.count[0], 1)] = key_of(-INFINITY, t0 + tid);
+    __syncthreads();
+    n += sh.count[0] - first;
+    first = sh.count[0];
   }
+  const unsigned long long *keys = sh.buffer;
+  if (!over && n > first) {  // those that reach the last bar, together
+    const float least = sh.bar;
+#pragma unroll 1
+    for (int i = 0; i < kEpochs; ++i)
+      for (int c = tid; c < sh.count[i]; c += kThreads) {
+        const unsigned long long k = sh.buffer[epoch_start(i) + c];
+        if (key_logit(k) >= least) {
+          const int to = atomicAdd(&sh.keep, 1);
+          if (to < kKept) sh.kept[to] = k;
+        }
+      }
+    __syncthreads();
+    keys = sh.kept, n = sh.keep, over = n > kKept;
+  }
+  if (over) take_in_rounds(sh, x, t0, t1, K);
+  else rank_candidates(sh, keys, n, K);
 #pragma unroll
   for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
   if (lane == 0) sh.sums[warp] = make_float2(m, l);
@@ -367,16 +404,17 @@ __device__ __forceinline__ bool warp_best(unsigned long long k) {
   return hi == top && lo == low && k != 0;
 }
 
-// The offers of one beam, best first, from the sorted lists of its slices.
-__device__ __forceinline__ int offers_of_row(const BeamArgs &a, Shared &sh, int group, int beam) {
+// The offers of one beam, best first by lanes, from the sorted lists of its
+// slices: keys of score, beam and rank; 0 past the last.
+__device__ __forceinline__ unsigned long long offers_of_row(const BeamArgs &a, Shared &sh, int group, int beam) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.beams;
   const size_t row = (size_t)group * K + beam;
   const float base = a.scores[row];
   if (a.finished[row]) {
-    if (lane == 0) sh.score[beam][0] = base != base ? -INFINITY : base, sh.token[beam][0] = a.pad;
-    return 1;
+    if (lane == 0) sh.token[beam][0] = a.pad;
+    return lane == 0 ? key_of(base != base ? -INFINITY : base, beam * 32) : 0ull;
   }
-  unsigned long long *lists = sh.buffer + warp * kListKeys;
+  unsigned long long *lists = sh.buffer + warp * kListKeys, top;
   for (int i = lane; i < a.slices * K; i += 32) lists[i] = __ldcg(a.best + row * a.slices * K + i);
   float m = -INFINITY, l = 0.f;
   if (lane < a.slices) {
@@ -387,19 +425,26 @@ __device__ __forceinline__ int offers_of_row(const BeamArgs &a, Shared &sh, int 
   for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
   const float lse = m + logf(l);
   __syncwarp();
-  int at = 0, r = 0;
-  const int n = min(K, a.vocab);
-  for (; r < n; ++r) {
-    const unsigned long long k = lane < a.slices && at < K ? lists[lane * K + at] : 0ull;
-    if (warp_best(k)) {
-      const float x = key_logit(k);
-      const float s = x == -INFINITY ? -INFINITY : base + (x - lse);
-      sh.score[beam][r] = s != s ? -INFINITY : s;
-      sh.token[beam][r] = key_token(k);
-      ++at;
+  if (K <= 2 * (a.slices - 1)) {  // fewer ranks than lists: a lane per slice, the best of their heads once per rank
+    unsigned long long *taken = sh.kept + warp * 32;
+    taken[lane] = 0;
+    __syncwarp();
+    int at = 0;
+    for (int r = 0; r < min(K, a.vocab); ++r) {
+      const unsigned long long k = lane < a.slices && at < K ? lists[lane * K + at] : 0ull;
+      if (warp_best(k)) taken[r] = k, ++at;
     }
+    __syncwarp();
+    top = taken[lane];
+  } else {
+    top = lane < K ? lists[lane] : 0ull;
+    for (int i = 1; i < a.slices; ++i) top = warp_merged(top, 31 - lane < K ? lists[i * K + 31 - lane] : 0ull);
   }
-  return n;
+  __syncwarp();  // before the lists of the next beam
+  if (lane >= K || top == 0) return 0ull;
+  const float x = key_logit(top), s = x == -INFINITY ? -INFINITY : base + (x - lse);
+  sh.token[beam][lane] = key_token(top);
+  return key_of(s != s ? -INFINITY : s, beam * 32 + lane);
 }
 
 // Grid (slices, beams, batch). Finished beams have no logits to read: their
@@ -423,26 +468,28 @@ __global__ void __launch_bounds__(kThreads, 4) select_kernel(const __grid_consta
   } else if (open != 0 || blockIdx.x + blockIdx.y != 0) {
     return;
   }
+  // Keys order by score, beam and rank: ties go to the lowest beam.
+  unsigned long long best = 0;
   for (int beam = warp; beam < K; beam += kWarps) {
-    offers_of_row(a, sh, group, beam);
-    __syncwarp();
+    const unsigned long long k = offers_of_row(a, sh, group, beam);
+    best = beam == warp ? k : warp_merged(best, __shfl_sync(0xffffffffu, k, 31 - lane));
   }
-  __syncthreads();
+  for (int half = kWarps / 2; half; half >>= 1) {
+    if (K <= half) continue;
+    if (warp >= half && warp < 2 * half) sh.kept[warp * 32 + lane] = best;
+    __syncthreads();
+    if (warp < half) best = warp_merged(best, sh.kept[(warp + half) * 32 + 31 - lane]);
+  }
   if (warp != 0) return;
-  const int offers = lane >= K ? 0 : a.finished[group * K + lane] ? 1 : min(K, a.vocab);
-  int at = 0;
-  for (int r = 0; r < K; ++r) {
-    const float s = at < offers ? sh.score[lane][at] : 0.f;
-    // ties go to the lowest beam
-    if (warp_best(at < offers ? key_of(s + 0.f, lane) : 0ull)) {
-      const size_t to = (size_t)group * K + r;
-      const int token = sh.token[lane][at];
-      a.scores_out[to] = s;
-      a.parents[to] = lane;
-      a.tokens[to] = token;
-      a.finished_out[to] = a.finished[group * K + lane] != 0 || token == a.eos;
-      ++at;
-    }
+  __syncwarp();
+  if (lane < K) {  // every beam has an offer
+    const int beam = key_token(best) >> 5 & (kMaxBeams - 1), token = sh.token[beam][key_token(best) & 31];
+    const size_t to = (size_t)group * K + lane;
+    const bool over = a.finished[group * K + beam] != 0 || token == a.eos;
+    a.scores_out[to] = key_logit(best);
+    a.parents[to] = beam;
+    a.tokens[to] = token;
+    a.finished_out[to] = over;
   }
 }
 
