@@ -6,23 +6,27 @@
 // in tiles held in registers, and keeps a running (max, sum) per thread and
 // the slice's `beams` best keys. A tile's candidates are found by a threshold
 // that is a lower bound of its beams-th best value: for the first tile from
-// the sorted lane maxima of the warps, later the first tile's beams-th best
-// (without that step, with some 17 candidates
-// a tile in the place of 8 / tile, 64 x 8 beams take 31 us in the place of
-// 22). They are collected without a barrier, and at the end their ranks
-// (counted, each against all) put them in order. Keys are (logit, token)
-// pairs as 64-bit integers, all different, so the order is total and
-// independent of the order in which threads append.
+// the sorted lane maxima of the warps, later the beams-th best of the tiles
+// so far, taken again whenever their number has doubled. (Without that step,
+// with some 17 candidates a tile in the place of 8 / tile, 64 x 8 beams take
+// 31 us in the place of 21; with it once, after the first tile, 32 x 16 beams
+// over 95,351 take 157 us in the place of 45, for their candidates no longer
+// fit.) They are collected without a barrier. At the end those that reach the
+// last bar are put in order by their ranks, counted, each against all. Keys
+// are (logit, token) pairs as 64-bit integers, all different, so the order is
+// total and independent of the order in which threads append.
 //
-// The last CTA of a batch element to arrive joins the slices: a warp per
-// beam plays the sorted lists of its slices off against one another (a lane
-// per slice), then one warp does the same with the beams' sorted offers.
+// The last CTA of a batch element to arrive joins the slices: a warp takes a
+// beam, whose slices' sorted lists are merged by shuffles (up to eight beams:
+// a lane per slice, the best of their heads once per rank, since there may be
+// 32 lists), and merges it with its other beams' offers; then the warps'.
+// (Once per rank throughout: 1 x 32 beams over 4,096 tokens 26 us, merged 11.)
 //
-// Measured (B200): 4 beams over 32,000 fp32 logits 6.1 us; 64 x 8 beams 23 us
-// = 2.9 TB/s of the 65.5 MB: a row's CTA spends half its time outside the
-// tiles (threshold, ranks, arrival and join, about 13,000 cycles), and with
+// Measured (B200): 4 beams over 32,000 fp32 logits 6.2 us; 64 x 8 beams 21.4
+// us = 3.1 TB/s of the 65.5 MB; 32 x 32 beams 51 us: a row's CTA spends half
+// its time outside the tiles (threshold, ranks, arrival and join), and with
 // three or four rows on an SM that is not all hidden. More slices only
-// multiply it (two 24 us, four 32 us).
+// multiply it (two 24 us, four 32 us), loads two tiles ahead change nothing.
 #include <float.h>
 
 #include <algorithm>
@@ -41,7 +45,7 @@ constexpr int kElems = 16;         // logits per thread and tile
 // Epochs of a slice: the first tile, then 2, 4, 8, 16, 32 tiles, then the rest.
 constexpr int kEpochs = 7;
 constexpr int kFirst = 512;        // candidates of the first epoch
-constexpr int kLater = 256;        // of each later one
+constexpr int kLater = 640;        // of each later one: warps may run eight tiles ahead of a bar
 constexpr int kKept = 512;         // candidates that are ranked
 constexpr int kListKeys = 256;     // keys of one beam's lists at the join: slices x beams
 
@@ -128,7 +132,7 @@ __device__ __forceinline__ void add_sum(float &m, float &l, float m1, float l1) 
 }
 
 struct Shared {
-  unsigned long long buffer[kWarps * kListKeys];  // candidates; at the join the lists, per warp
+  unsigned long long buffer[kFirst + (kEpochs - 1) * kLater];  // candidates; at the join the lists, per warp
   unsigned long long top[kMaxBeams];
   float2 kth[kWarps];
   float2 sums[kWarps];
@@ -140,7 +144,7 @@ struct Shared {
   float best[32];                  // of the epochs that all warps have passed, sorted
   float bar;                       // what a later tile's candidates exceed
 };
-static_assert(kFirst + (kEpochs - 1) * kLater == kWarps * kListKeys && kFirst >= 3 * kMaxBeams, "candidates by epochs");
+static_assert(kFirst + (kEpochs - 1) * kLater >= kWarps * kListKeys && kFirst >= 3 * kMaxBeams, "the lists of the join");
 static_assert(kKept >= 32 * kWarps, "a list per warp");
 static_assert(kElems == 16, "four tops of four");
 
@@ -425,7 +429,7 @@ __device__ __forceinline__ unsigned long long offers_of_row(const BeamArgs &a, S
   for (int o = 16; o; o >>= 1) add_sum(m, l, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, l, o));
   const float lse = m + logf(l);
   __syncwarp();
-  if (K <= 2 * (a.slices - 1)) {  // fewer ranks than lists: a lane per slice, the best of their heads once per rank
+  if (K <= 8 && a.slices > 1) {  // few ranks, up to 32 lists: a lane per slice, the best of their heads once per rank
     unsigned long long *taken = sh.kept + warp * 32;
     taken[lane] = 0;
     __syncwarp();
@@ -437,8 +441,21 @@ __device__ __forceinline__ unsigned long long offers_of_row(const BeamArgs &a, S
     __syncwarp();
     top = taken[lane];
   } else {
-    top = lane < K ? lists[lane] : 0ull;
-    for (int i = 1; i < a.slices; ++i) top = warp_merged(top, 31 - lane < K ? lists[i * K + 31 - lane] : 0ull);
+    unsigned long long t[8];  // the odd ones in the opposite order
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = i % 2 ? 31 - lane : lane;
+      t[i] = i < a.slices && at < K ? lists[i * K + at] : 0ull;
+    }
+#pragma unroll
+    for (int step = 1; step < 8; step *= 2)  // merges of a round side by side
+      if (step < a.slices)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2 * step) {
+          t[i] = warp_merged(t[i], t[i + step]);
+          if (i / (2 * step) % 2) t[i] = __shfl_sync(0xffffffffu, t[i], 31 - lane);
+        }
+    top = t[0];
   }
   __syncwarp();  // before the lists of the next beam
   if (lane >= K || top == 0) return 0ull;
@@ -496,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 4) select_kernel(const __grid_consta
 // Slices of a row: enough CTAs for about three on every SM, no slice below one
 // tile of a CTA, and lists that fit the join.
 int slices_of(int rows, int beams, int vocab, int sms) {
-  const int most = std::min({32, kListKeys / beams, (vocab + kThreads * kElems - 1) / (kThreads * kElems)});
+  const int most = std::min({beams <= 8 ? 32 : 8, kListKeys / beams, (vocab + kThreads * kElems - 1) / (kThreads * kElems)});
   return std::max(1, std::min(most, (3 * sms + rows - 1) / rows));
 }
 

@@ -70,6 +70,42 @@ def test_ties_across_tiles_of_long_rows(ce, dev):
     check(run(ce, dev, x, scores, finished), R.beam_select(x.float().cpu().numpy(), scores, finished, 2, 0), V)
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("B,K,V", [(3, 16, 50001), (2, 24, 128256), (1, 32, 95351), (4, 9, 70003), (32, 32, 20011)])
+def test_many_beams(ce, dev, io, B, K, V):
+    """Rows of several slices, and slices of several tiles, with many offers."""
+    rng = np.random.default_rng(V)
+    logits = torch.from_numpy(rng.standard_normal((B * K, V)).astype(np.float32) * 2.5).to(dev).to(DT[io])
+    logits[1::5, ::3] = logits[1::5, 1:2]  # a third of the row equal
+    scores = (-20 * rng.random((B, K))).astype(np.float32)
+    finished = rng.random((B, K)) < 0.2
+    got = run(ce, dev, logits, scores, finished)
+    check(got, R.beam_select(logits.float().cpu().numpy(), scores, finished, 2, 0), V)
+
+
+def test_very_long_rows_of_one_cta(ce, dev):
+    """So many rows that each is one CTA's, 74 tiles long: random, with ties,
+    ascending, descending. The other rows are finished and not read. (A sum is
+    one of at most 74 + 16 + 13 additions in sequence: 2^-17.3 of it.)"""
+    rng = np.random.default_rng(3)
+    B, K, V = 56, 8, 300001
+    x = torch.empty(B * K, V, dtype=torch.bfloat16, device=dev)
+    finished = np.ones((B, K), bool)
+    finished[[0, 55]] = False
+    rows = np.flatnonzero(finished.ravel() == 0)
+    part = (rng.standard_normal((len(rows), V)) * 2).astype(np.float32)
+    part[2] = np.linspace(-9, 9, V)
+    part[3] = part[2, ::-1]
+    part[4, [7, 5000, 13000, 29000, 60000, 130000, 270000, V - 1]] = 12
+    part[5, 257 * 1000:] += 6
+    x[torch.from_numpy(rows).to(dev)] = torch.from_numpy(part).to(dev).to(torch.bfloat16)
+    scores = -rng.random((B, K)).astype(np.float32)
+    got = run(ce, dev, x, scores, finished)
+    part = torch.from_numpy(part).to(torch.bfloat16).float().numpy()
+    check([g[[0, 55]] for g in got], R.beam_select(part, scores[[0, 55]], finished[[0, 55]], 2, 0), V)
+    assert (got[2][1:55] == 0).all() and got[3][1:55].all()
+
+
 @pytest.mark.parametrize("V", [50, 9000])
 def test_infinities_and_nan(ce, dev, V):
     """Banned (-inf) and NaN logits are never taken before a finite one; a row
