@@ -1057,6 +1057,13 @@ def _dense(t, name, dtype, count=None):
     return t.data_ptr()
 
 
+def _workspace(t):
+    """(pointer, bytes) of a workspace: a contiguous device tensor of any type."""
+    if not t.is_cuda or not t.is_contiguous():
+        raise TypeError(f"workspace must be a contiguous device tensor (got {t.device}, strides {t.stride()})")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
 def _heads_of(t, name, tokens, heads, dim):
     """(pointer, token stride) of a [tokens][heads][dim] tensor whose heads are contiguous."""
     ld, sh, sd = st = t.stride() if t.dim() == 3 else (0, 0, 0)
@@ -1184,10 +1191,10 @@ def paged_attention(kv, out, q, pt, lse=None, scale=None, layer=0, workspace=Non
     op, o_ld = _heads_of(out, "out", n, heads, D)
     if q.dtype != out.dtype:
         raise TypeError("q and out must have one dtype")
-    ws = kv.workspace() if workspace is None else workspace
+    ws, ws_bytes = _workspace(kv.workspace() if workspace is None else workspace)
     check(_L.ce_paged_attention(kv._p, layer, pt._p, op, _dense(lse, "lse", _F32, n * heads), qp,
                                    _type(q, "q"), heads, q_ld, o_ld, D ** -0.5 if scale is None else scale,
-                                   ws.data_ptr(), ws.numel(), _stream_of(stream)))
+                                   ws, ws_bytes, _stream_of(stream)))
     return out
 
 
@@ -1210,13 +1217,14 @@ def beam_select(scores_out, parents, tokens, finished_out, logits, scores, finis
     n, V = B * K, logits.shape[1]
     if logits.dim() != 2 or logits.shape[0] != n or not logits.is_cuda or (V > 1 and logits.stride(1) != 1):
         raise ValueError(f"logits must be a device tensor [{n}][vocab] with contiguous rows (got {tuple(logits.shape)})")
+    ws, ws_bytes = _workspace(workspace)
     check(_L.ce_beam_select(_dense(scores_out, "scores_out", _F32, n),
                                _dense(parents, "parents", _I32, n), _dense(tokens, "tokens", _I32, n),
                                _dense(finished_out, "finished_out", _BOOL, n), logits.data_ptr(),
                                _type(logits, "logits"), logits.stride(0) if n > 1 else max(V, logits.stride(0)),
                                _dense(scores, "scores", _F32),
-                               _dense(finished, "finished", _BOOL, n), B, K, V, eos, pad, workspace.data_ptr(),
-                               workspace.numel(), _stream_of(stream)))
+                               _dense(finished, "finished", _BOOL, n), B, K, V, eos, pad, ws, ws_bytes,
+                               _stream_of(stream)))
 
 
 def paged_reorder(pt, parents, beams, out, kv=None, copies=None, status=None, stream=None):

@@ -172,3 +172,13 @@ def test_select_repeats_bit_for_bit_and_in_a_graph(ce, dev):
     torch.cuda.synchronize()
     for a, b in zip(first, o):
         assert np.array_equal(a, b.cpu().numpy())
+
+
+def test_select_refuses_a_workspace_that_is_not_on_the_device(ce, dev):
+    """Before any launch: the kernel would follow the host pointer."""
+    x = torch.zeros(2, 50, device=dev)
+    scores, finished = np.zeros((1, 2), np.float32), np.zeros((1, 2), bool)
+    ws = ce.beam_workspace(1, 2, 50)
+    for bad in (ws.cpu(), torch.zeros(2 * ws.numel(), dtype=torch.uint8, device=dev)[::2]):
+        with pytest.raises(TypeError, match="workspace"):
+            run(ce, dev, x, scores, finished, ws=bad)

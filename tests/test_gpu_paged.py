@@ -657,3 +657,21 @@ def test_one_row_with_any_stride(ce, dev):
     ce.paged_attention(kv, want, a.clone().contiguous(), pt)
     ce.device_status()
     assert torch.equal(out, want)
+
+
+def test_attention_refuses_a_workspace_that_is_not_on_the_device(ce, dev):
+    """Before any launch: the kernels would follow the host pointer."""
+    rng = np.random.default_rng(13)
+    k, v = (pool(rng, dev, "bf16", 1, 2, 1, 16, 32, "hnd") for _ in "kv")
+    kv, pt = ce.PagedKV(k, v), ce.PageTable.empty(1, 1, 2, 16)
+    q = torch.zeros(1, 1, 32, dtype=torch.bfloat16, device=dev)
+    ws = ce.paged_attention_workspace()
+    for bad in (ws.cpu(), torch.zeros(2 * ws.numel(), dtype=torch.uint8, device=dev)[::2]):
+        with pytest.raises(TypeError, match="workspace"):
+            ce.paged_attention(kv, torch.empty_like(q), q, pt, workspace=bad)
+    with pytest.raises(ce.CeError, match="workspace"):
+        ce.paged_attention(kv, torch.empty_like(q), q, pt, workspace=ws[:-16])
+    out = torch.full_like(q, float("nan"))
+    ce.paged_attention(kv, out, q, pt, workspace=ws.view(torch.int32))  # bytes count, not elements
+    ce.device_status()
+    assert (out == 0).all()
