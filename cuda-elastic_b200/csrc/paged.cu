@@ -26,6 +26,7 @@ namespace {
 __device__ DeviceStatus g_paged_status;
 
 constexpr int kTableThreads = 1024;
+constexpr int kMaxCapacity = 0x7fffffff - 127;  // new tokens of a resize, numbered by ints a warp's 128 at a time
 
 // ---------------------------------------------------------------------------
 // Pieces that resize and reorder share
@@ -829,6 +830,7 @@ int ce_paged_resize(const ce_page_table *to, const ce_page_table *from, const in
   CE_REQUIRE(new_lens != nullptr, "null new lengths");
   CE_REQUIRE(capacity >= 0 && (capacity == 0 || (slots != nullptr && pos != nullptr)),
              "slots and pos are required for a capacity of %d", capacity);
+  CE_REQUIRE(capacity <= kMaxCapacity, "capacity must be at most %d (got %d)", kMaxCapacity, capacity);
   rc = configure_tables();
   if (rc != CE_OK) return rc;
   const int ranks = resize_ranks(from, capacity);

@@ -891,6 +891,7 @@ typedef struct ce_page_table {
  * or when the free pages or the capacity do not suffice for it and those
  * before it; from the first that does not suffice on, all are refused.
  * status[0..3] = pages taken, requests refused, pages still free, new tokens.
+ * capacity is at most 2^31 - 128.
  *
  * `to` and `from` describe the same rows and pages; each of their buffers may
  * be the same one (in place) or another. */

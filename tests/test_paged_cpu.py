@@ -165,3 +165,11 @@ def test_oracle_beam_search_finds_the_best_sequences():
                   reverse=True)[:K]
     assert [h for _, h in best] == hist
     assert np.allclose([s for s, _ in best], scores[0], atol=1e-5)
+
+
+def test_resize_refuses_a_capacity_whose_numbers_would_overflow(ce):
+    """A warp numbers 128 tokens at once: from 2^31 - 127 on the last ones
+    would be negative and index before the outputs."""
+    f = ce.lib().ce_paged_resize
+    for capacity in (2 ** 31 - 127, 2 ** 31 - 1):
+        refused(ce, f(pt(ce), pt(ce), PTR, PTR, PTR, capacity, None, None, None), "capacity")
