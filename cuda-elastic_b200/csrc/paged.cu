@@ -852,6 +852,10 @@ int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const i
                "the cache has %d pages of %d, the block table %d of %d", kv->pages, kv->page_size, from->pages,
                from->page_size);
   }
+  // 16-byte pieces of a page's tokens in one layer, at most
+  const long long most =
+      kv != nullptr ? (kv->page_size - 1ll) * kv->kv_heads * (kv->head_dim * type_bytes(kv->type) / 16) : 0;
+  CE_REQUIRE(most < (1ll << 30), "a page of a layer is too large (%d tokens, %d heads)", kv->page_size, kv->kv_heads);
   rc = configure_tables();
   if (rc != CE_OK) return rc;
   const cudaStream_t s = (cudaStream_t)stream;
@@ -864,8 +868,6 @@ int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const i
                       kv->layer_stride * b, kv->page_stride * b, kv->head_stride * b, kv->token_stride * b,
                       from->seqs, kv->layers, kv->kv_heads, kv->head_dim * b / 16, kv->page_size};
   const long long pairs = (long long)from->seqs * kv->layers, ctas = 8ll * sm_count();
-  const long long most = (kv->page_size - 1ll) * c.kv_heads * c.pieces;  // pieces of a pair
-  CE_REQUIRE(most < (1ll << 30), "a page of a layer is too large (%d tokens, %d heads)", kv->page_size, kv->kv_heads);
   const unsigned x = (unsigned)std::min(pairs, ctas);
   const unsigned y = (unsigned)std::max(1ll, std::min(ctas / x, most / (4 * kCopyThreads)));
   return launch_kernel(copy_pages_kernel, dim3(x, y), dim3(kCopyThreads), 0, s, true, "copy_pages_kernel", c);

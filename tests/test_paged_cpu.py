@@ -173,3 +173,13 @@ def test_resize_refuses_a_capacity_whose_numbers_would_overflow(ce):
     f = ce.lib().ce_paged_resize
     for capacity in (2 ** 31 - 127, 2 ** 31 - 1):
         refused(ce, f(pt(ce), pt(ce), PTR, PTR, PTR, capacity, None, None, None), "capacity")
+
+
+def test_reorder_refuses_too_large_a_page_before_any_launch(ce):
+    """1,023 tokens of 2^18 heads are more 16-byte pieces than the copy counts;
+    the tables must not have changed by then."""
+    table = dict(page_size=1024, max_pages=5)
+    other = ce._PageTableStruct(PTR + 256, PTR, PTR, 8, 5, 10, 1024)
+    cache = kv(ce, page_size=1024, kv_heads=1 << 18, head_stride=65536, page_stride=1 << 34, layer_stride=1 << 35)
+    refused(ce, ce.lib().ce_paged_reorder(ctypes.byref(other), pt(ce, **table), PTR, 4, cache, PTR, None, None),
+            "too large")
