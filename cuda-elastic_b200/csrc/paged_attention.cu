@@ -205,8 +205,11 @@ __device__ __forceinline__ int row_len(const AttnArgs &a, int b) {
   return len;
 }
 
+// (unsigned: lengths go up to 2^31 - 1)
 template <int UNIT>
-__device__ __forceinline__ int slots_of(int len) { return len > 0 ? (len + UNIT - 1) / UNIT + 1 : 0; }
+__device__ __forceinline__ int units_of(int len) { return (int)(((unsigned)len + UNIT - 1) / UNIT); }
+template <int UNIT>
+__device__ __forceinline__ int slots_of(int len) { return len > 0 ? units_of<UNIT>(len) + 1 : 0; }
 
 // A place on the line of units. Requests of length 0 have none.
 template <int UNIT>
@@ -220,7 +223,7 @@ struct Cursor {
       }
       len = row_len(a, row);
     } while (len == 0);
-    units = (len + UNIT - 1) / UNIT;
+    units = units_of<UNIT>(len);
   }
   __device__ __forceinline__ void step(const AttnArgs &a) {
     if (++k < units) return;
@@ -369,7 +372,7 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
         before += slots_of<kUnit>(at.len);
       }
     }
-    at.units = max(1, (at.len + kUnit - 1) / kUnit);
+    at.units = max(1, units_of<kUnit>(at.len));
     const uint32_t in = slot - before * (uint32_t)passes, each = (uint32_t)at.units + 1;
     const int pass = (int)min((uint32_t)passes - 1, in / each);
     at.kh = pass / a.tiles, at.tile = pass % a.tiles;
@@ -390,10 +393,10 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
     auto look_up = [&] {
       left = 0;
       if (to_look <= 0) return;
-      const int key = look.k * kUnit + sub;
+      const unsigned key = (unsigned)look.k * kUnit + sub;
       left = look.len - look.k * kUnit;
       head = look.kh;
-      token = key & mask;
+      token = (int)(key & mask);
       page = sub < min(left, kUnit) ? __ldg(pages + (key >> a.shift)) : 0;
       to_look -= look.k + 1 == look.units ? 2 : 1;  // the unit's slot, and that of the change to the next request
       if (to_look <= 0) return;

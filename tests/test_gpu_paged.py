@@ -675,3 +675,27 @@ def test_attention_refuses_a_workspace_that_is_not_on_the_device(ce, dev):
     ce.paged_attention(kv, out, q, pt, workspace=ws.view(torch.int32))  # bytes count, not elements
     ce.device_status()
     assert (out == 0).all()
+
+
+def test_attention_of_the_longest_row(ce, dev):
+    """2^31 - 16 tokens, as many as 16-token pages allow: one page 2^27 - 1
+    times over, so that its 16 tokens weigh as they would alone and the log
+    sum is larger by log(2^27 - 1). A warp (12 on each SM at this head size)
+    adds at most ceil(2^26 / (12 SMs)) units, of two halves in two 16-bit
+    parts each, one after the other, every sum off by at most 2^-23 of it."""
+    page, columns = 16, 2 ** 27 - 1
+    rng = np.random.default_rng(14)
+    k, v = (pool(rng, dev, "bf16", 1, 1, 1, page, 16, "hnd") for _ in "kv")
+    pt = ce.PageTable(torch.zeros(1, columns, dtype=torch.int32, device=dev),
+                      torch.tensor([columns * page], dtype=torch.int32, device=dev),
+                      torch.ones(1, dtype=torch.int32, device=dev), page)
+    q = torch.from_numpy(rng.standard_normal((1, 2, 16)).astype(np.float32)).to(dev).to(torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty(1, 2, device=dev)
+    ce.paged_attention(ce.PagedKV(k, v), out, q, pt, lse=lse)
+    ce.device_status()
+    want, wlse, _, spread = R.attention(host(q), host(k[0]), host(v[0]), np.zeros((1, 1), np.int32), [page], page, 0.25)
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
+    rel = 4 * -(-2 ** 26 // (12 * sms)) * 2.0 ** -23
+    assert rel < 0.02
+    assert (np.abs(host(out) - want) <= 2 * rel * spread + UNIT["bf16"] * np.abs(want)).all()
+    assert (np.abs(host(lse) - wlse - np.log(columns)) <= 2 * rel).all()
