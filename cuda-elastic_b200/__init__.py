@@ -1077,10 +1077,11 @@ class PagedKV:
     """Pools of keys and values: k, v device tensors
     [layers][pages][kv_heads][page_size][head_dim] of bfloat16, float16 or
     float8_e4m3fn with the same strides (token-major pages are a permuted
-    view); k_scale, v_scale float32 [kv_heads] for an 8-bit cache. Holds the
-    attention workspace: calls of paged_attention on one PagedKV must be
-    ordered (one stream), or pass a workspace of their own
-    (paged_attention_workspace)."""
+    view); k_scale, v_scale float32 [kv_heads] for an 8-bit cache. Holds an
+    attention workspace, ready for any stream once the object is made: calls
+    of paged_attention on one PagedKV must be ordered (one stream after the
+    other), or pass a workspace of their own (paged_attention_workspace). An
+    object made during a graph capture holds none: its attention needs one."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if _L is None:
@@ -1097,11 +1098,12 @@ class PagedKV:
                                  _dense(v_scale, "v_scale", _F32, H), _type(k, "cache"), L, P, H, S, D,
                                  st[0], st[1], st[2], st[3])
         self._p = ctypes.addressof(self._c)
-        self._ws = None
+        self._ws = None if _capturing() else paged_attention_workspace(k.device)
 
     def workspace(self):
         if self._ws is None:
-            self._ws = paged_attention_workspace(self.k.device)
+            raise RuntimeError("this PagedKV was made during a graph capture, where no workspace can be zeroed for later "
+                               "calls: make it before, or pass workspace=")
         return self._ws
 
 
@@ -1173,12 +1175,27 @@ def paged_append(kv, q_out, q, k, v, slots, pos=None, rope=None, layer=0, stream
     return q_out
 
 
+def _capturing():
+    import torch
+    return torch.cuda.is_current_stream_capturing()
+
+
+def _zeroed(nbytes, device):
+    """A workspace that any stream may use at once: the zeros have been written
+    on return. (During a capture they are the graph's: written by its every
+    replay, and there alone.)"""
+    import torch
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    if not _capturing():
+        torch.cuda.current_stream(ws.device).synchronize()
+    return ws
+
+
 def paged_attention_workspace(device="cuda"):
     """A zeroed workspace (uint8 device tensor) of paged_attention."""
-    import torch
     n = ctypes.c_size_t()
     check(lib().ce_paged_attention_workspace(ctypes.byref(n)))
-    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+    return _zeroed(n.value, device)
 
 
 def paged_attention(kv, out, q, pt, lse=None, scale=None, layer=0, workspace=None, stream=None):
@@ -1200,10 +1217,9 @@ def paged_attention(kv, out, q, pt, lse=None, scale=None, layer=0, workspace=Non
 
 def beam_workspace(batch, beams, vocab, device="cuda"):
     """A zeroed workspace (uint8 device tensor) of beam_select."""
-    import torch
     n = ctypes.c_size_t()
     check(lib().ce_beam_workspace(batch, beams, vocab, ctypes.byref(n)))
-    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+    return _zeroed(n.value, device)
 
 
 def beam_select(scores_out, parents, tokens, finished_out, logits, scores, finished, eos, pad, workspace, stream=None):

@@ -699,3 +699,83 @@ def test_attention_of_the_longest_row(ce, dev):
     assert rel < 0.02
     assert (np.abs(host(out) - want) <= 2 * rel * spread + UNIT["bf16"] * np.abs(want)).all()
     assert (np.abs(host(lse) - wlse - np.log(columns)) <= 2 * rel).all()
+
+
+def first_attention(ce, dev):
+    """A cache that no call has used, its answer by another object, and a call on it."""
+    lens = [6000, 31, 0, 90]  # the first row is split over CTAs: it needs the workspace's counters
+    out, *_, (kv, pt, q) = attention_case(ce, dev, 15, lens, 2, 4, 64, 16, "bf16", "bf16", "hnd")
+    return out, pt, q, kv.k, kv.v
+
+
+def keep_busy(dev):
+    """Work of some 50 ms at least on the current stream."""
+    x = torch.randn(8192, 8192, device=dev)
+    for _ in range(5):
+        x = x @ x * 1e-4
+    return x
+
+
+def test_a_first_call_on_another_stream(ce, dev):
+    """The workspace is zeroed before a stream other than the current one,
+    which is busy, uses it: the attention's and the beam selection's."""
+    want, pt, q, k, v = first_attention(ce, dev)
+    # what the workspaces will be made from is not zero: one block of each size, among others of the size
+    sizes = [x.numel() for x in (ce.paged_attention_workspace(), ce.beam_workspace(1, 2, 128256))]
+    dirt = [[torch.full((n,), 0x55, dtype=torch.uint8, device=dev) for _ in range(65)] for n in sizes]
+    side = torch.cuda.Stream()
+    other = torch.full_like(want, float("nan"))
+    x, scores = torch.randn(2, 128256, device=dev), torch.zeros(1, 2, device=dev)
+    done = torch.zeros(1, 2, dtype=torch.bool, device=dev)
+
+    def select(ws, **stream):
+        o = [torch.full((1, 2), -7, dtype=t, device=dev) for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+        torch.cuda.synchronize()
+        return lambda: ce.beam_select(*o[:3], o[3].view(torch.bool), x, scores, done, -1, 0, ws(), **stream) or o
+
+    best = select(lambda: ce.beam_workspace(1, 2, 128256))()
+    go = select(lambda: ce.beam_workspace(1, 2, 128256), stream=side)
+    busy = keep_busy(dev)
+    torch.cuda.synchronize()
+    for blocks in dirt:
+        del blocks[32]
+    busy = keep_busy(dev)
+    ce.paged_attention(ce.PagedKV(k, v), other, q, pt, stream=side)
+    busy = keep_busy(dev)
+    got = go()
+    side.synchronize()
+    assert torch.equal(other, want)
+    assert all(torch.equal(a, b) for a, b in zip(got, best))
+    ce.device_status()
+
+
+def test_a_captured_first_call_and_an_eager_one_before_its_replay(ce, dev):
+    want, pt, q, k, v = first_attention(ce, dev)
+    kv = ce.PagedKV(k, v)
+    a, b = torch.full_like(want, float("nan")), torch.full_like(want, float("nan"))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ce.paged_attention(kv, a, q, pt)
+    at = kv.workspace().data_ptr()  # not of the graph's memory, which only a replay would zero
+    pools = [x["segment_pool_id"] for x in torch.cuda.memory_snapshot() if x["address"] <= at < x["address"] + x["total_size"]]
+    assert pools == [(0, 0)]
+    ce.paged_attention(kv, b, q, pt)
+    assert torch.equal(b, want)
+    for _ in range(2):
+        a.fill_(float("nan"))
+        g.replay()
+        assert torch.equal(a, want)
+    ce.device_status()
+
+
+def test_a_cache_made_during_a_capture_has_no_workspace(ce, dev):
+    want, pt, q, k, v = first_attention(ce, dev)
+    out, ws = torch.full_like(want, float("nan")), ce.paged_attention_workspace()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv = ce.PagedKV(k, v)
+        with pytest.raises(RuntimeError, match="capture"):
+            ce.paged_attention(kv, out, q, pt)
+        ce.paged_attention(kv, out, q, pt, workspace=ws)
+    g.replay()
+    assert torch.equal(out, want)
