@@ -133,12 +133,15 @@ class PagedLlama:
         return self._gemm(self._norm(x, w["rms_final"]), w["wcls"])
 
     def prefill(self, prompts, rows):
-        """Writes the prompts (lists of tokens) into the cache rows `rows`; the
-        last token's logits of each. Every prompt token attends as a row of
-        its own, with the block table of its prompt and the length up to it."""
+        """Writes the prompts (lists of tokens) into the cache rows `rows`,
+        whose old sequences end; the last token's logits of each. Every prompt
+        token attends as a row of its own, with the block table of its prompt
+        and the length up to it."""
         dev = self.rope.device
         lens = [len(p) for p in prompts]
         new = torch.full((self.rows,), -1, dtype=torch.int32)
+        new[torch.tensor(rows)] = 0
+        self.grow(new.to(dev), 0)
         new[torch.tensor(rows)] = torch.tensor(lens, dtype=torch.int32)
         order = sorted(range(len(rows)), key=lambda i: rows[i])  # tokens are numbered row by row
         tokens = torch.tensor([t for i in order for t in prompts[i]], device=dev)
@@ -153,10 +156,12 @@ class PagedLlama:
 
     def beam_search(self, prompts, beams, steps, eos=2, pad=0):
         """Generates `steps` tokens for every prompt: (sequences int32
-        [batch][beams][steps], log probabilities [batch][beams]), best first."""
+        [batch][beams][steps], log probabilities [batch][beams]), best first.
+        What the cache held before ends; the new sequences stay in it."""
         ce, dev, B = self.ce, self.rope.device, len(prompts)
         if B * beams != self.rows:
             raise ValueError(f"{B} prompts x {beams} beams need a cache of {B * beams} rows (has {self.rows})")
+        self.release()
         logits = self.prefill(prompts, list(range(0, self.rows, beams))).repeat_interleave(beams, 0)
         scores = torch.full((B, beams), float("-inf"), device=dev)
         scores[:, 0] = 0.0  # the other beams part from the first

@@ -194,3 +194,41 @@ def test_a_pool_too_small_is_reported(pb, dev):
     m = pb.PagedLlama(CFG, w, 4, 64, pages=3, page_size=8)
     with pytest.raises(RuntimeError, match="pool is too small"):
         m.beam_search([[1, 2, 3, 4, 5]], 4, 12, eos=-1)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_searches_one_after_the_other_on_one_model(pb, dev, cache):
+    """Each as on a model of its own, whatever the cache still holds: after
+    longer, shorter and equally long sequences, in a pool with room for one
+    search only."""
+    w = pb.PagedLlama.random_weights(CFG, 7, std=0.08)
+    rng = np.random.default_rng(7)
+    K, page, top = 3, 8, 48
+
+    def model():
+        return pb.PagedLlama(CFG, w, 2 * K, top, pages=2 * K * (top // page), page_size=page, cache=cache)
+
+    m = model()
+    for lengths, steps in (((5, 12), 6), ((3, 2), 20), ((40, 33), 8), ((40, 33), 8), ((23, 4), 3)):
+        prompts = [rng.integers(0, 512, n).tolist() for n in lengths]
+        out, scores = m.beam_search(prompts, K, steps, eos=-1)
+        want, wscores = model().beam_search(prompts, K, steps, eos=-1)
+        assert torch.equal(out, want) and torch.equal(scores, wscores)
+        assert m.pt.lens.tolist() == [n + steps - 1 for n in lengths for _ in range(K)]
+
+
+def test_prompts_into_rows_that_hold_a_sequence(pb, dev):
+    """A longer, a shorter and an equally long one; the row between keeps its own."""
+    w = pb.PagedLlama.random_weights(CFG, 8, std=0.08)
+    rng = np.random.default_rng(8)
+    m, fresh = (pb.PagedLlama(CFG, w, 4, 64, page_size=8) for _ in range(2))
+    m.prefill([rng.integers(0, 512, n).tolist() for n in (10, 30, 9, 21)], [0, 1, 2, 3])
+    kept = cached(m, 2)
+    prompts = [rng.integers(0, 512, n).tolist() for n in (24, 7, 21)]
+    got, want = m.prefill(prompts, [0, 1, 3]), fresh.prefill(prompts, [0, 1, 3])
+    m.ce.device_status()
+    assert torch.equal(got, want) and m.pt.lens.tolist() == [24, 7, 9, 21]
+    assert all(torch.equal(a, b) for a, b in zip(kept, cached(m, 2)))
+    for r in (0, 1, 3):
+        assert all(torch.equal(a, b) for a, b in zip(cached(m, r), cached(fresh, r)))
+    assert int(m.refused) == 0 and int(m.pt.refs.sum()) == 3 + 1 + 2 + 3
