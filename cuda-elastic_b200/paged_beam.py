@@ -162,6 +162,7 @@ class PagedLlama:
         if B * beams != self.rows:
             raise ValueError(f"{B} prompts x {beams} beams need a cache of {B * beams} rows (has {self.rows})")
         self.release()
+        self.refused.zero_()
         logits = self.prefill(prompts, list(range(0, self.rows, beams))).repeat_interleave(beams, 0)
         scores = torch.full((B, beams), float("-inf"), device=dev)
         scores[:, 0] = 0.0  # the other beams part from the first

@@ -232,3 +232,13 @@ def test_prompts_into_rows_that_hold_a_sequence(pb, dev):
     for r in (0, 1, 3):
         assert all(torch.equal(a, b) for a, b in zip(cached(m, r), cached(fresh, r)))
     assert int(m.refused) == 0 and int(m.pt.refs.sum()) == 3 + 1 + 2 + 3
+
+
+def test_a_search_after_one_that_found_no_page(pb, dev):
+    w = pb.PagedLlama.random_weights(CFG, 6)
+    m = pb.PagedLlama(CFG, w, 4, 64, pages=6, page_size=8)
+    with pytest.raises(RuntimeError, match="pool is too small"):
+        m.beam_search([[1, 2, 3, 4, 5]], 4, 30, eos=-1)
+    out, scores = m.beam_search([[1, 2, 3]], 4, 5, eos=-1)
+    want, wscores = pb.PagedLlama(CFG, w, 4, 64, page_size=8).beam_search([[1, 2, 3]], 4, 5, eos=-1)
+    assert torch.equal(out, want) and torch.equal(scores, wscores)
