@@ -46,7 +46,7 @@ class PagedLlama:
     sequences of at most max_len tokens in `pages` pages."""
 
     def __init__(self, cfg, weights, rows, max_len, pages=None, page_size=16, cache="bf16", device="cuda"):
-        self.ce, self.cfg, self.rows = _ce(), cfg, rows
+        self.ce, self.cfg, self.rows, self.max_len = _ce(), cfg, rows, max_len
         ce = self.ce
         D, H, L = cfg["dim"], cfg["n_heads"], cfg["n_layers"]
         self.hs, self.heads, self.kv_heads, self.layers = D // H, H, cfg["n_kv_heads"], L
@@ -139,6 +139,12 @@ class PagedLlama:
         and the length up to it."""
         dev = self.rope.device
         lens = [len(p) for p in prompts]
+        if not prompts or len(rows) != len(prompts) or len(set(rows)) != len(rows) or not all(0 <= r < self.rows for r in rows):
+            raise ValueError(f"prompts need a row each of 0 .. {self.rows - 1} (got {len(prompts)} for rows {list(rows)})")
+        if not all(0 < n <= self.max_len for n in lens):
+            raise ValueError(f"prompts must have 1 .. {self.max_len} tokens (got {lens})")
+        if not all(0 <= t < self.cfg["vocab_size"] for p in prompts for t in p):
+            raise ValueError(f"prompt tokens must be in 0 .. {self.cfg['vocab_size'] - 1}")
         new = torch.full((self.rows,), -1, dtype=torch.int32)
         new[torch.tensor(rows)] = 0
         self.grow(new.to(dev), 0)
@@ -158,9 +164,11 @@ class PagedLlama:
         """Generates `steps` tokens for every prompt: (sequences int32
         [batch][beams][steps], log probabilities [batch][beams]), best first.
         What the cache held before ends; the new sequences stay in it."""
-        ce, dev, B = self.ce, self.rope.device, len(prompts)
+        ce, dev, B, V = self.ce, self.rope.device, len(prompts), self.cfg["vocab_size"]
         if B * beams != self.rows:
             raise ValueError(f"{B} prompts x {beams} beams need a cache of {B * beams} rows (has {self.rows})")
+        if not -V <= pad < V:  # a finished beam's next tokens, looked up in the embedding like any
+            raise ValueError(f"pad must be a token of the vocabulary of {V} (got {pad})")
         self.release()
         self.refused.zero_()
         logits = self.prefill(prompts, list(range(0, self.rows, beams))).repeat_interleave(beams, 0)
@@ -169,7 +177,7 @@ class PagedLlama:
         finished = torch.zeros(B, beams, dtype=torch.bool, device=dev)
         scores2, finished2 = torch.empty_like(scores), torch.empty_like(finished)
         parents, tokens = (torch.empty(B, beams, dtype=torch.int32, device=dev) for _ in "pt")
-        ws = ce.beam_workspace(B, beams, self.cfg["vocab_size"], dev)
+        ws = ce.beam_workspace(B, beams, V, dev)
         out = torch.empty(B, beams, 0, dtype=torch.int32, device=dev)
         for step in range(steps):
             ce.beam_select(scores2, parents, tokens, finished2, logits, scores, finished, eos, pad, ws)

@@ -242,3 +242,21 @@ def test_a_search_after_one_that_found_no_page(pb, dev):
     out, scores = m.beam_search([[1, 2, 3]], 4, 5, eos=-1)
     want, wscores = pb.PagedLlama(CFG, w, 4, 64, page_size=8).beam_search([[1, 2, 3]], 4, 5, eos=-1)
     assert torch.equal(out, want) and torch.equal(scores, wscores)
+
+
+def test_prompts_that_cannot_be_read_are_refused(pb, dev):
+    """Before any device work: an empty prompt has no last token, a token past
+    the vocabulary would be looked up outside the embedding."""
+    m = pb.PagedLlama(CFG, pb.PagedLlama.random_weights(CFG, 9), 2, 20, page_size=8)
+    m.prefill([[4, 5, 6]], [1])
+    for prompts, rows, word in (([[1], []], [0, 1], "1 .. 20"), ([[1] * 21], [0], "1 .. 20"), ([], [], "a row each"),
+                                ([[1], [2]], [0], "a row each"), ([[1], [2]], [0, 0], "a row each"),
+                                ([[1]], [2], "a row each"), ([[1]], [-1], "a row each"), ([[1, 512]], [0], "tokens"),
+                                ([[-1]], [0], "tokens")):
+        with pytest.raises(ValueError, match=word):
+            m.prefill(prompts, rows)
+    with pytest.raises(ValueError, match="pad"):
+        m.beam_search([[1], [2]], 1, 3, pad=512)
+    assert m.pt.lens.tolist() == [0, 3]
+    out, _ = m.beam_search([[1], [2]], 1, 3, pad=-1)
+    assert out.shape == (2, 1, 3)
