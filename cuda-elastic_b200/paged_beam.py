@@ -39,6 +39,7 @@ def _ce():
 
 
 NAMES = ("wqkv", "wo", "w13", "w2")
+TABLE_ROWS = 8192  # rows of a block table at most
 
 
 class PagedLlama:
@@ -153,12 +154,16 @@ class PagedLlama:
         tokens = torch.tensor([t for i in order for t in prompts[i]], device=dev)
         slots, pos = self.grow(new.to(dev), tokens.numel())
         owner = torch.tensor([rows[i] for i in order for _ in prompts[i]], device=dev)
-        pt = self.ce.PageTable(self.pt.table[owner].contiguous(), pos + 1, self.pt.refs, self.pt.page_size)
-        logits = self.forward(tokens, slots, pos, pt)
-        last = torch.tensor(np.cumsum([lens[i] for i in order]) - 1, device=dev)
+        last = np.cumsum([lens[i] for i in order]) - 1  # the tokens whose logits are wanted
+        logits = []
+        for a in range(0, tokens.numel(), TABLE_ROWS):
+            part = slice(a, a + TABLE_ROWS)
+            pt = self.ce.PageTable(self.pt.table[owner[part]].contiguous(), pos[part] + 1, self.pt.refs, self.pt.page_size)
+            wanted = torch.tensor(last[(last >= a) & (last < part.stop)] - a, device=dev)
+            logits.append(self.forward(tokens[part], slots[part], pos[part], pt)[wanted])
         back = torch.empty(len(rows), dtype=torch.long, device=dev)
-        back[torch.tensor(order, device=dev)] = last
-        return logits[back]
+        back[torch.tensor(order, device=dev)] = torch.arange(len(rows), device=dev)
+        return torch.cat(logits)[back]
 
     def beam_search(self, prompts, beams, steps, eos=2, pad=0):
         """Generates `steps` tokens for every prompt: (sequences int32

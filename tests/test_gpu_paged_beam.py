@@ -260,3 +260,27 @@ def test_prompts_that_cannot_be_read_are_refused(pb, dev):
     assert m.pt.lens.tolist() == [0, 3]
     out, _ = m.beam_search([[1], [2]], 1, 3, pad=-1)
     assert out.shape == (2, 1, 3)
+
+
+def test_prompts_of_more_tokens_than_a_table_has_rows(pb, dev):
+    """8,192 tokens are the rows of one block table: longer prompts, and several
+    that are longer together, go in parts, each of which attends to what the
+    parts before have cached. Against each prompt by itself, fed in two steps
+    of which neither reaches the limit, and the fp32 forward."""
+    cfg = dict(CFG, n_layers=1, dim=64, hidden_dim=64, n_heads=1, n_kv_heads=1)
+    w = pb.PagedLlama.random_weights(cfg, 10, std=0.1)
+    rng = np.random.default_rng(10)
+    prompts = [rng.integers(0, 512, n).tolist() for n in (8193, 3, 8190, 2)]
+    m = pb.PagedLlama(cfg, w, 4, 8200, page_size=16)
+    got = m.prefill(prompts, [1, 0, 3, 2])
+    m.ce.device_status()
+    assert m.pt.lens.tolist() == [3, 8193, 2, 8190]
+    for p, row, logits in zip(prompts, [1, 0, 3, 2], got):
+        f = pb.PagedLlama(cfg, w, 1, 8200, page_size=16)
+        alone = f.prefill([p[:-1]], [0])
+        slots, pos = f.grow(f.pt.lens + 1, 1)
+        alone = f.forward(torch.tensor(p[-1:], device=dev), slots, pos, f.pt)[0]
+        assert all(torch.equal(a, b) for a, b in zip(cached(m, row), cached(f, 0)))
+        assert rel(logits, alone) <= 1e-2
+        if len(p) < 8193:
+            assert rel(logits.cpu(), plain_logits(w, cfg, p)[-1]) <= 1e-2
