@@ -34,10 +34,15 @@
 //     little is spent on padding, accumulators stay in registers beside the
 //     softmax, and the tensor pipe is active 15 to 19% of the time. A tcgen05
 //     tile would have 128 rows of queries to fill from at most 16.
-//   * The softmax keeps a running maximum and sum per query head in fp32. The
-//     weights e^(s - max) enter the second product as two 16-bit parts (the
-//     rounded value and what the rounding lost): rounded once to 16 bits they
-//     would err as much as the output's own rounding.
+//   * The softmax keeps a running reference and sum per query head in fp32.
+//     The weights e^(s - reference) enter the second product as two 16-bit
+//     parts (the rounded value and what the rounding lost): rounded once to 16
+//     bits they would err as much as the output's own rounding. Two bf16 parts
+//     hold 16 bits of any weight. Two f16 parts hold 22 of a large one but end
+//     at 2^-24, so for f16 and E4M3 caches the reference follows the units'
+//     largest scores down as well as up (see the softmax below): it costs
+//     nothing where memory is the bound, up to 2% of the other calls (64
+//     requests of 1,024 tokens, 32 heads of 128, E4M3: 73.6 and 74.9 us).
 //   * A request split over warps or CTAs is joined from (max, sum, O) parts:
 //     within a CTA from shared memory, across CTAs by the last to arrive or,
 //     where parts are many, by a launch of their own; in the order of the
@@ -598,9 +603,16 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
         }
       }
       // ---- softmax: keys of rows g (elements 0, 1) and g + 8 (2, 3), heads 2t, 2t + 1.
-      // The maximum that the weights refer to moves only when a score passes
-      // it by more than 8 (2^8 is far inside both 16-bit types' range), so
-      // that most units need a vote instead of a reduction and a rescaling.
+      // The weights are 2^(s - m) of a reference m near the unit's largest
+      // score. It moves only when that score leaves a window about it, so that
+      // most units need a vote instead of a reduction and a rescaling. For
+      // bf16 parts, with fp32's exponents, the window has an upper end alone.
+      // f16 parts end at 2^-24: weights far below the largest so far (an
+      // attention sink, say) would keep few bits or none. So m follows the
+      // scores down, and a unit's largest weight is between 2^-9 and 2^15.9,
+      // 2^11 where m has been set: what a weight loses below 2^-25 is at most
+      // 2^-16 of the unit's largest. O and l, in fp32, thereby grow to
+      // 2^kRoom at most; from there on m stays.
       if (tail) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -610,25 +622,51 @@ attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUt
             for (int i = 0; i < 4; ++i)
               if (pi + 8 * (i >> 1) + 16 * hf >= n_live) s[nt][hf][i] = -INFINITY;
       }
-      bool grew = false;
+      constexpr float kBelow = BF ? 0.f : 11.f;  // m is set this far below the unit's largest score
+      constexpr float kUp = BF ? 8.f : 15.875f, kDown = -9.f;
+      constexpr int kRoom = 64;
+      auto largest = [&](int nt, int j) {
+        float top = fmaxf(s[nt][0][j], s[nt][0][j + 2]);
+        if constexpr (H == 2) top = fmaxf(top, fmaxf(s[nt][1][j], s[nt][1][j + 2]));
+        return top;
+      };
+      bool moved = false;
+      if constexpr (BF) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = fmaxf(s[nt][0][j], s[nt][0][j + 2]);
-          if constexpr (H == 2) top = fmaxf(top, fmaxf(s[nt][1][j], s[nt][1][j + 2]));
-          grew = grew || top > m[nt][j] + 8.f;
-        }
-      if (__any_sync(0xffffffffu, grew)) {
+          for (int j = 0; j < 2; ++j) moved = moved || largest(nt, j) > m[nt][j] + kUp;
+        moved = __any_sync(0xffffffffu, moved);
+      } else {
+        uint32_t seen = 0;  // a bit per head with a score not too low, and one for a score too high
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(s[nt][0][j], s[nt][0][j + 2]);
-            if constexpr (H == 2) top = fmaxf(top, fmaxf(s[nt][1][j], s[nt][1][j + 2]));
+            const float above = largest(nt, j) - m[nt][j];
+            if (above >= kDown) seen |= 1u << (2 * nt + j);
+            if (above > kUp) seen |= 0x80000000u >> (2 * NT * t);
+          }
+        seen = __reduce_or_sync(0xffffffffu, seen << (2 * NT * t));
+        moved = seen != (1u << (8 * NT)) - 1u;
+      }
+      if (moved) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = largest(nt, j);
 #pragma unroll
             for (int y = 4; y < 32; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-            const float mn = fmaxf(m[nt][j], top);
+            float mn = fmaxf(m[nt][j], top - kBelow);
+            if constexpr (!BF) {
+              float most = l[nt][j];
+#pragma unroll
+              for (int y = 4; y < 32; y <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, y));
+              const int room = kRoom + 126 - (int)(__float_as_uint(most) >> 23);  // most < 2^(kRoom - room)
+              if (top > -INFINITY && top - m[nt][j] < kDown)
+                mn = fmaxf(top - kBelow, m[nt][j] - (float)min(max(room, 0), kRoom));
+            }
             const float f = mn == -INFINITY ? 1.f : exp2_approx(m[nt][j] - mn);
             m[nt][j] = mn;
             l[nt][j] *= f;

@@ -929,7 +929,11 @@ int ce_paged_attention_workspace(size_t *bytes);
  * A request of length 0 gets out = 0, lse = -inf. q and out are
  * [seqs][heads][head_dim] of io_type (the pool's type; for an E4M3 pool
  * CE_TYPE_BF16 or _F16), rows of one request contiguous, requests q_ld /
- * out_ld elements apart (16-byte aligned). Scores, softmax and sums are fp32.
+ * out_ld elements apart (16-byte aligned). Scores, softmax and sums are fp32;
+ * a weight meets the values as the sum of two values of 16 bits (bf16 for a
+ * bf16 pool, else f16), which hold it to 2^-16 of itself or, for f16, of the
+ * largest weight among the 16 or 32 keys about it. A value that is not finite
+ * makes its element of the outputs that attend to it NaN or infinite.
  * Lengths past max_pages * page_size are cut there, pages outside the pool
  * read as zeros; both are reported by ce_device_status (CE_ERR_USAGE). */
 int ce_paged_attention(const ce_paged_kv *kv, int layer, const ce_page_table *pages, void *out_dev,

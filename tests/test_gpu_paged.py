@@ -779,3 +779,98 @@ def test_a_cache_made_during_a_capture_has_no_workspace(ce, dev):
         ce.paged_attention(kv, out, q, pt, workspace=ws)
     g.replay()
     assert torch.equal(out, want)
+
+
+def sink_case(ce, dev, seed, n, kv_heads, group, dim, cache, io, gap, sinks):
+    """Requests of n tokens with keys (`sinks`) that score `gap` nats above
+    all others and have values of 0, so that what the others add is all there
+    is. The first dimension carries the gap, the others a small spread."""
+    rng = np.random.default_rng(seed)
+    page, rows = 16, len(sinks)
+    table, refs = tables(rng, [n] * rows, page)
+    s8 = 16.0 if cache == "e4m3" else 1.0
+    k = torch.from_numpy((rng.standard_normal((1, len(refs), kv_heads, page, dim)) * 0.2 * s8).astype(np.float32))
+    v = torch.from_numpy(((1 + 0.2 * rng.standard_normal(k.shape)) * s8).astype(np.float32))
+    k[..., 0] = 0
+    high = (gap * dim ** 0.5) ** 0.5
+    for i, places in enumerate(sinks):
+        for p in places:
+            k[0, table[i, p // page], :, p % page] = 0
+            k[0, table[i, p // page], :, p % page, 0] = high * s8
+            v[0, table[i, p // page], :, p % page] = 0
+    k, v = k.to(dev).to(DT[cache]), v.to(dev).to(DT[cache])
+    poison(k, table, [n] * rows, page)
+    poison(v, table, [n] * rows, page)
+    ks = vs = None
+    if cache == "e4m3":
+        ks, vs = (torch.full((kv_heads,), 1.0 / 16, device=dev) for _ in "kv")
+    H = kv_heads * group
+    q = torch.from_numpy((rng.standard_normal((rows, H, dim)) * 0.4).astype(np.float32))
+    q[:, :, 0] = high
+    q = q.to(dev).to(DT[io])
+    out, lse = torch.full_like(q, float("nan")), torch.full((rows, H), float("nan"), device=dev)
+    pt = ce.PageTable(torch.from_numpy(table).to(dev), torch.full((rows,), n, dtype=torch.int32, device=dev),
+                      torch.from_numpy(refs).to(dev), page)
+    ce.paged_attention(ce.PagedKV(k, v, ks, vs), out, q, pt, lse=lse)
+    ce.device_status()
+    hk, hv = host(k[0]) / s8, host(v[0]) / s8
+    return host(out), host(lse), host(q), hk, hv, table, page
+
+
+def check_sinks(r, n, group, dim, cache, io, sinks):
+    """Every weight enters the product as two 16-bit parts. In bf16 they hold
+    2^-16 of it; in f16 2^-22 of it and, where it is small, 2^-25. There the
+    largest weight of its unit (16 keys, 32 where a head's row has at most 128
+    bytes) is 2^11 when the reference is set; the sinks leave the window, the
+    others differ by less than e, so 2^9 is the least: 2^-34 of that weight.
+    `extra` adds these up with the values. The rest as in check_attention,
+    with the spread of each key alone: |q k| of the sinks for the sum, of the
+    others for what they add; sums of at most 256 numbers in sequence (a
+    warp's units in two halves and parts, then 12 warps and 148 CTAs), 2^-23
+    each; e^x by 2^x, 2^-18 with its argument's rounding; the output rounded
+    once, in f16 with its least spacing."""
+    out, lse, q, hk, hv, table, page = r
+    unit = 16 if dim > 64 and cache != "e4m3" else 32
+    for i in range(len(sinks)):
+        ids = table[i, :R.pages_of(n, page)]
+        for h in range(q.shape[1]):
+            kk, vv = (x[ids, h // group].reshape(-1, dim)[:n] for x in (hk, hv))
+            s = kk @ q[i, h] * dim ** -0.5
+            mag = np.abs(kk) @ np.abs(q[i, h]) * dim ** -0.5
+            w = np.exp(s - s.max())
+            total = w.sum()
+            want = w @ vv / total
+            other = np.ones(n, bool)
+            other[sinks[i]] = False
+            spread = w @ np.abs(vv) / total
+            starts = np.arange(0, n, unit)
+            top = np.repeat(np.maximum.reduceat(w, starts), np.diff(np.append(starts, n)))
+            assert np.ptp(s[other]) < 1
+            extra = (2.0 ** -16 * spread if cache == "bf16" else
+                     2.0 ** -22 * spread + 2.0 ** -34 * (top @ np.abs(vv)) / total)
+            score = (dim + 16) * 2.0 ** -22 * (mag.max() + mag[other].max()) + 2 * 2.0 ** -18
+            rel = score + 2 * 256 * 2.0 ** -23
+            tol = rel * spread + extra + UNIT[io] * np.abs(want) * (1 + rel) + (2.0 ** -25 if io == "f16" else 0)
+            err = np.abs(out[i, h] - want)
+            assert (err <= tol).all(), (i, h, (err / tol).max(), want[:4], out[i, h, :4])
+            wlse = s.max() + np.log(total)
+            assert abs(lse[i, h] - wlse) <= score + 256 * 2.0 ** -23 + 2.0 ** -22 * abs(wlse)
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+@pytest.mark.parametrize("gap", [12, 18, 30])
+@pytest.mark.parametrize("group,dim", [(2, 64), (3, 128), (12, 128)])
+def test_attention_sinks_in_short_rows(ce, dev, cache, io, gap, group, dim):
+    """First, last, in the middle, several apart, in one unit with others only."""
+    sinks = [[0], [999], [500], [3, 17, 400, 996], [31, 32]]
+    r = sink_case(ce, dev, gap + dim, 1000, 1, group, dim, cache, io, gap, sinks)
+    check_sinks(r, 1000, group, dim, cache, io, sinks)
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+@pytest.mark.parametrize("gap", [15, 18, 40])
+def test_attention_sinks_in_long_rows(ce, dev, cache, io, gap):
+    """Split over all CTAs; far below (e^-40) only the sums' exponents hold the rest."""
+    sinks = [[0], [70001]]
+    r = sink_case(ce, dev, gap, 100003, 1, 2, 64, cache, io, gap, sinks)
+    check_sinks(r, 100003, 2, 64, cache, io, sinks)
