@@ -286,7 +286,9 @@ __device__ __forceinline__ bool slice_of_row(const BeamArgs &a, Shared &sh, int 
     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     if (!(top <= -INFINITY)) {
       float base = fmaxf(top, m), s = sum_exp(e, base);
-      if (!(s <= kElems * 1.001f)) {  // a NaN, +inf, or values so large that their product with log2 e is not finite
+      // a NaN, +inf, or values so large that the rounding of their product with
+      // log2 e is no small number (from 2^30 on its 2^y can be 0 or infinite)
+      if (!(s <= kElems * 1.001f) || fabsf(base) > 1048576.f) {
         top = -INFINITY, s = 0.f;
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {

@@ -182,3 +182,24 @@ def test_select_refuses_a_workspace_that_is_not_on_the_device(ce, dev):
     for bad in (ws.cpu(), torch.zeros(2 * ws.numel(), dtype=torch.uint8, device=dev)[::2]):
         with pytest.raises(TypeError, match="workspace"):
             run(ce, dev, x, scores, finished, ws=bad)
+
+
+def test_very_large_logits(ce, dev):
+    """Where the product of the largest logit and log2 e is rounded by more than
+    the exponents that e^x has (1,580,999,936: by -127), and all the way up to
+    the largest float, of either sign. All others lie further below than e^x
+    reaches, so that the best token's score is its beam's own."""
+    rng = np.random.default_rng(17)
+    B, K, V = 64, 8, 5000
+    x = rng.standard_normal((B * K, V)).astype(np.float32)
+    top = np.exp2(rng.uniform(20, 127.9, B * K)).astype(np.float32)
+    top[:200] = rng.uniform(1.5e9, 2.9e9, 200)
+    top[0], top[1], top[2], top[3] = 1580999936.0, 3.4028234e38, 1048576.0, 1048577.0
+    x[np.arange(B * K), rng.integers(0, V, B * K)] = top
+    for r in range(0, B * K, 3):  # large negative ones
+        x[r] = np.where(x[r] == top[r], -top[r], max(-2.0 * float(top[r]), -3.4e38))
+    scores, finished = -rng.random((B, K)).astype(np.float32), np.zeros((B, K), bool)
+    got = run(ce, dev, torch.from_numpy(x).to(dev), scores, finished)
+    want = R.beam_select(x, scores, finished, 2, 0)
+    assert np.isfinite(got[0]).all()
+    check(got, want, V)
