@@ -519,6 +519,13 @@ int slices_of(int rows, int beams, int vocab, int sms) {
   return std::max(1, std::min(most, (3 * sms + rows - 1) / rows));
 }
 
+// (The outputs of an element are written while other CTAs, of finished beams or
+// other elements, may still have the inputs to read.)
+bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+
 }  // namespace
 }  // namespace paged
 }  // namespace ce
@@ -551,6 +558,13 @@ int ce_beam_select(float *scores_out, int32_t *parents, int32_t *tokens, uint8_t
   CE_REQUIRE(ld >= vocab, "the row stride %lld is shorter than the vocabulary %d", (long long)ld, vocab);
   CE_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= need,
              "the workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need, workspace_bytes);
+  const size_t n = (size_t)batch * beams, row = (size_t)type_bytes(type) * vocab;
+  const std::pair<const void *, size_t> outputs[] = {{scores_out, 4 * n}, {parents, 4 * n}, {tokens, 4 * n}, {finished_out, n}};
+  const std::pair<const void *, size_t> inputs[] = {
+      {scores, 4 * n}, {finished, n}, {logits, (n - 1) * (size_t)type_bytes(type) * ld + row}};
+  for (const auto &o : outputs)
+    for (const auto &i : inputs)
+      CE_REQUIRE(!overlap(o.first, o.second, i.first, i.second), "an output lies over an input");
   const int slices = slices_of(batch * beams, beams, vocab, sm_count());
   const size_t lists = (size_t)batch * beams * slices;
   BeamArgs a = {scores_out, parents, tokens, finished_out, logits, ld, scores, finished, batch, beams, vocab, eos, pad,

@@ -203,3 +203,27 @@ def test_very_large_logits(ce, dev):
     want = R.beam_select(x, scores, finished, 2, 0)
     assert np.isfinite(got[0]).all()
     check(got, want, V)
+
+
+def test_outputs_beside_inputs(ce, dev):
+    """In one allocation, next to each other, they are no overlap; in place they are refused."""
+    rng = np.random.default_rng(18)
+    B, K, V = 3, 4, 100
+    x = torch.from_numpy(rng.standard_normal((B * K, V)).astype(np.float32)).to(dev)
+    scores, finished = -rng.random((B, K)).astype(np.float32), rng.random((B, K)) < 0.3
+    want = run(ce, dev, x, scores, finished)
+    n = B * K
+    words = torch.zeros(3 * n, device=dev)  # scores out, scores, parents' words
+    flags = torch.zeros(2 * n, dtype=torch.bool, device=dev)
+    so, sc, pa = (words[i * n:(i + 1) * n].view(B, K) for i in range(3))
+    fi, fo = flags[:n].view(B, K), flags[n:].view(B, K)
+    sc.copy_(torch.from_numpy(scores))
+    fi.copy_(torch.from_numpy(finished))
+    to = torch.empty(B, K, dtype=torch.int32, device=dev)
+    ws = ce.beam_workspace(B, K, V)
+    ce.beam_select(so, pa.view(torch.int32), to, fo, x, sc, fi, 2, 0, ws)
+    for a, b in zip((so, pa.view(torch.int32), to, fo), want):
+        assert np.array_equal(a.cpu().numpy(), b)
+    for o in ((sc, pa.view(torch.int32), to, fo), (so, pa.view(torch.int32), to, fi), (so, sc.view(torch.int32), to, fo)):
+        with pytest.raises(ce.CeError, match="over an input"):
+            ce.beam_select(*o, x, sc, fi, 2, 0, ws)

@@ -183,3 +183,19 @@ def test_reorder_refuses_too_large_a_page_before_any_launch(ce):
     cache = kv(ce, page_size=1024, kv_heads=1 << 18, head_stride=65536, page_stride=1 << 34, layer_stride=1 << 35)
     refused(ce, ce.lib().ce_paged_reorder(ctypes.byref(other), pt(ce, **table), PTR, 4, cache, PTR, None, None),
             "too large")
+
+
+def test_beam_selection_refuses_outputs_over_inputs(ce):
+    """Scores or flags in place, or one element into the other's memory."""
+    f, n = ce.lib().ce_beam_select, 12  # 3 x 4 beams
+    at = dict(so=0x1000, pa=0x2000, to=0x3000, fo=0x4000, sc=0x5000, fi=0x6000, lg=0x10000, ws=0x80000)
+
+    def call(**change):
+        a = dict(at, **change)
+        return f(a["so"], a["pa"], a["to"], a["fo"], a["lg"], ce.TYPE_F32, 128, a["sc"], a["fi"], 3, 4, 100, 2, 0, a["ws"],
+                 1 << 30, None)
+
+    end = 0x10000 + 4 * (11 * 128 + 100)  # of the logits
+    for change in (dict(so=at["sc"]), dict(so=at["sc"] + 4 * n - 4), dict(so=at["sc"] - 4 * n + 4), dict(fo=at["fi"]),
+                   dict(fo=at["fi"] + n - 1), dict(fi=at["to"] + 3), dict(pa=at["sc"]), dict(to=0x10000), dict(so=end - 4)):
+        refused(ce, call(**change), "over an input")
