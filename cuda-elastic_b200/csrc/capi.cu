@@ -218,15 +218,16 @@ int ce_device_info(int *sms, int *sm100) {
 // Synchronizes the device and returns CE_ERR_TIMEOUT if a bounded device
 // wait of a tensor-core kernel gave up since the last call, CE_ERR_USAGE if a
 // paged operator met a slot, position, page or length out of range (clearing
-// either).
+// either). Waits that gave up come first; they are looked at last, so that the
+// message is theirs, too.
 int ce_device_status(void) {
-  const int a = gemm_status();
-  const int b = gemm_bs_status();
-  const int c = rowx_status();
-  const int d = rows_status();
   const int e = paged_status();
   const int f = paged_attention_status();
-  return a != CE_OK ? a : b != CE_OK ? b : c != CE_OK ? c : d != CE_OK ? d : e != CE_OK ? e : f;
+  const int d = rows_status();
+  const int c = rowx_status();
+  const int b = gemm_bs_status();
+  const int a = gemm_status();
+  return a != CE_OK ? a : b != CE_OK ? b : c != CE_OK ? c : d != CE_OK ? d : f != CE_OK ? f : e;
 }
 
 int ce_set_wait_limit(double seconds) {

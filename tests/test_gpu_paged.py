@@ -874,3 +874,23 @@ def test_attention_sinks_in_long_rows(ce, dev, cache, io, gap):
     sinks = [[0], [70001]]
     r = sink_case(ce, dev, gap, 100003, 1, 2, 64, cache, io, gap, sinks)
     check_sinks(r, 100003, 2, 64, cache, io, sinks)
+
+
+def test_a_wait_that_gave_up_is_reported_before_a_bad_slot(ce, dev):
+    """Both since the last look: the status and the message are the wait's, an
+    exchange with a rank that never came."""
+    x = ce.RowExchange(4, 64, 2, 0)
+    kv = ce.PagedKV(*(torch.zeros(1, 2, 1, 16, 32, dtype=torch.bfloat16, device=dev) for _ in "kv"))
+    try:
+        ce.set_wait_limit(0.05)
+        ce.paged_append(kv, None, None, *(torch.zeros(1, 1, 32, device=dev) for _ in "kv"),
+                        torch.tensor([32], dtype=torch.int64, device=dev))
+        torch.cuda.synchronize()
+        x.wait()
+        with pytest.raises(ce.CeError) as e:
+            ce.device_status()
+        assert e.value.status == ce.ERR_TIMEOUT and "row-shard exchange wait" in str(e.value)
+        ce.device_status()
+    finally:
+        ce.set_wait_limit(2.0)
+        x.close()
