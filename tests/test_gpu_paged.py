@@ -894,3 +894,49 @@ def test_a_wait_that_gave_up_is_reported_before_a_bad_slot(ce, dev):
     finally:
         ce.set_wait_limit(2.0)
         x.close()
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+@pytest.mark.parametrize("kv_heads,group,dim", [(1, 16, 128), (2, 4, 64)])
+@pytest.mark.parametrize("at", [0, 31, 63])
+def test_attention_one_long_row_among_many_short_ones(ce, dev, cache, io, kv_heads, group, dim, at):
+    """Most of the CTAs share one request, the other 63 a few: both joins and
+    rows that no CTA shares, in one call; the long row first, inside, last."""
+    lens = np.random.default_rng(at).integers(1, 300, 64).tolist()
+    lens[at] = 20011
+    r = attention_case(ce, dev, at, lens, kv_heads, group, dim, 16, cache, io, "hnd")
+    check_attention(io, dim, lens, *r[:6])
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_attention_of_rows_that_share_pages(ce, dev, cache, io, layout):
+    """Beams of two prompts: rows that share all pages, all but the last, the
+    prompt's only, and none; the same page twice in one row. Each is what it
+    is with pages of its own, bit for bit, and the oracle's."""
+    page, lens = 16, [70, 70, 75, 48, 33, 130, 130, 160, 20, 64]
+    share = [None, (0, 5), (0, 4), (0, 3), None, None, (5, 9), (5, 8), (4, 1), None]  # (row, leading pages taken over)
+    own = attention_case(ce, dev, 21, lens, 2, 3, 64, page, cache, io, layout)
+    out, lse, _, _, _, _, (kv, pt, q) = own
+    table = pt.table.cpu().numpy().copy()
+    for i, s in enumerate(share):
+        if s is not None:
+            table[i, :s[1]] = table[s[0], :s[1]]
+    table[9, 2] = table[9, 0]
+    # a pool in which every row has copies of these pages to itself
+    k, v, apart = torch.zeros_like(kv.k), torch.zeros_like(kv.v), pt.table.cpu().numpy()
+    for i, n in enumerate(lens):
+        for j in range(R.pages_of(n, page)):
+            k[:, apart[i, j]] = kv.k[:, table[i, j]]
+            v[:, apart[i, j]] = kv.v[:, table[i, j]]
+    # a row's last page may be another's with more tokens in it: what lies past each length stays out
+    ce.paged_attention(ce.PagedKV(k, v, kv.k_scale, kv.v_scale), out, q, pt, lse=lse)
+    pt2 = ce.PageTable(torch.from_numpy(table).to(dev), pt.lens, pt.refs, page)
+    out2, lse2 = torch.full_like(out, float("nan")), torch.full_like(lse, float("nan"))
+    ce.paged_attention(kv, out2, q, pt2, lse=lse2)
+    ce.device_status()
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    hk, hv = host(kv.k[0]), host(kv.v[0])
+    if kv.k_scale is not None:
+        hk, hv = hk * host(kv.k_scale)[None, :, None, None], hv * host(kv.v_scale)[None, :, None, None]
+    check_attention(io, 64, lens, out2, lse2, *R.attention(host(q), hk, hv, table, lens, page, 64 ** -0.5))
