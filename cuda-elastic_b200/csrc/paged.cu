@@ -737,8 +737,8 @@ Tables tables_of(const ce_page_table *to, const ce_page_table *from, int32_t *st
 template <typename In, typename Out, typename Cache>
 int launch_append(const AppendArgs &a, dim3 grid, dim3 block, cudaStream_t s) {
   if constexpr (sizeof(In) == 2) {
-    constexpr long long kWave = 148 * (2048 / kAppendThreads);
-    if (grid.y >= 3 && (long long)grid.x * grid.y > 2 * kWave) {
+    const long long wave = (long long)sm_count() * (2048 / kAppendThreads);
+    if (grid.y >= 3 && (long long)grid.x * grid.y > 2 * wave) {
       grid.y = (grid.y + 2) / 3;
       return launch_kernel(append_kernel<In, Out, Cache, 3>, grid, block, 0, s, true, "append_kernel", a);
     }
