@@ -932,7 +932,8 @@ int ce_paged_attention_workspace(size_t *bytes);
  * out_ld elements apart (16-byte aligned). Scores, softmax and sums are fp32;
  * a weight meets the values as the sum of two values of 16 bits (bf16 for a
  * bf16 pool, else f16), which hold it to 2^-16 of itself or, for f16, of the
- * largest weight among the 16 or 32 keys about it. A value that is not finite
+ * largest weight among the 16 or 32 keys about it (down to 2^-60 of the
+ * request's largest). A value that is not finite
  * makes its element of the outputs that attend to it NaN or infinite.
  * Lengths past max_pages * page_size are cut there, pages outside the pool
  * read as zeros; both are reported by ce_device_status (CE_ERR_USAGE). */
@@ -971,8 +972,9 @@ int ce_beam_select(float *scores_out_dev, int32_t *parents_dev, int32_t *tokens_
  * which the lens % page_size tokens are copied, in all layers of kv (NULL:
  * the tables alone). copies[i] = (from page, to page), or (-1, -1);
  * status[0..3] = pages taken, rows that found no free page (they keep
- * sharing; ce_paged_resize refuses to grow them), pages still free, rows
- * copied. copies is required, status may be NULL. The table buffers of `to`
+ * sharing; ce_paged_resize refuses to grow them), pages still free (not
+ * those that were shared by several groups and lost every row to copies of
+ * this call: they are free for the next), rows copied. copies is required, status may be NULL. The table buffers of `to`
  * and `from` must differ; lens and refs may be the same or others. */
 int ce_paged_reorder(const ce_page_table *to, const ce_page_table *from, const int32_t *parents_dev, int beams,
                      const ce_paged_kv *kv, int32_t *copies_dev, int32_t *status_dev, ce_stream_t stream);

@@ -940,3 +940,45 @@ def test_attention_of_rows_that_share_pages(ce, dev, cache, io, layout):
     if kv.k_scale is not None:
         hk, hv = hk * host(kv.k_scale)[None, :, None, None], hv * host(kv.v_scale)[None, :, None, None]
     check_attention(io, 64, lens, out2, lse2, *R.attention(host(q), hk, hv, table, lens, page, 64 ** -0.5))
+
+
+@pytest.mark.parametrize("cache,io", TYPES)
+def test_attention_of_values_and_keys_that_are_not_finite(ce, dev, cache, io):
+    """A value that is not finite stays in its element of the heads that attend
+    to it, a NaN key in its head; the rest is what it is without, bit for bit."""
+    lens = [100, 700]
+    out, _, _, _, _, _, (kv, pt, q) = attention_case(ce, dev, 23, lens, 2, 3, 64, 16, cache, io, "hnd")
+    bad = 0x7f if cache == "e4m3" else float("inf")  # E4M3 has NaN alone
+    at = int(pt.table[1, 20])
+    x = kv.v.view(torch.uint8) if cache == "e4m3" else kv.v
+    x[0, at, 1, 3, 5] = bad
+    got = torch.empty_like(out)
+    ce.paged_attention(kv, got, q, pt)
+    ce.device_status()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[1, 3:, 5] = True  # the second kv head's query heads
+    assert not torch.isfinite(got[hit].float()).any() and torch.equal(got[~hit], out[~hit])
+    x[0, at, 1, 3, 5] = 0
+    k = kv.k.view(torch.uint8) if cache == "e4m3" else kv.k
+    k[0, at, 0, 3, 5] = 0x7f if cache == "e4m3" else float("nan")
+    ce.paged_attention(kv, got, q, pt)
+    ce.device_status()
+    assert torch.isnan(got[1, :3].float()).all() and torch.equal(got[0], out[0]) and torch.isfinite(got[1, 3:].float()).all()
+
+
+def test_reorder_of_a_last_page_that_two_groups_share(ce, dev):
+    """Every row of both copies it; it is free after the call, but not in its count."""
+    page, beams = 8, 2
+    table, lens = np.array([[0, 1, -1]] * 4, np.int32), np.full(4, 11, np.int32)
+    refs = np.array([4, 4] + [0] * 6, np.int32)
+    args = [torch.from_numpy(x).to(dev) for x in (table, lens, refs)]
+    pt, out = ce.PageTable(*args, page), ce.PageTable(torch.full_like(args[0], -1), args[1], args[2], page)
+    status = torch.zeros(4, dtype=torch.int32, device=dev)
+    parents = np.array([0, 1, 1, 1], np.int32)
+    copies = ce.paged_reorder(pt, torch.from_numpy(parents).to(dev), beams, out, status=status)
+    for g, w in zip((out.table, out.lens, out.refs, copies, status), R.reorder(table, lens, refs, parents, beams, page)):
+        assert np.array_equal(g.cpu().numpy(), w)
+    assert out.refs.tolist() == [4, 0, 1, 1, 1, 1, 0, 0] and status.tolist() == [4, 0, 2, 4]
+    slots, pos = (torch.zeros(32, dtype=t, device=dev) for t in (torch.int64, torch.int32))
+    ce.paged_resize(out, torch.tensor([17, -1, -1, -1], dtype=torch.int32, device=dev), slots, pos, status=status)
+    assert status.tolist() == [1, 0, 2, 6] and out.table[0].tolist() == [0, 2, 1]
