@@ -22,8 +22,8 @@
 // 32 lists), and merges it with its other beams' offers; then the warps'.
 // (Once per rank throughout: 1 x 32 beams over 4,096 tokens 26 us, merged 11.)
 //
-// Measured (B200): 4 beams over 32,000 fp32 logits 6.2 us; 64 x 8 beams 21.4
-// us = 3.1 TB/s of the 65.5 MB; 32 x 32 beams 51 us: a row's CTA spends half
+// Measured (B200): 4 beams over 32,000 fp32 logits 6.3 us; 64 x 8 beams, 15% of
+// them finished and not read, 20.6 us = 2.7 TB/s; 32 x 32 beams 51 us: a row's CTA spends half
 // its time outside the tiles (threshold, ranks, arrival and join), and with
 // three or four rows on an SM that is not all hidden. More slices only
 // multiply it (two 24 us, four 32 us), loads two tiles ahead change nothing.

@@ -13,7 +13,7 @@
 // us; both are chains of dependent reads, barriers and code run once, far
 // from any rate. Reorder of 4 beams, 12 layers 8.3 us, of 128 beams, 32 layers
 // 15 us. Append of 8,190 tokens of 32 + 2 x 8 heads of 128, bf16 into an
-// E4M3 cache, 42 us = 4.5 TB/s; of 64 tokens of 32 + 2 x 32 heads, fp32 into
+// E4M3 cache, 34 us = 5.5 TB/s; of 64 tokens of 32 + 2 x 32 heads, fp32 into
 // bf16, 2.1 us.
 #include <algorithm>
 
@@ -582,8 +582,9 @@ __device__ __forceinline__ void store8(__nv_fp8_e4m3 *p, const float (&x)[8]) {
 // a thread with the divisions, 159 without). The slot and the position are
 // fetched at once, behind the heads: one link less in the chain from the slot
 // to the rotary row is 42 -> 40 us at 8,190 tokens of 32 + 2 x 8 heads of 128,
-// bf16 into E4M3, and three heads for one look-up 34.6 us = 5.4 TB/s. Every
-// element is read and written once.
+// bf16 into E4M3, and three heads for one look-up 34.6 us. Every element is
+// read and written once. Six CTAs of three heads to an SM cost 8 to 20 bytes
+// of spills a thread and are worth it: 33.3 us, 34.2 with five and none.
 constexpr int kAppendThreads = 256;
 template <typename In, typename Out, typename Cache, int Heads>
 __global__ void __launch_bounds__(kAppendThreads, Heads == 1 ? 8 : 6) append_kernel(const __grid_constant__ AppendArgs a) {

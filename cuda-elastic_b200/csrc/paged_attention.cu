@@ -32,8 +32,9 @@
 //     the eight lanes of a phase meet eight different bank groups in both.
 //   * mma.sync (m16n8k16), not tcgen05: with 8 query heads on the narrow side
 //     little is spent on padding, accumulators stay in registers beside the
-//     softmax, and the tensor pipe is active 15 to 19% of the time. A tcgen05
-//     tile would have 128 rows of queries to fill from at most 16.
+//     softmax, and the tensor pipe is active 14% of the time (bf16, one query
+//     head per kv head; E4M3 with five of them 21%). A tcgen05 tile would have
+//     128 rows of queries to fill from at most 16.
 //   * The softmax keeps a running reference and sum per query head in fp32.
 //     The weights e^(s - reference) enter the second product as two 16-bit
 //     parts (the rounded value and what the rounding lost): rounded once to 16
@@ -43,7 +44,7 @@
 //     largest scores down as well as up (see the softmax below): it costs
 //     nothing where memory is the bound, up to 2% of the other calls (64
 //     requests of 1,024 tokens, 32 heads of 128, E4M3: 73.6 and 74.9 us).
-//   * A request split over warps or CTAs is joined from (max, sum, O) parts:
+//   * A request split over warps or CTAs is joined from (reference, sum, O) parts:
 //     within a CTA from shared memory, across CTAs by the last to arrive or,
 //     where parts are many, by a launch of their own; in the order of the
 //     keys, so the result does not depend on who is last.
@@ -51,10 +52,10 @@
 // Measured (B200, measured copy rate 6.45 TB/s): 64 requests of 32 heads of
 // 128, 782 MB of bf16 keys and values, 128 us = 6.1 TB/s; six documents with
 // 8 kv heads of 128, 1.99 GB, 297 us = 6.7 TB/s; 96 requests over an E4M3
-// cache with 3 kv heads of 96, 123 MB, 36.6 us = 3.4 TB/s, where the bound is
+// cache with 3 kv heads of 96, 123 MB, 37.2 us = 3.3 TB/s, where the bound is
 // the chain of instructions per unit (two conversions per four cached bytes,
 // a third of the issue slots used by 10 warps); one request of 512 tokens, 12
-// heads of 64: 8.7 us, of which the lengths and pages take 2, the unit 1.5,
+// heads of 64: 8.9 us, of which the lengths and pages take 2, the unit 1.5,
 // the joins 4.
 #include <algorithm>
 #include <type_traits>
@@ -1061,7 +1062,9 @@ size_t workspace_bytes_of(int grid) {
 
 // Whether the joins across CTAs are a launch of their own. One CTA reads the
 // parts of a request at about 40 bytes a cycle; where few requests share the
-// whole grid these are many. 30,000 tokens, 2 kv heads of 128, one request:
+// whole grid these are many. (Lengths are on the device, so the rule goes by
+// the mean: a long request among many short ones has more parts than it
+// expects and is still joined by the last CTA.) 30,000 tokens, 2 kv heads of 128, one request:
 // 16 query heads each (600 KB of parts a kv head) 41.5 us joined by the last
 // CTA, 20.6 with the launch; 4 heads (150 KB) 17.0 and 14.7; four requests
 // of 4,000 tokens, 2 kv heads of 96, 8 query heads each (55 KB) 15.8 and
